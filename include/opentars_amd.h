@@ -14,7 +14,7 @@
  * golden model's "every check before any write" rule (tars_mini/golden.py:450-472).
  *
  * Results are bit-exact against the golden model's arithmetic (tars_mini/golden.py,
- * tars_mini/numerics.py): exact int32 dot products, then the fp32 epilogue one rounded step at a
+ * tars_mini/numerics.py; the paged cache's attention is outside that contract): exact int32 dot products, then the fp32 epilogue one rounded step at a
  * time (round-to-nearest-even, subnormals flushed on the way in and out, canonical NaN, no FMA).
  * Results never depend on launch geometry.
  */
@@ -293,6 +293,91 @@ int tars_attention_noalloc(const float* const* q, int64_t ldq, const float* cons
                            int64_t ldatt, int32_t out, uint32_t out_scale_bits, float* sc, int64_t ldsc,
                            float* pr, int64_t ldpr, int32_t heads, int32_t M, int32_t nk, int32_t hd,
                            int32_t causal_k, void* stream);
+
+/* ---------------------------------------------------------------- paged key / value cache
+ * A serving cache of 16- or 8-bit K and V rows in pages that many sequences share, and the attention
+ * that reads it. It has no counterpart in the reference, whose attention reads one sequence's dense
+ * fp32 / binary16 rows (tars_attention above), and it is not part of the golden contract: results
+ * are rounded once at the end from fp32 sums whose order is the kernels' own (they do not depend on
+ * the stream, on other calls or on time; which kernel runs depends on the call's sizes).
+ *
+ * A pool holds `pages` pages of `page` positions (a power of two, 16 or more) for kv_heads heads of
+ * hd (64, 128 or 256) elements. K of page i, head h, slot t is the row at
+ * k + i * k_page + h * k_head + t * k_slot (byte strides, multiples of 16, in any order of size that
+ * keeps the rows apart); V likewise. Pointers are 16-byte aligned, offsets 64-bit. dtype BF16 or FP16
+ * is the type of the rows stored and of q; E4M3 (OCP, 448 the largest) takes either, and holds
+ * x / scale with one positive fp32 scale for each head (kscale / vscale, fp32 [kv_heads]; NULL: 1).
+ *
+ * Sequence b of `seqs` has lens[b] positions (device int32, its new rows included); position p is
+ * slot p % page of the page that table[b][p / page] names (device int32 [seqs, table_pages] at
+ * ld_table bytes, 0 = dense; table_pages * page at most 2^30). The call's rows are packed sequence
+ * after sequence: rows starts[b] .. starts[b + 1] - 1 (device int32 [seqs + 1], ascending; row counts
+ * may be 0) are the last ones of sequence b, so row i of its n is at position lens[b] - n + i.
+ * Device arrays are not checked on the host; whatever they hold, nothing outside the call's buffers is
+ * read or written: lens is clamped to [0, table_pages * page], starts to [0, rows], a page number
+ * outside the pool means that its positions hold nothing. */
+#define TARS_KV_BF16  0
+#define TARS_KV_FP16  1
+#define TARS_KV_E4M3  2
+
+typedef struct tars_kv_pool {
+  void* k;
+  void* v;
+  const float* kscale;   /* E4M3 only: fp32 [kv_heads], or NULL for 1 */
+  const float* vscale;
+  int64_t k_page, k_head, k_slot;  /* byte strides */
+  int64_t v_page, v_head, v_slot;
+  int32_t pages;
+  int32_t page;
+  int32_t kv_heads;
+  int32_t hd;
+  int32_t dtype;
+} tars_kv_pool;
+
+/*
+ * Stores the K and V rows ([rows, kv_heads * hd], BF16 or FP16, row strides ldk / ldv bytes, 0 =
+ * dense) of new tokens at their positions; an E4M3 pool gets x / scale rounded to nearest even and
+ * saturated (NaN kept). starts NULL: one row for each sequence (rows == seqs). Rows behind the last
+ * sequence, at negative positions or on pages outside the pool are not stored. No two rows may have
+ * one slot (a table that names a shared page where a sequence writes), and the pools overlap no input.
+ */
+int tars_kv_append(const tars_kv_pool* pool, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                   int32_t dtype, int32_t rows, const int32_t* table, int64_t ld_table,
+                   int32_t table_pages, const int32_t* lens, const int32_t* starts, int32_t seqs,
+                   void* stream);
+
+/* Bytes of device scratch that tars_paged_attention (decode = 0) or tars_paged_decode (decode = 1)
+ * needs for these sizes, for the parts of a sequence whose length is split over workgroups; 0 where
+ * none is (or for sizes the calls refuse). Host only. */
+int64_t tars_paged_workspace(int32_t heads, int32_t kv_heads, int32_t hd, int32_t rows, int32_t seqs,
+                             int32_t table_pages, int32_t page, int32_t decode);
+
+/*
+ * y = softmax(scale q K^T) V for packed rows (prompts, chunks of them, speculative rounds) over the
+ * cache, which holds their own K and V already. The row at position p sees the positions j <= p with
+ * window == 0, j > p - window or j < sinks (first tokens that stay visible). A position that a row
+ * does not see never changes its result, whatever the cache holds there. A row that sees nothing is
+ * 0; rows behind the last sequence are left as they were.
+ *   q [rows, heads * hd] at ldq, BF16 or FP16; query head h reads K / V head h / (heads / kv_heads).
+ *   y [rows, heads * hd] at ldy, out = FP32 or q's type (BF16 / FP16). fp32 scores, maxima and sums;
+ *   the softmax's numerators are rounded to q's type for the product with V.
+ *   scale > 0; work: tars_paged_workspace bytes, 16-byte aligned, for this call until it is done.
+ */
+int tars_paged_attention(const tars_kv_pool* pool, const void* q, int64_t ldq, int32_t dtype,
+                         int32_t heads, int32_t rows, void* y, int64_t ldy, int32_t out, float scale,
+                         int32_t window, int32_t sinks, const int32_t* table, int64_t ld_table,
+                         int32_t table_pages, const int32_t* lens, const int32_t* starts, int32_t seqs,
+                         void* work, int64_t work_bytes, void* stream);
+
+/*
+ * The same for one row per sequence at its last position, lens[b] - 1 (decode): row b of q and y
+ * belongs to sequence b, and a sequence of length 0 (an idle slot) gets a row of zeros.
+ */
+int tars_paged_decode(const tars_kv_pool* pool, const void* q, int64_t ldq, int32_t dtype,
+                      int32_t heads, int32_t seqs, void* y, int64_t ldy, int32_t out, float scale,
+                      int32_t window, int32_t sinks, const int32_t* table, int64_t ld_table,
+                      int32_t table_pages, const int32_t* lens, void* work, int64_t work_bytes,
+                      void* stream);
 
 /* Library version string ("opentars_amd <semver> gfx950"). Host only, never fails. */
 const char* tars_version(void);

@@ -6,7 +6,7 @@ there is no CPU fallback anywhere in the package.
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, c_char_p, c_int, c_int32, c_int64, c_uint32, c_uint64, c_void_p
+from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_uint32, c_uint64, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libopentars_amd.so"
@@ -27,6 +27,14 @@ class W8A8Out(ctypes.Structure):
 class QueueStatus(ctypes.Structure):
     """tars_queue_status: the end state of a descriptor-queue run."""
     _fields_ = [("done", c_int32), ("err_code", c_int32), ("op_idx", c_int32), ("host_op", c_int32)]
+
+
+class KvPool(ctypes.Structure):
+    """tars_kv_pool: the pages of a key / value cache."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("kscale", c_void_p), ("vscale", c_void_p),
+                ("k_page", c_int64), ("k_head", c_int64), ("k_slot", c_int64),
+                ("v_page", c_int64), ("v_head", c_int64), ("v_slot", c_int64),
+                ("pages", c_int32), ("page", c_int32), ("kv_heads", c_int32), ("hd", c_int32), ("dtype", c_int32)]
 
 
 # Every exported entry point: name -> (restype, argtypes)
@@ -73,6 +81,15 @@ SIGNATURES = {
                                        c_int64, c_int32, POINTER(c_void_p), c_int64, c_int32, c_uint32, c_void_p,
                                        c_int64, c_void_p, c_int64, c_int32, c_int32, c_int32, c_int32, c_int32,
                                        c_void_p]),
+    "tars_kv_append": (c_int, [POINTER(KvPool), c_void_p, c_int64, c_void_p, c_int64, c_int32, c_int32, c_void_p, c_int64,
+                               c_int32, c_void_p, c_void_p, c_int32, c_void_p]),
+    "tars_paged_workspace": (c_int64, [c_int32] * 8),
+    "tars_paged_attention": (c_int, [POINTER(KvPool), c_void_p, c_int64, c_int32, c_int32, c_int32, c_void_p, c_int64,
+                                     c_int32, c_float, c_int32, c_int32, c_void_p, c_int64, c_int32, c_void_p, c_void_p,
+                                     c_int32, c_void_p, c_int64, c_void_p]),
+    "tars_paged_decode": (c_int, [POINTER(KvPool), c_void_p, c_int64, c_int32, c_int32, c_int32, c_void_p, c_int64,
+                                  c_int32, c_float, c_int32, c_int32, c_void_p, c_int64, c_int32, c_void_p, c_void_p,
+                                  c_int64, c_void_p]),
 }
 
 _lib: ctypes.CDLL | None = None

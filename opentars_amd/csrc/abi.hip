@@ -142,6 +142,125 @@ float f32_of(uint32_t b) {
   return f;
 }
 
+// ---- the paged key / value cache
+
+constexpr int kMaxPagedRows = 1 << 22, kMaxPositions = 1 << 30, kMaxPagedHeads = 1024;
+
+// Whether n_i items at stride_i (in any order of the three) hold `row` bytes each without sharing a byte; `end` gets
+// the extent.
+bool strides_ok(int64_t row, const int64_t (&n)[3], const int64_t (&stride)[3], int64_t* end) {
+  int at[3] = {0, 1, 2};
+  std::sort(at, at + 3, [&](int i, int j) { return stride[i] < stride[j]; });
+  __int128 extent = row;
+  for (int i : at) {
+    if (n[i] == 1) continue;
+    if (stride[i] < extent) return false;
+    extent += static_cast<__int128>(stride[i]) * (n[i] - 1);
+  }
+  if (extent > INT64_MAX / 2) return false;
+  *end = static_cast<int64_t>(extent);
+  return true;
+}
+
+struct PagedCall {
+  tars::KvPool pool;
+  tars::KvSeqs seqs;
+  Mat k, v;          // the pools' extents
+  Mat meta[5];       // table, lens, starts, scales
+  int nmeta;
+};
+
+// The checks that storing and attention share: the pool, its element type beside the rows', the sequences.
+int check_paged(const tars_kv_pool* p, int32_t dtype, int32_t rows_, const int32_t* table, int64_t ld_table,
+                int32_t table_pages, const int32_t* lens, const int32_t* starts, int32_t seqs, PagedCall& c) {
+  if (!p || !p->k || !p->v || !table || !lens) return fail(TARS_E_ARG, "NULL pointer");
+  if (dtype != TARS_KV_BF16 && dtype != TARS_KV_FP16) return fail(TARS_E_FIELD, "rows are BF16 or FP16");
+  if (p->dtype != dtype && p->dtype != TARS_KV_E4M3) return fail(TARS_E_FIELD, "the pool holds the rows' type or E4M3");
+  if (p->dtype != TARS_KV_E4M3 && (p->kscale || p->vscale)) return fail(TARS_E_FIELD, "scales belong to E4M3 pools");
+  if (p->hd != 64 && p->hd != 128 && p->hd != 256) return fail(TARS_E_FIELD, "hd must be 64, 128 or 256");
+  if (p->page < 16 || (p->page & (p->page - 1)) || p->page > kMaxPositions)
+    return fail(TARS_E_FIELD, "page must be a power of two, 16 or more");
+  if (p->kv_heads < 1 || p->kv_heads > kMaxPagedHeads) return fail(TARS_E_FIELD, "kv_heads must be 1..1024");
+  if (p->pages < 1 || table_pages < 1 || seqs < 1 || rows_ < 1) return fail(TARS_E_ALIGN, "pages, table_pages, seqs, rows >= 1");
+  if (!starts && rows_ != seqs) return fail(TARS_E_FIELD, "without starts every sequence has one row");
+  if (ld_table == 0) ld_table = 4LL * table_pages;
+  if (ld_table < 4LL * table_pages || ld_table % 4) return fail(TARS_E_ALIGN, "table rows: a multiple of 4 bytes holding a row");
+  if (!aligned(table, 4) || !aligned(lens, 4) || !aligned(starts, 4) || !aligned(p->kscale, 4) || !aligned(p->vscale, 4))
+    return fail(TARS_E_ALIGN, "4-byte data must be 4-byte aligned");
+  const int64_t el = p->dtype == TARS_KV_E4M3 ? 1 : 2, row = el * p->hd;
+  const int64_t n[3] = {p->pages, p->kv_heads, p->page};
+  const int64_t ks[3] = {p->k_page, p->k_head, p->k_slot}, vs[3] = {p->v_page, p->v_head, p->v_slot};
+  for (int i = 0; i < 3; ++i)
+    if (ks[i] % 16 || vs[i] % 16) return fail(TARS_E_ALIGN, "pool strides must be multiples of 16");
+  if (!aligned(p->k, 16) || !aligned(p->v, 16)) return fail(TARS_E_ALIGN, "pointers must be 16-byte aligned");
+  int64_t kend, vend;
+  if (!strides_ok(row, n, ks, &kend) || !strides_ok(row, n, vs, &vend))
+    return fail(TARS_E_ALIGN, "pool strides must keep the rows of pages, heads and slots apart");
+  if (rows_ > kMaxPagedRows) return fail(TARS_E_RANGE, "rows must be at most 2^22");
+  if (static_cast<int64_t>(table_pages) * p->page > kMaxPositions)
+    return fail(TARS_E_RANGE, "a table row names at most 2^30 positions");
+  if (!extent_ok(p->k, kend, 1, kend) || !extent_ok(p->v, vend, 1, vend) || !extent_ok(table, ld_table, seqs, 4LL * table_pages))
+    return fail(TARS_E_RANGE, "extent overflows");
+  c.pool = {static_cast<char*>(p->k), static_cast<char*>(p->v), p->kscale, p->vscale, ks[0], ks[1], ks[2],
+            vs[0], vs[1], vs[2], p->pages, __builtin_ctz(p->page), p->kv_heads, p->hd, p->dtype};
+  c.seqs = {table, ld_table / 4, lens, starts, seqs, rows_, table_pages * p->page};
+  c.k = one(p->k, kend);
+  c.v = one(p->v, vend);
+  c.nmeta = 0;
+  c.meta[c.nmeta++] = rows(table, ld_table, seqs, 4LL * table_pages);
+  c.meta[c.nmeta++] = one(lens, 4LL * seqs);
+  if (starts) c.meta[c.nmeta++] = one(starts, 4LL * (seqs + 1LL));
+  if (p->kscale) c.meta[c.nmeta++] = one(p->kscale, 4LL * p->kv_heads);
+  if (p->vscale) c.meta[c.nmeta++] = one(p->vscale, 4LL * p->kv_heads);
+  return TARS_OK;
+}
+
+int check_rows(const void* p, int64_t& ld, int64_t n, int64_t row_bytes) {
+  if (ld == 0) ld = row_bytes;
+  if (ld < row_bytes || ld % 16) return fail(TARS_E_ALIGN, "strides must be multiples of 16 holding a row");
+  if (!aligned(p, 16)) return fail(TARS_E_ALIGN, "pointers must be 16-byte aligned");
+  if (!extent_ok(p, ld, n, row_bytes)) return fail(TARS_E_RANGE, "extent overflows");
+  return TARS_OK;
+}
+
+int paged_attention(const tars_kv_pool* pool, const void* q, int64_t ldq, int32_t dtype, int32_t heads, int32_t rows_,
+                    void* y, int64_t ldy, int32_t out, float scale, int32_t window, int32_t sinks, const int32_t* table,
+                    int64_t ld_table, int32_t table_pages, const int32_t* lens, const int32_t* starts, int32_t seqs,
+                    void* work, int64_t work_bytes, bool decode, void* stream) {
+  g_last_error.clear();
+  if (!q || !y) return fail(TARS_E_ARG, "NULL pointer");
+  PagedCall c;
+  if (int rc = check_paged(pool, dtype, rows_, table, ld_table, table_pages, lens, starts, seqs, c)) return rc;
+  if (heads < 1 || heads > kMaxPagedHeads || heads % pool->kv_heads)
+    return fail(TARS_E_FIELD, "heads must be 1..1024 and a multiple of kv_heads");
+  if (out != TARS_OUT_FP32 && out != (dtype == TARS_KV_BF16 ? TARS_OUT_BF16 : TARS_OUT_FP16))
+    return fail(TARS_E_FIELD, "out must be FP32 or q's type");
+  if (!(scale > 0) || scale > 3.4e38f) return fail(TARS_E_FIELD, "scale must be positive and finite");
+  if (window < 0 || sinks < 0) return fail(TARS_E_FIELD, "window and sinks must not be negative");
+  const int64_t qrow = 2LL * heads * pool->hd, yrow = static_cast<int64_t>(esize(out)) * heads * pool->hd;
+  if (int rc = check_rows(q, ldq, rows_, qrow)) return rc;
+  if (int rc = check_rows(y, ldy, rows_, yrow)) return rc;
+  const int64_t need = tars::paged_workspace(heads, pool->kv_heads, pool->hd, rows_, seqs, c.seqs.cap, decode);
+  if (need > 0 && !work) return fail(TARS_E_ARG, "the call needs a workspace (tars_paged_workspace)");
+  if (need > 0 && !aligned(work, 16)) return fail(TARS_E_ALIGN, "pointers must be 16-byte aligned");
+  if (work_bytes < need) return fail(TARS_E_RANGE, "the workspace is smaller than tars_paged_workspace says");
+  const Mat out_rows = rows(y, ldy, rows_, yrow), in_rows = rows(q, ldq, rows_, qrow);
+  if (overlaps(out_rows, in_rows) || overlaps(out_rows, c.k) || overlaps(out_rows, c.v))
+    return fail(TARS_E_OVERLAP, "the output overlaps an input");
+  for (int i = 0; i < c.nmeta; ++i)
+    if (overlaps(out_rows, c.meta[i])) return fail(TARS_E_OVERLAP, "the output overlaps an input");
+  if (need > 0) {
+    const Mat w = one(work, need);
+    bool hit = overlaps(w, in_rows) || overlaps(w, out_rows) || overlaps(w, c.k) || overlaps(w, c.v);
+    for (int i = 0; i < c.nmeta; ++i) hit = hit || overlaps(w, c.meta[i]);
+    if (hit) return fail(TARS_E_OVERLAP, "the workspace overlaps an input or the output");
+  }
+  tars::PagedAttnArgs a{c.pool, c.seqs, static_cast<const char*>(q), static_cast<char*>(y), ldq, ldy, dtype, heads,
+                        heads / pool->kv_heads, out == TARS_OUT_FP32, scale, window, sinks, static_cast<float*>(work)};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return launched(decode ? tars::launch_paged_decode(a, s) : tars::launch_paged_attention(a, s));
+}
+
 }  // namespace
 
 namespace tars {
@@ -755,6 +874,55 @@ int tars_embed_rows(const uint16_t* table, int64_t ld_table, int64_t table_rows,
     if (int rc = launched(tars::launch_embed_rows(a, s))) return rc;
   }
   return TARS_OK;
+}
+
+int tars_kv_append(const tars_kv_pool* pool, const void* k, int64_t ldk, const void* v, int64_t ldv, int32_t dtype,
+                   int32_t rows_, const int32_t* table, int64_t ld_table, int32_t table_pages, const int32_t* lens,
+                   const int32_t* starts, int32_t seqs, void* stream) {
+  g_last_error.clear();
+  if (!k || !v) return fail(TARS_E_ARG, "NULL pointer");
+  PagedCall c;
+  if (int rc = check_paged(pool, dtype, rows_, table, ld_table, table_pages, lens, starts, seqs, c)) return rc;
+  const int64_t row = 2LL * pool->kv_heads * pool->hd;
+  if (int rc = check_rows(k, ldk, rows_, row)) return rc;
+  if (int rc = check_rows(v, ldv, rows_, row)) return rc;
+  if (pool->k == pool->v) return fail(TARS_E_OVERLAP, "the K and V pools are the same memory");
+  const Mat kin = rows(k, ldk, rows_, row), vin = rows(v, ldv, rows_, row);
+  for (const Mat* m : {&c.k, &c.v}) {
+    bool hit = overlaps(*m, kin) || overlaps(*m, vin);
+    for (int i = 0; i < c.nmeta; ++i) hit = hit || overlaps(*m, c.meta[i]);
+    if (hit) return fail(TARS_E_OVERLAP, "the pool overlaps an input");
+  }
+  const tars::KvAppendArgs a{c.pool, c.seqs, static_cast<const char*>(k), static_cast<const char*>(v), ldk, ldv, dtype};
+  return launched(tars::launch_kv_append(a, static_cast<hipStream_t>(stream)));
+}
+
+int64_t tars_paged_workspace(int32_t heads, int32_t kv_heads, int32_t hd, int32_t rows_, int32_t seqs,
+                             int32_t table_pages, int32_t page, int32_t decode) {
+  if (heads < 1 || kv_heads < 1 || heads % kv_heads || hd < 1 || rows_ < 1 || seqs < 1 || table_pages < 1 || page < 1 ||
+      heads > kMaxPagedHeads || rows_ > kMaxPagedRows || static_cast<int64_t>(table_pages) * page > kMaxPositions)
+    return 0;
+  return tars::paged_workspace(heads, kv_heads, hd, rows_, seqs, table_pages * page, decode != 0);
+}
+
+int tars_paged_attention(const tars_kv_pool* pool, const void* q, int64_t ldq, int32_t dtype, int32_t heads,
+                         int32_t rows_, void* y, int64_t ldy, int32_t out, float scale, int32_t window, int32_t sinks,
+                         const int32_t* table, int64_t ld_table, int32_t table_pages, const int32_t* lens,
+                         const int32_t* starts, int32_t seqs, void* work, int64_t work_bytes, void* stream) {
+  if (!starts) {
+    g_last_error.clear();
+    return fail(TARS_E_ARG, "NULL pointer");
+  }
+  return paged_attention(pool, q, ldq, dtype, heads, rows_, y, ldy, out, scale, window, sinks, table, ld_table, table_pages,
+                         lens, starts, seqs, work, work_bytes, false, stream);
+}
+
+int tars_paged_decode(const tars_kv_pool* pool, const void* q, int64_t ldq, int32_t dtype, int32_t heads, int32_t seqs,
+                      void* y, int64_t ldy, int32_t out, float scale, int32_t window, int32_t sinks,
+                      const int32_t* table, int64_t ld_table, int32_t table_pages, const int32_t* lens, void* work,
+                      int64_t work_bytes, void* stream) {
+  return paged_attention(pool, q, ldq, dtype, heads, seqs, y, ldy, out, scale, window, sinks, table, ld_table, table_pages,
+                         lens, nullptr, seqs, work, work_bytes, true, stream);
 }
 
 }  // extern "C"

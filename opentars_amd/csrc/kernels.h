@@ -390,6 +390,51 @@ struct EmbedArgs {
   int32_t ids[kEmbedMaxIds];
 };
 hipError_t launch_embed_rows(const EmbedArgs& a, hipStream_t s);
+
+// The paged key / value cache (kv_append.hip, paged_attn.hip). A pool's strides are in bytes.
+enum KvType : int { KV_BF16 = 0, KV_FP16 = 1, KV_E4M3 = 2 };
+struct KvPool {
+  char* k;
+  char* v;
+  const float* kscale;  // E4M3: fp32 [kv_heads] (null: 1)
+  const float* vscale;
+  int64_t k_page, k_head, k_slot, v_page, v_head, v_slot;
+  int pages, page_shift, kv_heads, hd, dtype;
+};
+// The sequences of a call: table rows of page numbers (ld_table elements apart), lengths, and the rows of each
+// (starts [seqs + 1]; null: row b belongs to sequence b). cap: positions a table row can name, at most 2^30.
+struct KvSeqs {
+  const int32_t* table;
+  int64_t ld_table;
+  const int32_t* lens;
+  const int32_t* starts;
+  int seqs, rows, cap;
+};
+struct KvAppendArgs {
+  KvPool pool;
+  KvSeqs seqs;
+  const char* k;  // [rows, kv_heads * hd] at ldk bytes
+  const char* v;
+  int64_t ldk, ldv;
+  int dtype;      // KV_BF16 or KV_FP16; the pool's, unless that is KV_E4M3
+};
+hipError_t launch_kv_append(const KvAppendArgs& a, hipStream_t s);
+struct PagedAttnArgs {
+  KvPool pool;
+  KvSeqs seqs;
+  const char* q;  // [rows, heads * hd] at ldq bytes
+  char* y;        // the same shape at ldy bytes, q's type or fp32 (out_f32)
+  int64_t ldq, ldy;
+  int dtype, heads, group, out_f32;  // group: query heads per K / V head
+  float scale;
+  int window, sinks;
+  float* work;    // paged_workspace() bytes
+};
+// Bytes of scratch that a call needs: for the partial results of a sequence split over workgroups.
+int64_t paged_workspace(int heads, int kv_heads, int hd, int rows, int seqs, int cap, bool decode);
+hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t s);
+hipError_t launch_paged_decode(const PagedAttnArgs& a, hipStream_t s);
+
 hipError_t launch_attention(const AttnArgs& a, hipStream_t s);
 // Prompt rows (attn_rows.hip): 16 query rows of a head per workgroup; the arguments of launch_attention
 // (no scratch, no norm + RoPE prologue).

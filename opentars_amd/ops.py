@@ -17,6 +17,13 @@ bit-identical to the golden model (tars_mini/golden.py, tars_mini/numerics.py):
   fdot_nt(a, b) / fdot_nn(a, b)          Machine._fdot                  numerics.py:393-409
   embed_rows(table, ids, scale)          the runtime's embedding lookup tars_board.py:298-314
 
+and, outside the golden model and its bit-exactness, a serving cache in pages:
+
+  PagedCache(k, v, kscale, vscale)       the pool: pages of 16- or 8-bit K and V rows
+  kv_append(cache, k, v, table, lens)    new tokens' K and V rows into their pages
+  paged_attention(cache, q, ..., starts) prompts' rows over the cache: causal, sliding window, first tokens
+  paged_decode(cache, q, table, lens)    one row per sequence over the cache
+
 Inputs are torch tensors on the GPU (results stay there, stream-ordered on the current stream),
 or numpy arrays (copied in; results come back as numpy after a synchronize, which is what
 golden-style callers expect). 2-D operands may be row-strided views whose rows are contiguous.
@@ -509,6 +516,144 @@ def embed_rows(table, ids, scale=None, y=None):
     return _finish(nm, y)
 
 
+# ---------------------------------------------------------------- paged key / value cache
+_KV_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.int16: 1, torch.float8_e4m3fn: 2}
+_KV_OUT = {0: OUT_BF16, 1: OUT_FP16}
+
+
+class PagedCache:
+    """The pool of a paged key / value cache: k and v are GPU tensors [pages, kv_heads, page, hd], page a power of two
+    of 16 or more, hd 64, 128 or 256, bf16, fp16 (float16, or int16 bits) or float8_e4m3fn; each row of hd elements
+    contiguous, the other strides free (a [pages, page, kv_heads, hd] tensor's transpose(1, 2), or k and v cut from
+    one tensor). kscale / vscale: fp32 [kv_heads], positive, what an e4m3 value is multiplied by (1 without them).
+    Made once with the pool; every call takes it. It keeps the tensors alive and holds nothing else."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, kscale: torch.Tensor | None = None,
+                 vscale: torch.Tensor | None = None):
+        if not (k.is_cuda and v.is_cuda) or k.device != v.device:
+            raise ValueError("k and v must live on one GPU")
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _KV_DTYPES:
+            raise ValueError("k and v must be [pages, kv_heads, page, hd], both bf16, fp16 or e4m3")
+        if k.numel() == 0 or (k.shape[3] > 1 and (k.stride(3) != 1 or v.stride(3) != 1)):
+            raise ValueError("k and v must not be empty and their rows contiguous")
+        pages, kv_heads, page, hd = k.shape
+        for t, what in ((kscale, "kscale"), (vscale, "vscale")):
+            if t is not None:
+                if t.dtype != torch.float32 or t.device != k.device:
+                    raise ValueError(f"{what} must be fp32 on the pool's GPU")
+                _vec(t, kv_heads, what)
+        self.k, self.v, self.kscale, self.vscale = k, v, kscale, vscale
+        self.device, self.index = k.device, k.get_device()
+        self.kv_heads, self.page, self.hd, self.dtype = kv_heads, page, hd, _KV_DTYPES[k.dtype]
+        el = k.element_size()
+        self._pool = _lib.KvPool(k.data_ptr(), v.data_ptr(), _ptr(kscale), _ptr(vscale), *(el * s for s in k.stride()[:3]),
+                                 *(el * s for s in v.stride()[:3]), pages, page, kv_heads, hd, self.dtype)
+        self._ref = ctypes.byref(self._pool)
+
+
+def _paged_rows(cache: PagedCache, t: torch.Tensor, what: str) -> int:
+    """The element code of a call's packed rows, which must lie on the cache's GPU, the current one."""
+    code = _KV_DTYPES.get(t.dtype)
+    if code is None or code == 2:
+        raise ValueError(f"{what} must be bf16 or fp16")
+    if t.get_device() != cache.index or cache.index != torch.cuda.current_device():
+        raise ValueError(f"{what} must live on the cache's GPU, and that must be the current device")
+    return code
+
+
+def _paged_meta(cache: PagedCache, table: torch.Tensor, lens: torch.Tensor, starts: torch.Tensor | None):
+    seqs = lens.shape[0]
+    if table.dtype != torch.int32 or lens.dtype != torch.int32 or (starts is not None and starts.dtype != torch.int32):
+        raise ValueError("table, lens and starts must be int32")
+    if table.get_device() != cache.index or lens.get_device() != cache.index or (
+            starts is not None and starts.get_device() != cache.index):
+        raise ValueError("table, lens and starts must live on the cache's GPU")
+    _vec(lens, seqs, "lens")
+    if starts is not None:
+        _vec(starts, seqs + 1, "starts")
+    if table.shape[0] != seqs:
+        raise ValueError("table must have a row for each sequence")
+    return table.data_ptr(), _ld(table), table.shape[1], lens.data_ptr(), _ptr(starts), seqs
+
+
+def kv_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+              starts: torch.Tensor | None = None) -> None:
+    """Stores new tokens' K and V rows ([rows, kv_heads * hd], bf16 or fp16, the pool's type unless it is e4m3) in the
+    pages of their sequences. lens int32 [seqs]: each sequence's length with its new rows; table int32
+    [seqs, table_pages]: its page numbers; starts int32 [seqs + 1]: its rows are starts[b] .. starts[b + 1] - 1, its
+    last positions (without it, one row per sequence). Rows behind the last sequence, at negative positions (an idle
+    slot's, length 0) or on pages outside the pool are not stored. No rows: nothing is done."""
+    code = _paged_rows(cache, k, "k")
+    if _paged_rows(cache, v, "v") != code or k.shape != v.shape:
+        raise ValueError("k and v must have one shape and type")
+    ldk, ldv = _ld(k), _ld(v)
+    if k.shape[1] != cache.kv_heads * cache.hd:
+        raise ValueError("k and v must be [rows, kv_heads * hd]")
+    meta = _paged_meta(cache, table, lens, starts)
+    if k.shape[0] == 0 or (starts is not None and meta[5] == 0):
+        return
+    _check(_lib.lib().tars_kv_append(cache._ref, k.data_ptr(), ldk, v.data_ptr(), ldv, code, k.shape[0], *meta, _stream()))
+
+
+def _paged(cache: PagedCache, q: torch.Tensor, table, lens, starts, scale, window: int, sinks: int, out, y):
+    code = _paged_rows(cache, q, "q")
+    ldq = _ld(q)
+    rows, cols = q.shape
+    hd = cache.hd
+    heads = cols // hd
+    if heads * hd != cols or heads < 1 or heads % cache.kv_heads:
+        raise ValueError("q must be [rows, heads * hd], heads a multiple of kv_heads")
+    meta = _paged_meta(cache, table, lens, starts)
+    seqs = meta[5]
+    if starts is None and rows != seqs:
+        raise ValueError("q must have a row for each sequence")
+    if y is None:
+        if out is None:
+            out = _KV_OUT[code]
+        dtype = torch.float32 if out == OUT_FP32 else q.dtype
+        y = (torch.zeros if starts is not None else torch.empty)((rows, cols), dtype=dtype, device=q.device)
+    else:
+        if y.shape != q.shape or y.get_device() != cache.index or (y.dtype != torch.float32 and _KV_DTYPES.get(y.dtype) != code):
+            raise ValueError("y must have q's shape and place, fp32 or q's type")
+        is_f32 = y.dtype == torch.float32
+        if out is None:
+            out = OUT_FP32 if is_f32 else _KV_OUT[code]
+        elif is_f32 != (out == OUT_FP32):
+            raise ValueError("y must have the type that out names")
+    if rows == 0 or seqs == 0:
+        return y
+    lib = _lib.lib()
+    need = lib.tars_paged_workspace(heads, cache.kv_heads, hd, rows, seqs, meta[2], cache.page, starts is None)
+    work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    args = (cache._ref, q.data_ptr(), ldq, code, heads, rows, y.data_ptr(), _ld(y), out,
+            hd ** -0.5 if scale is None else scale, window, sinks, *meta[:4])
+    if starts is None:
+        _check(lib.tars_paged_decode(*args, _ptr(work), need, _stream()))
+    else:
+        _check(lib.tars_paged_attention(*args, meta[4], seqs, _ptr(work), need, _stream()))
+    return y
+
+
+def paged_attention(cache: PagedCache, q: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, starts: torch.Tensor,
+                    scale: float | None = None, window: int = 0, sinks: int = 0, out: int | None = None,
+                    y: torch.Tensor | None = None) -> torch.Tensor:
+    """y = softmax(scale q K^T) V for the packed rows of prompts, chunks of them or speculative rounds over the cache,
+    which holds their own K and V already (kv_append first). q [rows, heads * hd], bf16 or fp16; query head h reads
+    K / V head h // (heads // kv_heads). table, lens and starts as kv_append's: row i of a sequence's n is at position
+    lens - n + i and sees the positions up to its own, with a window w > 0 only its last w (its own among them) and
+    the first `sinks`. scale: 1 / sqrt(hd) unless given. y in q's type, or fp32 with out=OUT_FP32 (or as the given y);
+    a row that sees nothing is 0. Rows behind the last sequence stay as they were in a given y (0 without one)."""
+    return _paged(cache, q, table, lens, starts, scale, window, sinks, out, y)
+
+
+def paged_decode(cache: PagedCache, q: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+                 scale: float | None = None, window: int = 0, sinks: int = 0, out: int | None = None,
+                 y: torch.Tensor | None = None) -> torch.Tensor:
+    """paged_attention for one row per sequence at its last position: row b of q [seqs, heads * hd] is sequence b's. An
+    idle slot (length 0) gets zeros."""
+    return _paged(cache, q, table, lens, None, scale, window, sinks, out, y)
+
+
 def set_w8a8_path(path: str) -> str:
     """'auto' | 'gemv' | 'mfma': which W8A8 kernel family runs for M >= 2 (and M = 1). Returns the
     previous setting."""
@@ -518,7 +663,8 @@ def set_w8a8_path(path: str) -> str:
 
 
 __all__ = ["TarsError", "ContractError", "quant_rows", "gemm_rowcol", "quant_gemm_rowcol", "gemm_rowcol_ksplit",
-           "align_w4_groups", "gemm_w4", "embed_rows", "attention", "set_w8a8_path", "ESIZE", "softmax_rows", "softmax_rows_causal",
+           "align_w4_groups", "gemm_w4", "embed_rows", "attention",
+           "PagedCache", "kv_append", "paged_attention", "paged_decode", "set_w8a8_path", "ESIZE", "softmax_rows", "softmax_rows_causal",
            "layernorm_rows", "rmsnorm_rows", "l2norm_rows", "relu", "elt", "rope_rows", "fdot_nt", "fdot_nn",
            "ROW_SOFTMAX", "ROW_LAYERNORM", "ROW_RMSNORM", "ROW_L2NORM", "ELT_MUL", "ELT_ADD", "ELT_MULADD",
            "ELT_SUB", "BM_DENSE", "BM_ROW", "BM_COL", "BM_SCALAR"]
