@@ -144,7 +144,8 @@ float f32_of(uint32_t b) {
 
 // ---- the paged key / value cache
 
-constexpr int kMaxPagedRows = 1 << 22, kMaxPositions = 1 << 30, kMaxPagedHeads = 1024;
+constexpr int kMaxPagedRows = 1 << 22, kMaxPositions = 1 << 30, kMaxPagedHeads = 1024, kMaxPagedSeqs = 65535;
+constexpr int64_t kMaxSlotBytes = 1 << 26, kMaxSeqHeads = 1 << 23;
 
 // Whether n_i items at stride_i (in any order of the three) hold `row` bytes each without sharing a byte; `end` gets
 // the extent.
@@ -196,7 +197,9 @@ int check_paged(const tars_kv_pool* p, int32_t dtype, int32_t rows_, const int32
   int64_t kend, vend;
   if (!strides_ok(row, n, ks, &kend) || !strides_ok(row, n, vs, &vend))
     return fail(TARS_E_ALIGN, "pool strides must keep the rows of pages, heads and slots apart");
-  if (rows_ > kMaxPagedRows) return fail(TARS_E_RANGE, "rows must be at most 2^22");
+  if (rows_ > kMaxPagedRows || seqs > kMaxPagedSeqs) return fail(TARS_E_RANGE, "at most 2^22 rows and 65535 sequences");
+  if (ks[2] > kMaxSlotBytes || vs[2] > kMaxSlotBytes)
+    return fail(TARS_E_RANGE, "slots must be at most 2^26 bytes apart");
   if (static_cast<int64_t>(table_pages) * p->page > kMaxPositions)
     return fail(TARS_E_RANGE, "a table row names at most 2^30 positions");
   if (!extent_ok(p->k, kend, 1, kend) || !extent_ok(p->v, vend, 1, vend) || !extent_ok(table, ld_table, seqs, 4LL * table_pages))
@@ -233,6 +236,7 @@ int paged_attention(const tars_kv_pool* pool, const void* q, int64_t ldq, int32_
   if (int rc = check_paged(pool, dtype, rows_, table, ld_table, table_pages, lens, starts, seqs, c)) return rc;
   if (heads < 1 || heads > kMaxPagedHeads || heads % pool->kv_heads)
     return fail(TARS_E_FIELD, "heads must be 1..1024 and a multiple of kv_heads");
+  if (static_cast<int64_t>(seqs) * heads > kMaxSeqHeads) return fail(TARS_E_RANGE, "seqs * heads must be at most 2^23");
   if (out != TARS_OUT_FP32 && out != (dtype == TARS_KV_BF16 ? TARS_OUT_BF16 : TARS_OUT_FP16))
     return fail(TARS_E_FIELD, "out must be FP32 or q's type");
   if (!(scale > 0) || scale > 3.4e38f) return fail(TARS_E_FIELD, "scale must be positive and finite");
@@ -900,7 +904,8 @@ int tars_kv_append(const tars_kv_pool* pool, const void* k, int64_t ldk, const v
 int64_t tars_paged_workspace(int32_t heads, int32_t kv_heads, int32_t hd, int32_t rows_, int32_t seqs,
                              int32_t table_pages, int32_t page, int32_t decode) {
   if (heads < 1 || kv_heads < 1 || heads % kv_heads || hd < 1 || rows_ < 1 || seqs < 1 || table_pages < 1 || page < 1 ||
-      heads > kMaxPagedHeads || rows_ > kMaxPagedRows || static_cast<int64_t>(table_pages) * page > kMaxPositions)
+      heads > kMaxPagedHeads || rows_ > kMaxPagedRows || seqs > kMaxPagedSeqs ||
+      static_cast<int64_t>(seqs) * heads > kMaxSeqHeads || static_cast<int64_t>(table_pages) * page > kMaxPositions)
     return 0;
   return tars::paged_workspace(heads, kv_heads, hd, rows_, seqs, table_pages * page, decode != 0);
 }

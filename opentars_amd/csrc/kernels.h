@@ -432,6 +432,7 @@ struct PagedAttnArgs {
 };
 // Bytes of scratch that a call needs: for the partial results of a sequence split over workgroups.
 int64_t paged_workspace(int heads, int kv_heads, int hd, int rows, int seqs, int cap, bool decode);
+int64_t paged_decode_workspace(int heads, int kv_heads, int hd, int seqs, int cap);
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t s);
 hipError_t launch_paged_decode(const PagedAttnArgs& a, hipStream_t s);
 

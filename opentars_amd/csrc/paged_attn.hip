@@ -99,13 +99,14 @@ hipError_t go(const PagedAttnArgs& a, hipStream_t s) {
 
 }  // namespace
 
-int64_t paged_workspace(int, int, int, int, int, int, bool) { return 0; }
+int64_t paged_workspace(int heads, int kv_heads, int hd, int, int seqs, int cap, bool decode) {
+  return decode ? paged_decode_workspace(heads, kv_heads, hd, seqs, cap) : 0;
+}
 
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t s) {
   const bool e4m3 = a.pool.dtype == KV_E4M3;
   if (a.dtype == KV_BF16) return e4m3 ? go<Bf16, true>(a, s) : go<Bf16, false>(a, s);
   return e4m3 ? go<Fp16, true>(a, s) : go<Fp16, false>(a, s);
 }
-hipError_t launch_paged_decode(const PagedAttnArgs& a, hipStream_t s) { return launch_paged_attention(a, s); }
 
 }  // namespace tars

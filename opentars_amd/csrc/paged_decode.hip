@@ -1,0 +1,479 @@
+// Attention of one row per sequence over the paged cache, split over the caches' lengths and joined.
+//
+// Per sequence and K / V head the cache is read once for all the query heads that share it, 32 positions a step. Both
+// products run on matrix instructions with the positions as rows, so that nothing passes through LDS on the way:
+//   S^T = K Q^T   16 positions x 16 heads: lane l loads row l % 16 of K, 16 bytes of it, as the instruction wants it;
+//   O^T += V^T P^T  lane l loads the rows of V at the very positions whose scores it holds (16 t + 4 (l / 16) + i of
+//                 the step), hd / 16 columns of each: its block of 8 positions x hd / 16 columns, turned over by
+//                 v_perm_b32 in its own registers, is V^T's operand for hd / 16 products, and its 8 numerators, in
+//                 the order they left the softmax, are P^T's.
+// The order of a product's inner index is free as long as both operands use it, which is all this needs. A numerator
+// goes in as the sum of two values of q's type (its rounding and what that left), two products instead of one: next to
+// the loads they are free, and the result is rounded once, at the end.
+//
+// The running maximum is kept per head; accumulators are rescaled only when it grows, which after a few steps is rare.
+// Positions that the row does not see get a numerator of 0 and zeros for V (which may hold anything there). Only steps
+// at the end of the cache, at the window's edges or with a page number outside the pool pay for that.
+//
+// The split is made on the device from the lengths: every workgroup adds up the steps of all sequences, sets the share
+// C of a workgroup so that the shares fill the GPU, and finds its own (sequence, part) in the prefix sums. So one long
+// cache fills the GPU as well as many short ones, whatever the batch's longest is. A sequence of one part is written
+// at once; the parts of the others go to the workspace as (maximum, sum, unscaled output) in fp32 and a second launch
+// joins them in order.
+#include <algorithm>
+
+#include "paged_device.h"
+
+namespace tars {
+namespace {
+
+constexpr int kStep = 32;        // positions a wave takes at a time
+constexpr int kWaves = 4;
+constexpr int kHeads = 16;       // query heads of a workgroup
+constexpr int kSlots = 1024;     // workgroups that the work is dealt to
+constexpr int kMinShare = 8;     // steps that a part holds at least
+
+// The sequences' steps dealt to workgroups: `slots` shares for each K / V head (and head tile).
+struct Deal {
+  int slots, min_share;
+};
+struct Part {
+  int b, part, parts, first;     // the sequence, its part's number and count, the number of its first part among all
+  int len;
+  Steps steps;
+};
+
+__device__ __forceinline__ Steps steps_of(int len, int window, int sinks) {
+  return visible_steps(len - 1, len - 1, len, window, sinks, kStep);
+}
+
+// The share C of a workgroup, the same in every wave.
+__device__ __forceinline__ int share(const KvSeqs& s, int window, int sinks, const Deal& deal) {
+  const int lane = threadIdx.x & 63;
+  uint64_t mine = 0;
+  for (int b = lane; b < s.seqs; b += 64) mine += steps_of(seq_len(s.lens, b, s.cap), window, sinks).n();
+  const uint64_t lo = group_sum<64>(static_cast<int>(mine & 0xFFFFFF)), hi = group_sum<64>(static_cast<int>(mine >> 24));
+  const uint64_t total = lo + (hi << 24);
+  // in units of 2^16 steps where the sum has more than 31 bits (a share too long is no harm)
+  const int up = total < (1ull << 31) ? 0 : 16;
+  const uint32_t units = static_cast<uint32_t>((total + (1ull << up) - 1) >> up), slots = deal.slots;
+  const uint32_t c = min((units + slots - 1) / slots, 1u << 25 >> up) << up;  // no sequence has more than 2^25
+  return max(static_cast<int>(c), deal.min_share);
+}
+
+__device__ __forceinline__ int parts_of(int n, int c) { return max((n + c - 1) / c, 1); }
+
+__device__ __forceinline__ int inclusive_sum(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast 15 to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast 31 to rows 2 and 3
+  return x;
+}
+
+// The part numbered idx among all (b < 0: none), or, with idx < 0, part 0 of sequence `seq`.
+__device__ __forceinline__ Part find_part(const KvSeqs& s, int window, int sinks, int c, int idx, int seq) {
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int b0 = 0; b0 < s.seqs; b0 += 64) {
+    const int b = b0 + lane;
+    const int len = b < s.seqs ? seq_len(s.lens, b, s.cap) : 0;
+    const int parts = b < s.seqs ? parts_of(steps_of(len, window, sinks).n(), c) : 0;
+    const int upto = before + inclusive_sum(parts);
+    const uint64_t hit = __ballot(idx >= 0 ? upto > idx : b >= seq);
+    if (hit) {
+      const int at = __builtin_ctzll(hit);
+      Part p;
+      p.b = b0 + at;
+      p.len = __builtin_amdgcn_readlane(len, at);
+      p.parts = __builtin_amdgcn_readlane(parts, at);
+      p.first = __builtin_amdgcn_readlane(upto, at) - p.parts;
+      p.part = idx >= 0 ? idx - p.first : 0;
+      p.steps = steps_of(p.len, window, sinks);
+      return p;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+  return {-1, 0, 0, 0, 0, {}};
+}
+
+__device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
+
+template <class T>
+__device__ __forceinline__ v4f mfma16(const uint32_t (&a)[4], const uint32_t (&b)[4], v4f c) {
+  const uint4 x = make_uint4(a[0], a[1], a[2], a[3]), y = make_uint4(b[0], b[1], b[2], b[3]);
+  return T::mfma_16x16x32(x, y, c);
+}
+
+// N dwords from global memory: a scalar base and a lane offset.
+template <int N>
+__device__ __forceinline__ void load_dwords(uint32_t (&d)[N], const char* base, uint32_t off) {
+  if constexpr (N == 1) {
+    d[0] = *reinterpret_cast<const uint32_t*>(base + off);
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(base + off);
+    d[0] = v.x;
+    d[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(base + off + 4 * i);
+      d[i] = v.x;
+      d[i + 1] = v.y;
+      d[i + 2] = v.z;
+      d[i + 3] = v.w;
+    }
+  }
+}
+
+__device__ __forceinline__ float max_over_groups(float x) {  // over lanes l % 16
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_over_groups(float x) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// The two pages of a step and whether they are in the pool (bit t), the same in every lane.
+struct Pages {
+  int page[2];
+  int ok;
+};
+
+template <class T, bool E4M3, int D>
+__global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_kernel(PagedAttnArgs a, Deal deal, int head_tiles) {
+  constexpr int KS = D / 32;                        // products of a scores tile
+  constexpr int E = D / 16;                         // columns of V per lane
+  constexpr int KW = E4M3 ? 4 * KS / 2 : 4 * KS;    // dwords of a lane's K row part
+  constexpr int VW = E4M3 ? E / 4 : E / 2;          // dwords of a lane's V row part
+  constexpr int kPad = D + 4;
+  __shared__ __attribute__((aligned(16))) float os[kWaves][kHeads][kPad];
+  __shared__ float ms[kWaves][kHeads], ls[kWaves][kHeads];
+  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = share(a.seqs, a.window, a.sinks, deal);
+  const int columns = a.pool.kv_heads * head_tiles, number = blockIdx.x / columns, column = blockIdx.x % columns;
+  const Part part = find_part(a.seqs, a.window, a.sinks, c, number, 0);
+  if (part.b < 0) return;
+  const int h = column / head_tiles, tile = column % head_tiles;
+  const int heads = min(a.group - tile * kHeads, kHeads);   // of this workgroup
+  const int head0 = h * a.group + tile * kHeads;
+  const int n = part.steps.n(), per = (n + part.parts - 1) / part.parts;
+  const int t0 = part.part * per, t1 = min(n, t0 + per);
+  const int lo = a.window == 0 ? 0 : max(part.len - a.window, 0);
+
+  // Q^T: column = head. Heads of 256 keep it in LDS (every wave's own copy, 16 bytes of a lane at a time), where the
+  // registers are needed for K and V.
+  constexpr bool kQLds = D == 256;
+  uint32_t qf[kQLds ? 1 : KS][4];
+  const char* q = a.q + part.b * a.ldq + 2 * D * (head0 + min(col, heads - 1));
+  char* qs = reinterpret_cast<char*>(os[wave]) + 16 * lane;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    load_dwords<4>(qf[kQLds ? 0 : s], q, E4M3 ? 128 * (s / 2) + 16 * (s % 2) + 32 * g : 64 * s + 16 * g);
+    if constexpr (kQLds) *reinterpret_cast<uint4*>(qs + 1024 * s) = make_uint4(qf[0][0], qf[0][1], qf[0][2], qf[0][3]);
+  }
+  const float sc = a.scale * 1.44269504f * (E4M3 && a.pool.kscale ? a.pool.kscale[h] : 1.0f);
+
+  const int shift = a.pool.page_shift, mask = (1 << shift) - 1, last = (part.len - 1) >> shift;
+  const __attribute__((address_space(4))) int32_t* table = reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(
+      reinterpret_cast<uintptr_t>(a.seqs.table + part.b * a.seqs.ld_table));
+  const uint32_t koff = col * static_cast<uint32_t>(a.pool.k_slot) + 16 * g;
+  const uint32_t voff = 4 * g * static_cast<uint32_t>(a.pool.v_slot) + 4 * VW * col;
+  const char* kbase = a.pool.k + h * a.pool.k_head;
+  const char* vbase = a.pool.v + h * a.pool.v_head;
+  auto pages_of = [&](int i) {
+    const int k0 = part.steps.at(i) * kStep;
+    Pages p;
+    p.page[0] = table[min(k0 >> shift, last)];
+    p.page[1] = table[min((k0 + 16) >> shift, last)];
+    return p;
+  };
+  auto check = [&](Pages& p) {
+    p.ok = 0;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const bool in = static_cast<uint32_t>(p.page[t]) < static_cast<uint32_t>(a.pool.pages);
+      p.ok |= in << t;
+      p.page[t] = in ? p.page[t] : 0;
+    }
+  };
+  uint32_t kf[2][KW], vf[8][VW];
+  auto load_k = [&](int i, const Pages& p) {
+    const int k0 = part.steps.at(i) * kStep;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const char* base = kbase + p.page[t] * a.pool.k_page + ((k0 + 16 * t) & mask) * a.pool.k_slot;
+#pragma unroll
+      for (int s = 0; s < KW / 4; ++s)
+        load_dwords<4>(reinterpret_cast<uint32_t(&)[4]>(kf[t][4 * s]), base, koff + 64 * s);
+    }
+  };
+  auto load_v = [&](int i, const Pages& p) {
+    const int k0 = part.steps.at(i) * kStep;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const char* base = vbase + p.page[t] * a.pool.v_page + ((k0 + 16 * t) & mask) * a.pool.v_slot;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) load_dwords<VW>(vf[4 * t + j], base + j * a.pool.v_slot, voff);
+    }
+  };
+
+  float m = -INFINITY, l = 0;
+  v4f o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = v4f{0, 0, 0, 0};
+
+  Pages cur, next;
+  auto step = [&](int i, bool more) __attribute__((always_inline)) {
+    const int k0 = part.steps.at(i) * kStep;
+    v4f s[2] = {v4f{0, 0, 0, 0}, v4f{0, 0, 0, 0}};
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        uint32_t f[4];
+        if constexpr (E4M3) {
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const uint32_t x = kf[t][4 * (k / 2) + 2 * (k % 2) + w];
+            f[2 * w] = T::template from_e4m3<false>(x);
+            f[2 * w + 1] = T::template from_e4m3<true>(x);
+          }
+        } else {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) f[w] = kf[t][4 * k + w];
+        }
+        if constexpr (kQLds) {
+          const uint4 v = *reinterpret_cast<const uint4*>(qs + 1024 * k);
+          const uint32_t qk[4] = {v.x, v.y, v.z, v.w};
+          s[t] = mfma16<T>(f, qk, s[t]);
+        } else {
+          s[t] = mfma16<T>(f, qf[k], s[t]);
+        }
+      }
+    if (more) load_k(i + kWaves, next);
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = s[j >> 2][j & 3] * sc;
+    const bool whole = k0 + kStep <= part.len && (k0 >= lo || k0 + kStep <= a.sinks) && cur.ok == 3;
+    if (!whole) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int p = k0 + 16 * (j >> 2) + 4 * g + (j & 3);
+        const bool seen = p < part.len && (p >= lo || p < a.sinks) && (cur.ok >> (j >> 2) & 1);
+        x[j] = seen ? x[j] : -INFINITY;
+#pragma unroll
+        for (int w = 0; w < VW; ++w) vf[j][w] = seen ? vf[j][w] : 0;
+      }
+    }
+    float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    top = max_over_groups(top);
+    if (__ballot(top > m)) {
+      const float m2 = fmaxf(m, top);
+      const float keep = __builtin_amdgcn_exp2f(m2 == -INFINITY ? 0.0f : m - m2);
+      m = m2;
+      l *= keep;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] *= keep;
+    }
+    const float base = m == -INFINITY ? 0.0f : m;     // nothing seen yet: every numerator is 0
+    uint32_t hi[4], lo2[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float p0 = __builtin_amdgcn_exp2f(x[2 * w] - base), p1 = __builtin_amdgcn_exp2f(x[2 * w + 1] - base);
+      l += p0 + p1;
+      hi[w] = T::pair(p0, p1);
+      lo2[w] = T::pair(p0 - T::wide(hi[w] & 0xFFFFu), p1 - T::wide(hi[w] >> 16));
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      uint32_t f[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        if constexpr (E4M3) {
+          // columns e and e ^ 1 of a position are one pair
+          const uint32_t x0 = (e & 2) ? T::template from_e4m3<true>(vf[2 * w][e >> 2]) : T::template from_e4m3<false>(vf[2 * w][e >> 2]);
+          const uint32_t x1 = (e & 2) ? T::template from_e4m3<true>(vf[2 * w + 1][e >> 2]) : T::template from_e4m3<false>(vf[2 * w + 1][e >> 2]);
+          f[w] = perm(x1, x0, (e & 1) ? 0x07060302u : 0x05040100u);
+        } else {
+          f[w] = perm(vf[2 * w + 1][e >> 1], vf[2 * w][e >> 1], (e & 1) ? 0x07060302u : 0x05040100u);
+        }
+      }
+      o[e] = mfma16<T>(f, hi, o[e]);
+      o[e] = mfma16<T>(f, lo2, o[e]);
+    }
+    if (more) load_v(i + kWaves, next);
+  };
+
+  if (t0 + wave < t1) {
+    cur = pages_of(t0 + wave);
+    check(cur);
+    load_k(t0 + wave, cur);
+    load_v(t0 + wave, cur);
+    next = pages_of(min(t0 + wave + kWaves, t1 - 1));
+    int i = t0 + wave;
+    for (; i + kWaves < t1; i += kWaves) {
+      check(next);
+      Pages after = pages_of(min(i + 2 * kWaves, t1 - 1));
+      step(i, true);
+      cur = next;
+      next = after;
+    }
+    step(i, false);
+  }
+
+  // The waves' parts in one: output row e of lane (col, g): columns (4 g + i) E + e of head col.
+  l = sum_over_groups(l);
+  if (g == 0) {
+    ms[wave][col] = m;
+    ls[wave][col] = l;
+  }
+  __syncthreads();
+  float top = ms[0][col];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) top = fmaxf(top, ms[w][col]);
+  const float keep = __builtin_amdgcn_exp2f(top == -INFINITY ? 0.0f : m - top);
+  if (col < heads) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < E; e += 4)
+        *reinterpret_cast<float4*>(&os[wave][col][(4 * g + i) * E + e]) =
+            make_float4(o[e][i] * keep, o[e + 1][i] * keep, o[e + 2][i] * keep, o[e + 3][i] * keep);
+  }
+  __syncthreads();
+  const float vs = E4M3 && a.pool.vscale ? a.pool.vscale[h] : 1.0f;
+  for (int x = threadIdx.x; x < heads * (D / 4); x += 64 * kWaves) {
+    const int hh = x / (D / 4), d = 4 * (x % (D / 4));
+    float4 y = make_float4(0, 0, 0, 0);
+    float t = ms[0][hh];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) t = fmaxf(t, ms[w][hh]);
+    float sum = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float4 v = *reinterpret_cast<const float4*>(&os[w][hh][d]);
+      y.x += v.x;
+      y.y += v.y;
+      y.z += v.z;
+      y.w += v.w;
+      sum += ls[w][hh] * __builtin_amdgcn_exp2f(t == -INFINITY ? 0.0f : ms[w][hh] - t);
+    }
+    if (part.parts == 1) {
+      const float r = sum == 0 ? 0.0f : vs * __builtin_amdgcn_rcpf(sum);
+      store4<T>(a.y + part.b * a.ldy, (head0 + hh) * D + d, a.out_f32, y.x * r, y.y * r, y.z * r, y.w * r);
+    } else {
+      const int64_t at = static_cast<int64_t>(number) * a.heads + head0 + hh;
+      float* ws = a.work + at * (D + 4);
+      *reinterpret_cast<float4*>(ws + d) = y;
+      if (d == 0) *reinterpret_cast<float2*>(ws + D) = make_float2(t, sum);
+    }
+  }
+}
+
+// Joins the parts of a sequence: a workgroup per head, D / 4 lanes for a part's row.
+template <class T, int D>
+__global__ __launch_bounds__(64 * kWaves) void paged_join_kernel(PagedAttnArgs a, Deal deal) {
+  constexpr int L = D / 4, R = 64 * kWaves / L;     // lanes of a row, rows at a time
+  __shared__ float4 os[R][L];
+  __shared__ float ls[R];
+  const int c = share(a.seqs, a.window, a.sinks, deal);
+  const Part part = find_part(a.seqs, a.window, a.sinks, c, -1, blockIdx.y);
+  if (part.parts <= 1) return;
+  const int head = blockIdx.x, lane = threadIdx.x & 63, r = threadIdx.x / L, d = 4 * (threadIdx.x % L);
+  const float* ws = a.work + (static_cast<int64_t>(part.first) * a.heads + head) * (D + 4);
+  const int64_t ld = static_cast<int64_t>(a.heads) * (D + 4);
+  float top = -INFINITY;
+  for (int p = lane; p < part.parts; p += 64) top = fmaxf(top, ws[p * ld + D]);
+#pragma unroll
+  for (int i = 1; i < 64; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
+  const float base = top == -INFINITY ? 0.0f : top;
+  float4 y = make_float4(0, 0, 0, 0);
+  float sum = 0;
+#pragma unroll 4
+  for (int p = r; p < part.parts; p += R) {
+    const float4 v = *reinterpret_cast<const float4*>(ws + p * ld + d);
+    const float2 ml = *reinterpret_cast<const float2*>(ws + p * ld + D);
+    const float w = __builtin_amdgcn_exp2f(ml.x - base);
+    y.x += w * v.x;
+    y.y += w * v.y;
+    y.z += w * v.z;
+    y.w += w * v.w;
+    sum += w * ml.y;
+  }
+  os[r][threadIdx.x % L] = y;
+  if (d == 0) ls[r] = sum;
+  __syncthreads();
+  if (r) return;
+#pragma unroll
+  for (int i = 1; i < R; ++i) {
+    const float4 v = os[i][threadIdx.x];
+    y.x += v.x;
+    y.y += v.y;
+    y.z += v.z;
+    y.w += v.w;
+    sum += ls[i];
+  }
+  sum = __shfl(sum, 0);
+  const float vs = a.pool.vscale ? a.pool.vscale[head / a.group] : 1.0f;
+  const float k = sum == 0 ? 0.0f : vs * __builtin_amdgcn_rcpf(sum);
+  store4<T>(a.y + part.b * a.ldy, head * D + d, a.out_f32, y.x * k, y.y * k, y.z * k, y.w * k);
+}
+
+// The deal of a call and the most parts it can come to: the shares' and one more for each sequence, or every sequence
+// at its longest in the smallest shares.
+struct Plan {
+  Deal deal;
+  int64_t parts;
+  bool split;
+};
+Plan plan(int kv_heads, int group, int seqs, int cap, int window, int sinks) {
+  const int columns = kv_heads * ceil_div(group, kHeads);
+  Plan p;
+  p.deal = {std::max(kSlots / columns, 1), kMinShare};
+  int64_t longest = ceil_div(cap, kStep);
+  if (window > 0)
+    longest = std::min<int64_t>(longest, int64_t{window} / kStep + 2 + (int64_t{std::min(sinks, cap)} + kStep - 1) / kStep);
+  const int64_t most = (longest + kMinShare - 1) / kMinShare;
+  p.split = most > 1;
+  p.parts = std::min<int64_t>(int64_t{p.deal.slots} + seqs, most * seqs);
+  return p;
+}
+
+template <class T, bool E4M3, int D>
+hipError_t go(const PagedAttnArgs& a, hipStream_t s) {
+  const int tiles = ceil_div(a.group, kHeads);
+  const Plan p = plan(a.pool.kv_heads, a.group, a.seqs.seqs, a.seqs.cap, a.window, a.sinks);
+  const dim3 grid(static_cast<uint32_t>(a.pool.kv_heads * tiles * p.parts)), block(64 * kWaves);
+  hipLaunchKernelGGL((paged_decode_kernel<T, E4M3, D>), grid, block, 0, s, a, p.deal, tiles);
+  if (p.split) hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3(a.heads, a.seqs.seqs), block, 0, s, a, p.deal);
+  return hipGetLastError();
+}
+
+template <class T, bool E4M3>
+hipError_t by_hd(const PagedAttnArgs& a, hipStream_t s) {
+  return a.pool.hd == 64 ? go<T, E4M3, 64>(a, s) : a.pool.hd == 128 ? go<T, E4M3, 128>(a, s) : go<T, E4M3, 256>(a, s);
+}
+
+}  // namespace
+
+int64_t paged_decode_workspace(int heads, int kv_heads, int hd, int seqs, int cap) {
+  const Plan p = plan(kv_heads, heads / kv_heads, seqs, cap, 0, 0);
+  return p.split ? p.parts * heads * (hd + 4) * 4 : 0;
+}
+
+hipError_t launch_paged_decode(const PagedAttnArgs& a, hipStream_t s) {
+  const bool e4m3 = a.pool.dtype == KV_E4M3;
+  if (a.dtype == KV_BF16) return e4m3 ? by_hd<Bf16, true>(a, s) : by_hd<Bf16, false>(a, s);
+  return e4m3 ? by_hd<Fp16, true>(a, s) : by_hd<Fp16, false>(a, s);
+}
+
+}  // namespace tars

@@ -153,6 +153,7 @@ SHARED = [
     (dict(pool_kw=dict(v_page=0)), "E_ALIGN"), (dict(pool_kw=dict(v_head=-4096)), "E_ALIGN"),
     (dict(pool_kw=dict(k_page=2 ** 62, pages=100)), "E_ALIGN"),        # an extent past the address space
     (dict(table_pages=2 ** 26, pool_kw=dict(page=32)), "E_RANGE"),
+    (dict(pool_kw=dict(k_slot=2 ** 26 + 16, k_head=2 ** 32, k_page=2 ** 34)), "E_RANGE"),
 ]
 
 
@@ -179,6 +180,13 @@ def test_append_refusals(kw, code):
 def test_attention_refusals(kw, code, decode):
     assert attend(decode=decode, **kw) == getattr(_lib, code)
     assert _lib.last_error()
+
+
+def test_counts_past_the_launch_limits():
+    far = dict(lens=P + 6 * GB, starts=P + 7 * GB, table_pages=1)
+    assert append(seqs=65536, **far) == attend(seqs=65536, **far) == attend(decode=True, seqs=65536, **far) == _lib.E_RANGE
+    kw = dict(pool_kw=dict(kv_heads=1), heads=1024, seqs=8193, **far)
+    assert attend(**kw) == attend(decode=True, **kw) == _lib.E_RANGE
 
 
 def test_attention_needs_starts():
