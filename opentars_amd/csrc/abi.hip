@@ -145,7 +145,7 @@ float f32_of(uint32_t b) {
 // ---- the paged key / value cache
 
 constexpr int kMaxPagedRows = 1 << 22, kMaxPositions = 1 << 30, kMaxPagedHeads = 1024, kMaxPagedSeqs = 65535;
-constexpr int64_t kMaxSlotBytes = 1 << 26, kMaxSeqHeads = 1 << 23;
+constexpr int64_t kMaxSlotBytes = 1 << 26, kMaxSeqHeads = 1 << 22, kMaxRowHeads = 1 << 28;
 
 // Whether n_i items at stride_i (in any order of the three) hold `row` bytes each without sharing a byte; `end` gets
 // the extent.
@@ -236,10 +236,11 @@ int paged_attention(const tars_kv_pool* pool, const void* q, int64_t ldq, int32_
   if (int rc = check_paged(pool, dtype, rows_, table, ld_table, table_pages, lens, starts, seqs, c)) return rc;
   if (heads < 1 || heads > kMaxPagedHeads || heads % pool->kv_heads)
     return fail(TARS_E_FIELD, "heads must be 1..1024 and a multiple of kv_heads");
-  if (static_cast<int64_t>(seqs) * heads > kMaxSeqHeads) return fail(TARS_E_RANGE, "seqs * heads must be at most 2^23");
+  if (static_cast<int64_t>(seqs) * heads > kMaxSeqHeads || static_cast<int64_t>(rows_) * heads > kMaxRowHeads)
+    return fail(TARS_E_RANGE, "seqs * heads must be at most 2^22 and rows * heads 2^28");
   if (out != TARS_OUT_FP32 && out != (dtype == TARS_KV_BF16 ? TARS_OUT_BF16 : TARS_OUT_FP16))
     return fail(TARS_E_FIELD, "out must be FP32 or q's type");
-  if (!(scale > 0) || scale > 3.4e38f) return fail(TARS_E_FIELD, "scale must be positive and finite");
+  if (!(scale > 0) || scale > 1e30f) return fail(TARS_E_FIELD, "scale must be positive and at most 1e30");
   if (window < 0 || sinks < 0) return fail(TARS_E_FIELD, "window and sinks must not be negative");
   const int64_t qrow = 2LL * heads * pool->hd, yrow = static_cast<int64_t>(esize(out)) * heads * pool->hd;
   if (int rc = check_rows(q, ldq, rows_, qrow)) return rc;
@@ -905,7 +906,8 @@ int64_t tars_paged_workspace(int32_t heads, int32_t kv_heads, int32_t hd, int32_
                              int32_t table_pages, int32_t page, int32_t decode) {
   if (heads < 1 || kv_heads < 1 || heads % kv_heads || hd < 1 || rows_ < 1 || seqs < 1 || table_pages < 1 || page < 1 ||
       heads > kMaxPagedHeads || rows_ > kMaxPagedRows || seqs > kMaxPagedSeqs ||
-      static_cast<int64_t>(seqs) * heads > kMaxSeqHeads || static_cast<int64_t>(table_pages) * page > kMaxPositions)
+      static_cast<int64_t>(seqs) * heads > kMaxSeqHeads || static_cast<int64_t>(rows_) * heads > kMaxRowHeads ||
+      static_cast<int64_t>(table_pages) * page > kMaxPositions)
     return 0;
   return tars::paged_workspace(heads, kv_heads, hd, rows_, seqs, table_pages * page, decode != 0);
 }

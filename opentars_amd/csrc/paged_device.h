@@ -15,6 +15,7 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 
 // 16-bit element types: bits to fp32 (exact) and back (to nearest even).
 struct Bf16 {
+  static constexpr uint32_t kExponent = 0x7F80;  // all ones: infinite or NaN
   static __device__ __forceinline__ float wide(uint32_t bits) { return __uint_as_float(bits << 16); }
   static __device__ __forceinline__ uint32_t pair(float lo, float hi) {
     const v2bf r = {static_cast<__bf16>(lo), static_cast<__bf16>(hi)};
@@ -33,6 +34,7 @@ struct Bf16 {
   }
 };
 struct Fp16 {
+  static constexpr uint32_t kExponent = 0x7C00;
   static __device__ __forceinline__ float wide(uint32_t bits) {
     return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)));
   }

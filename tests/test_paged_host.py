@@ -185,8 +185,9 @@ def test_attention_refusals(kw, code, decode):
 def test_counts_past_the_launch_limits():
     far = dict(lens=P + 6 * GB, starts=P + 7 * GB, table_pages=1)
     assert append(seqs=65536, **far) == attend(seqs=65536, **far) == attend(decode=True, seqs=65536, **far) == _lib.E_RANGE
-    kw = dict(pool_kw=dict(kv_heads=1), heads=1024, seqs=8193, **far)
+    kw = dict(pool_kw=dict(kv_heads=1), heads=1024, seqs=4097, **far)
     assert attend(**kw) == attend(decode=True, **kw) == _lib.E_RANGE
+    assert attend(pool_kw=dict(kv_heads=1), heads=128, rows=2 ** 21 + 1) == _lib.E_RANGE
 
 
 def test_attention_needs_starts():
