@@ -98,8 +98,6 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t x) {  // 0xFFFF in each 
   return ((x & e) == e ? 0xFFFFu : 0) | ((x >> 16 & e) == e ? 0xFFFF0000u : 0);
 }
 
-typedef short v4s __attribute__((ext_vector_type(4)));
-
 template <class T, bool E4M3, int D, int NW>
 __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void paged_prompt_kernel(PagedAttnArgs a, int splits, int least) {
   constexpr int M = 32 * NW, KS = D / 16, NT = D / 32;

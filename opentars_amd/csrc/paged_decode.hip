@@ -27,11 +27,12 @@
 namespace tars {
 namespace {
 
-constexpr int kStep = 32;        // positions a wave takes at a time
+// Positions that a wave takes at a time: 16 for heads of 256, whose K and V rows fill the registers.
+constexpr int step_of(int hd) { return hd == 256 ? 16 : 32; }
 constexpr int kWaves = 4;
 constexpr int kHeads = 16;       // query heads of a workgroup
 constexpr int kSlots = 1024;     // workgroups that the work is dealt to
-constexpr int kMinShare = 8;     // steps that a part holds at least
+constexpr int kMinShare = 256;   // positions that a part holds at least
 
 // The sequences' steps dealt to workgroups: `slots` shares for each K / V head (and head tile).
 struct Deal {
@@ -43,15 +44,17 @@ struct Part {
   Steps steps;
 };
 
+template <int STEP>
 __device__ __forceinline__ Steps steps_of(int len, int window, int sinks) {
-  return visible_steps(len - 1, len - 1, len, window, sinks, kStep);
+  return visible_steps(len - 1, len - 1, len, window, sinks, STEP);
 }
 
 // The share C of a workgroup, the same in every wave.
+template <int STEP>
 __device__ __forceinline__ int share(const KvSeqs& s, int window, int sinks, const Deal& deal) {
   const int lane = threadIdx.x & 63;
   uint64_t mine = 0;
-  for (int b = lane; b < s.seqs; b += 64) mine += steps_of(seq_len(s.lens, b, s.cap), window, sinks).n();
+  for (int b = lane; b < s.seqs; b += 64) mine += steps_of<STEP>(seq_len(s.lens, b, s.cap), window, sinks).n();
   const uint64_t lo = group_sum<64>(static_cast<int>(mine & 0xFFFFFF)), hi = group_sum<64>(static_cast<int>(mine >> 24));
   const uint64_t total = lo + (hi << 24);
   // in units of 2^16 steps where the sum has more than 31 bits (a share too long is no harm)
@@ -74,13 +77,14 @@ __device__ __forceinline__ int inclusive_sum(int x) {
 }
 
 // The part numbered idx among all (b < 0: none), or, with idx < 0, part 0 of sequence `seq`.
+template <int STEP>
 __device__ __forceinline__ Part find_part(const KvSeqs& s, int window, int sinks, int c, int idx, int seq) {
   const int lane = threadIdx.x & 63;
   int before = 0;
   for (int b0 = 0; b0 < s.seqs; b0 += 64) {
     const int b = b0 + lane;
     const int len = b < s.seqs ? seq_len(s.lens, b, s.cap) : 0;
-    const int parts = b < s.seqs ? parts_of(steps_of(len, window, sinks).n(), c) : 0;
+    const int parts = b < s.seqs ? parts_of(steps_of<STEP>(len, window, sinks).n(), c) : 0;
     const int upto = before + inclusive_sum(parts);
     const uint64_t hit = __ballot(idx >= 0 ? upto > idx : b >= seq);
     if (hit) {
@@ -91,7 +95,7 @@ __device__ __forceinline__ Part find_part(const KvSeqs& s, int window, int sinks
       p.parts = __builtin_amdgcn_readlane(parts, at);
       p.first = __builtin_amdgcn_readlane(upto, at) - p.parts;
       p.part = idx >= 0 ? idx - p.first : 0;
-      p.steps = steps_of(p.len, window, sinks);
+      p.steps = steps_of<STEP>(p.len, window, sinks);
       return p;
     }
     before = __builtin_amdgcn_readlane(upto, 63);
@@ -105,6 +109,10 @@ template <class T>
 __device__ __forceinline__ v4f mfma16(const uint32_t (&a)[4], const uint32_t (&b)[4], v4f c) {
   const uint4 x = make_uint4(a[0], a[1], a[2], a[3]), y = make_uint4(b[0], b[1], b[2], b[3]);
   return T::mfma_16x16x32(x, y, c);
+}
+template <class T>
+__device__ __forceinline__ v4f mfma16(const uint32_t (&a)[2], const uint32_t (&b)[2], v4f c) {
+  return T::mfma_16x16x16(make_uint2(a[0], a[1]), make_uint2(b[0], b[1]), c);
 }
 
 // N dwords from global memory: a scalar base and a lane offset.
@@ -148,19 +156,20 @@ struct Pages {
 };
 
 template <class T, bool E4M3, int D>
-__global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_kernel(PagedAttnArgs a, Deal deal, int head_tiles) {
+__global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttnArgs a, Deal deal, int head_tiles) {
   constexpr int KS = D / 32;                        // products of a scores tile
   constexpr int E = D / 16;                         // columns of V per lane
   constexpr int KW = E4M3 ? 4 * KS / 2 : 4 * KS;    // dwords of a lane's K row part
   constexpr int VW = E4M3 ? E / 4 : E / 2;          // dwords of a lane's V row part
   constexpr int kPad = D + 4;
-  __shared__ __attribute__((aligned(16))) float os[kWaves][kHeads][kPad];
+  constexpr int kStep = step_of(D), kTiles = kStep / 16, NK = kStep / 4;  // NK: positions of a lane
+  __shared__ __attribute__((aligned(16))) float os[kWaves / 2][kHeads][kPad];
   __shared__ float ms[kWaves][kHeads], ls[kWaves][kHeads];
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c = share(a.seqs, a.window, a.sinks, deal);
+  const int c = share<step_of(D)>(a.seqs, a.window, a.sinks, deal);
   const int columns = a.pool.kv_heads * head_tiles, number = blockIdx.x / columns, column = blockIdx.x % columns;
-  const Part part = find_part(a.seqs, a.window, a.sinks, c, number, 0);
+  const Part part = find_part<step_of(D)>(a.seqs, a.window, a.sinks, c, number, 0);
   if (part.b < 0) return;
   const int h = column / head_tiles, tile = column % head_tiles;
   const int heads = min(a.group - tile * kHeads, kHeads);   // of this workgroup
@@ -174,7 +183,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_ke
   constexpr bool kQLds = D == 256;
   uint32_t qf[kQLds ? 1 : KS][4];
   const char* q = a.q + part.b * a.ldq + 2 * D * (head0 + min(col, heads - 1));
-  char* qs = reinterpret_cast<char*>(os[wave]) + 16 * lane;
+  char* qs = reinterpret_cast<char*>(os) + 1024 * KS * wave + 16 * lane;
+  static_assert(!kQLds || 1024 * KS * kWaves <= sizeof(os), "Q's copies fit the rows that join the waves");
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
     load_dwords<4>(qf[kQLds ? 0 : s], q, E4M3 ? 128 * (s / 2) + 16 * (s % 2) + 32 * g : 64 * s + 16 * g);
@@ -193,23 +203,23 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_ke
     const int k0 = part.steps.at(i) * kStep;
     Pages p;
     p.page[0] = table[min(k0 >> shift, last)];
-    p.page[1] = table[min((k0 + 16) >> shift, last)];
+    p.page[1] = kTiles == 2 ? table[min((k0 + 16) >> shift, last)] : 0;
     return p;
   };
   auto check = [&](Pages& p) {
     p.ok = 0;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < kTiles; ++t) {
       const bool in = static_cast<uint32_t>(p.page[t]) < static_cast<uint32_t>(a.pool.pages);
       p.ok |= in << t;
       p.page[t] = in ? p.page[t] : 0;
     }
   };
-  uint32_t kf[2][KW], vf[8][VW];
+  uint32_t kf[kTiles][KW], vf[NK][VW];
   auto load_k = [&](int i, const Pages& p) {
     const int k0 = part.steps.at(i) * kStep;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < kTiles; ++t) {
       const char* base = kbase + p.page[t] * a.pool.k_page + ((k0 + 16 * t) & mask) * a.pool.k_slot;
 #pragma unroll
       for (int s = 0; s < KW / 4; ++s)
@@ -219,7 +229,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_ke
   auto load_v = [&](int i, const Pages& p) {
     const int k0 = part.steps.at(i) * kStep;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < kTiles; ++t) {
       const char* base = vbase + p.page[t] * a.pool.v_page + ((k0 + 16 * t) & mask) * a.pool.v_slot;
 #pragma unroll
       for (int j = 0; j < 4; ++j) load_dwords<VW>(vf[4 * t + j], base + j * a.pool.v_slot, voff);
@@ -234,9 +244,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_ke
   Pages cur, next;
   auto step = [&](int i, bool more) __attribute__((always_inline)) {
     const int k0 = part.steps.at(i) * kStep;
-    v4f s[2] = {v4f{0, 0, 0, 0}, v4f{0, 0, 0, 0}};
+    v4f s[kTiles];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < kTiles; ++t) {
+      s[t] = v4f{0, 0, 0, 0};
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         uint32_t f[4];
@@ -259,14 +270,17 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_ke
           s[t] = mfma16<T>(f, qf[k], s[t]);
         }
       }
+    }
+    issue_fence();  // keeps the phases' registers apart
     if (more) load_k(i + kWaves, next);
-    float x[8];
+    issue_fence();
+    float x[NK];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = s[j >> 2][j & 3] * sc;
-    const bool whole = k0 + kStep <= part.len && (k0 >= lo || k0 + kStep <= a.sinks) && cur.ok == 3;
+    for (int j = 0; j < NK; ++j) x[j] = s[j >> 2][j & 3] * sc;
+    const bool whole = k0 + kStep <= part.len && (k0 >= lo || k0 + kStep <= a.sinks) && cur.ok == (1 << kTiles) - 1;
     if (!whole) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < NK; ++j) {
         const int p = k0 + 16 * (j >> 2) + 4 * g + (j & 3);
         const bool seen = p < part.len && (p >= lo || p < a.sinks) && (cur.ok >> (j >> 2) & 1);
         x[j] = seen ? x[j] : -INFINITY;
@@ -274,7 +288,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_ke
         for (int w = 0; w < VW; ++w) vf[j][w] = seen ? vf[j][w] : 0;
       }
     }
-    float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    float top = x[0];
+#pragma unroll
+    for (int j = 1; j < NK; ++j) top = fmaxf(top, x[j]);
     top = max_over_groups(top);
     if (__ballot(top > m)) {
       const float m2 = fmaxf(m, top);
@@ -285,9 +301,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_ke
       for (int e = 0; e < E; ++e) o[e] *= keep;
     }
     const float base = m == -INFINITY ? 0.0f : m;     // nothing seen yet: every numerator is 0
-    uint32_t hi[4], lo2[4];
+    uint32_t hi[NK / 2], lo2[NK / 2];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < NK / 2; ++w) {
       const float p0 = __builtin_amdgcn_exp2f(x[2 * w] - base), p1 = __builtin_amdgcn_exp2f(x[2 * w + 1] - base);
       l += p0 + p1;
       hi[w] = T::pair(p0, p1);
@@ -295,9 +311,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_ke
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      uint32_t f[4];
+      uint32_t f[NK / 2];
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < NK / 2; ++w) {
         if constexpr (E4M3) {
           // columns e and e ^ 1 of a position are one pair
           const uint32_t x0 = (e & 2) ? T::template from_e4m3<true>(vf[2 * w][e >> 2]) : T::template from_e4m3<false>(vf[2 * w][e >> 2]);
@@ -310,7 +326,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_ke
       o[e] = mfma16<T>(f, hi, o[e]);
       o[e] = mfma16<T>(f, lo2, o[e]);
     }
+    issue_fence();
     if (more) load_v(i + kWaves, next);
+    issue_fence();
   };
 
   if (t0 + wave < t1) {
@@ -341,15 +359,28 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_ke
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) top = fmaxf(top, ms[w][col]);
   const float keep = __builtin_amdgcn_exp2f(top == -INFINITY ? 0.0f : m - top);
-  if (col < heads) {
+  // the upper half of the waves leaves its rows in LDS, the lower half adds its own
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+  for (int e = 0; e < E; ++e) o[e] *= keep;
+  float* mine = &os[wave % (kWaves / 2)][col][4 * g * E];
 #pragma unroll
-      for (int e = 0; e < E; e += 4)
-        *reinterpret_cast<float4*>(&os[wave][col][(4 * g + i) * E + e]) =
-            make_float4(o[e][i] * keep, o[e + 1][i] * keep, o[e + 2][i] * keep, o[e + 3][i] * keep);
+  for (int turn = 1; turn >= 0; --turn) {
+    if (wave / (kWaves / 2) == turn && col < heads) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < E; e += 4) {
+          float4 y = make_float4(o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]);
+          float4* at = reinterpret_cast<float4*>(mine + i * E + e);
+          if (turn == 0) {
+            const float4 v = *at;
+            y = make_float4(y.x + v.x, y.y + v.y, y.z + v.z, y.w + v.w);
+          }
+          *at = y;
+        }
+    }
+    __syncthreads();
   }
-  __syncthreads();
   const float vs = E4M3 && a.pool.vscale ? a.pool.vscale[h] : 1.0f;
   for (int x = threadIdx.x; x < heads * (D / 4); x += 64 * kWaves) {
     const int hh = x / (D / 4), d = 4 * (x % (D / 4));
@@ -360,11 +391,13 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_ke
     float sum = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const float4 v = *reinterpret_cast<const float4*>(&os[w][hh][d]);
-      y.x += v.x;
-      y.y += v.y;
-      y.z += v.z;
-      y.w += v.w;
+      if (w < kWaves / 2) {
+        const float4 v = *reinterpret_cast<const float4*>(&os[w][hh][d]);
+        y.x += v.x;
+        y.y += v.y;
+        y.z += v.z;
+        y.w += v.w;
+      }
       sum += ls[w][hh] * __builtin_amdgcn_exp2f(t == -INFINITY ? 0.0f : ms[w][hh] - t);
     }
     if (part.parts == 1) {
@@ -385,8 +418,8 @@ __global__ __launch_bounds__(64 * kWaves) void paged_join_kernel(PagedAttnArgs a
   constexpr int L = D / 4, R = 64 * kWaves / L;     // lanes of a row, rows at a time
   __shared__ float4 os[R][L];
   __shared__ float ls[R];
-  const int c = share(a.seqs, a.window, a.sinks, deal);
-  const Part part = find_part(a.seqs, a.window, a.sinks, c, -1, blockIdx.y);
+  const int c = share<step_of(D)>(a.seqs, a.window, a.sinks, deal);
+  const Part part = find_part<step_of(D)>(a.seqs, a.window, a.sinks, c, -1, blockIdx.y);
   if (part.parts <= 1) return;
   const int head = blockIdx.x, lane = threadIdx.x & 63, r = threadIdx.x / L, d = 4 * (threadIdx.x % L);
   const float* ws = a.work + (static_cast<int64_t>(part.first) * a.heads + head) * (D + 4);
@@ -435,14 +468,14 @@ struct Plan {
   int64_t parts;
   bool split;
 };
-Plan plan(int kv_heads, int group, int seqs, int cap, int window, int sinks) {
+Plan plan(int kv_heads, int group, int hd, int seqs, int cap, int window, int sinks) {
   const int columns = kv_heads * ceil_div(group, kHeads);
   Plan p;
-  p.deal = {std::max(kSlots / columns, 1), kMinShare};
-  int64_t longest = ceil_div(cap, kStep);
-  if (window > 0)
-    longest = std::min<int64_t>(longest, int64_t{window} / kStep + 2 + (int64_t{std::min(sinks, cap)} + kStep - 1) / kStep);
-  const int64_t most = (longest + kMinShare - 1) / kMinShare;
+  const int step = step_of(hd);
+  p.deal = {std::max(kSlots / columns, 1), kMinShare / step};
+  int64_t longest = ceil_div(cap, step);
+  if (window > 0) longest = std::min<int64_t>(longest, window / step + 2 + ceil_div(std::min(sinks, cap), step));
+  const int64_t most = (longest + p.deal.min_share - 1) / p.deal.min_share;
   p.split = most > 1;
   p.parts = std::min<int64_t>(int64_t{p.deal.slots} + seqs, most * seqs);
   return p;
@@ -451,7 +484,7 @@ Plan plan(int kv_heads, int group, int seqs, int cap, int window, int sinks) {
 template <class T, bool E4M3, int D>
 hipError_t go(const PagedAttnArgs& a, hipStream_t s) {
   const int tiles = ceil_div(a.group, kHeads);
-  const Plan p = plan(a.pool.kv_heads, a.group, a.seqs.seqs, a.seqs.cap, a.window, a.sinks);
+  const Plan p = plan(a.pool.kv_heads, a.group, D, a.seqs.seqs, a.seqs.cap, a.window, a.sinks);
   const dim3 grid(static_cast<uint32_t>(a.pool.kv_heads * tiles * p.parts)), block(64 * kWaves);
   hipLaunchKernelGGL((paged_decode_kernel<T, E4M3, D>), grid, block, 0, s, a, p.deal, tiles);
   if (p.split) hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3(a.heads, a.seqs.seqs), block, 0, s, a, p.deal);
@@ -466,7 +499,7 @@ hipError_t by_hd(const PagedAttnArgs& a, hipStream_t s) {
 }  // namespace
 
 int64_t paged_decode_workspace(int heads, int kv_heads, int hd, int seqs, int cap) {
-  const Plan p = plan(kv_heads, heads / kv_heads, seqs, cap, 0, 0);
+  const Plan p = plan(kv_heads, heads / kv_heads, hd, seqs, cap, 0, 0);
   return p.split ? p.parts * heads * (hd + 4) * 4 : 0;
 }
 
