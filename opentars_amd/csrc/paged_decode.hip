@@ -31,12 +31,14 @@ namespace {
 constexpr int step_of(int hd) { return hd == 256 ? 16 : 32; }
 constexpr int kWaves = 4;
 constexpr int kHeads = 16;       // query heads of a workgroup
-constexpr int kSlots = 1024;     // workgroups that the work is dealt to
-constexpr int kMinShare = 256;   // positions that a part holds at least
+constexpr int kSlots = 1536;     // workgroups that long work is dealt to: two rounds of the three on every CU
+constexpr int kFew = 512;        // and short work, in shares of kLeast to kShort positions: one round
+constexpr int kLeast = 64, kShort = 512;
 
 // The sequences' steps dealt to workgroups: `slots` shares for each K / V head (and head tile).
 struct Deal {
-  int slots, min_share;
+  int slots, few;        // workgroups for a K / V head and head tile, of long and of short work
+  int least, most_few;   // steps
 };
 struct Part {
   int b, part, parts, first;     // the sequence, its part's number and count, the number of its first part among all
@@ -59,9 +61,10 @@ __device__ __forceinline__ int share(const KvSeqs& s, int window, int sinks, con
   const uint64_t total = lo + (hi << 24);
   // in units of 2^16 steps where the sum has more than 31 bits (a share too long is no harm)
   const int up = total < (1ull << 31) ? 0 : 16;
-  const uint32_t units = static_cast<uint32_t>((total + (1ull << up) - 1) >> up), slots = deal.slots;
-  const uint32_t c = min((units + slots - 1) / slots, 1u << 25 >> up) << up;  // no sequence has more than 2^25
-  return max(static_cast<int>(c), deal.min_share);
+  const uint32_t units = static_cast<uint32_t>((total + (1ull << up) - 1) >> up);
+  const auto per = [&](uint32_t slots) { return min((units + slots - 1) / slots, 1u << 25 >> up) << up; };
+  const int c = max(static_cast<int>(per(deal.slots)), min(static_cast<int>(per(deal.few)), deal.most_few));
+  return max(c, deal.least);  // no sequence has more than 2^25 steps
 }
 
 __device__ __forceinline__ int parts_of(int n, int c) { return max((n + c - 1) / c, 1); }
@@ -76,9 +79,9 @@ __device__ __forceinline__ int inclusive_sum(int x) {
   return x;
 }
 
-// The part numbered idx among all (b < 0: none), or, with idx < 0, part 0 of sequence `seq`.
+// The part numbered idx among all (b < 0: none).
 template <int STEP>
-__device__ __forceinline__ Part find_part(const KvSeqs& s, int window, int sinks, int c, int idx, int seq) {
+__device__ __forceinline__ Part find_part(const KvSeqs& s, int window, int sinks, int c, int idx) {
   const int lane = threadIdx.x & 63;
   int before = 0;
   for (int b0 = 0; b0 < s.seqs; b0 += 64) {
@@ -86,7 +89,7 @@ __device__ __forceinline__ Part find_part(const KvSeqs& s, int window, int sinks
     const int len = b < s.seqs ? seq_len(s.lens, b, s.cap) : 0;
     const int parts = b < s.seqs ? parts_of(steps_of<STEP>(len, window, sinks).n(), c) : 0;
     const int upto = before + inclusive_sum(parts);
-    const uint64_t hit = __ballot(idx >= 0 ? upto > idx : b >= seq);
+    const uint64_t hit = __ballot(upto > idx);
     if (hit) {
       const int at = __builtin_ctzll(hit);
       Part p;
@@ -94,7 +97,7 @@ __device__ __forceinline__ Part find_part(const KvSeqs& s, int window, int sinks
       p.len = __builtin_amdgcn_readlane(len, at);
       p.parts = __builtin_amdgcn_readlane(parts, at);
       p.first = __builtin_amdgcn_readlane(upto, at) - p.parts;
-      p.part = idx >= 0 ? idx - p.first : 0;
+      p.part = idx - p.first;
       p.steps = steps_of<STEP>(p.len, window, sinks);
       return p;
     }
@@ -115,23 +118,23 @@ __device__ __forceinline__ v4f mfma16(const uint32_t (&a)[2], const uint32_t (&b
   return T::mfma_16x16x16(make_uint2(a[0], a[1]), make_uint2(b[0], b[1]), c);
 }
 
-// N dwords from global memory: a scalar base and a lane offset.
-template <int N>
+// N dwords from global memory, read once: a scalar base and a lane offset; past four, FAR bytes from one four to the next.
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+template <int FAR, int N>
 __device__ __forceinline__ void load_dwords(uint32_t (&d)[N], const char* base, uint32_t off) {
   if constexpr (N == 1) {
-    d[0] = *reinterpret_cast<const uint32_t*>(base + off);
+    d[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(base + off));
   } else if constexpr (N == 2) {
-    const uint2 v = *reinterpret_cast<const uint2*>(base + off);
-    d[0] = v.x;
-    d[1] = v.y;
+    const v2u v = __builtin_nontemporal_load(reinterpret_cast<const v2u*>(base + off));
+    d[0] = v[0];
+    d[1] = v[1];
   } else {
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
-      const uint4 v = *reinterpret_cast<const uint4*>(base + off + 4 * i);
-      d[i] = v.x;
-      d[i + 1] = v.y;
-      d[i + 2] = v.z;
-      d[i + 3] = v.w;
+      const v4u v = __builtin_nontemporal_load(reinterpret_cast<const v4u*>(base + off + FAR * (i / 4)));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) d[i + j] = v[j];
     }
   }
 }
@@ -155,12 +158,17 @@ struct Pages {
   int ok;
 };
 
+// The workspace: (first part, parts) of every sequence, then every part's rows.
+__host__ __device__ __forceinline__ int64_t head_bytes(int seqs) { return (8ll * seqs + 15) / 16 * 16; }
+__device__ __forceinline__ float* parts_at(const PagedAttnArgs& a) { return a.work + head_bytes(a.seqs.seqs) / 4; }
+
 template <class T, bool E4M3, int D>
 __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttnArgs a, Deal deal, int head_tiles) {
   constexpr int KS = D / 32;                        // products of a scores tile
   constexpr int E = D / 16;                         // columns of V per lane
   constexpr int KW = E4M3 ? 4 * KS / 2 : 4 * KS;    // dwords of a lane's K row part
   constexpr int VW = E4M3 ? E / 4 : E / 2;          // dwords of a lane's V row part
+  constexpr int C = VW == 8 ? 8 : E;                // its neighbouring columns: two runs of 8 for 16-bit rows of 256
   constexpr int kPad = D + 4;
   constexpr int kStep = step_of(D), kTiles = kStep / 16, NK = kStep / 4;  // NK: positions of a lane
   __shared__ __attribute__((aligned(16))) float os[kWaves / 2][kHeads][kPad];
@@ -169,7 +177,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttnA
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = share<step_of(D)>(a.seqs, a.window, a.sinks, deal);
   const int columns = a.pool.kv_heads * head_tiles, number = blockIdx.x / columns, column = blockIdx.x % columns;
-  const Part part = find_part<step_of(D)>(a.seqs, a.window, a.sinks, c, number, 0);
+  const Part part = find_part<step_of(D)>(a.seqs, a.window, a.sinks, c, number);
   if (part.b < 0) return;
   const int h = column / head_tiles, tile = column % head_tiles;
   const int heads = min(a.group - tile * kHeads, kHeads);   // of this workgroup
@@ -187,7 +195,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttnA
   static_assert(!kQLds || 1024 * KS * kWaves <= sizeof(os), "Q's copies fit the rows that join the waves");
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
-    load_dwords<4>(qf[kQLds ? 0 : s], q, E4M3 ? 128 * (s / 2) + 16 * (s % 2) + 32 * g : 64 * s + 16 * g);
+    load_dwords<16>(qf[kQLds ? 0 : s], q, E4M3 ? 128 * (s / 2) + 16 * (s % 2) + 32 * g : 64 * s + 16 * g);
     if constexpr (kQLds) *reinterpret_cast<uint4*>(qs + 1024 * s) = make_uint4(qf[0][0], qf[0][1], qf[0][2], qf[0][3]);
   }
   const float sc = a.scale * 1.44269504f * (E4M3 && a.pool.kscale ? a.pool.kscale[h] : 1.0f);
@@ -196,7 +204,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttnA
   const __attribute__((address_space(4))) int32_t* table = reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(
       reinterpret_cast<uintptr_t>(a.seqs.table + part.b * a.seqs.ld_table));
   const uint32_t koff = col * static_cast<uint32_t>(a.pool.k_slot) + 16 * g;
-  const uint32_t voff = 4 * g * static_cast<uint32_t>(a.pool.v_slot) + 4 * VW * col;
+  const uint32_t voff = 4 * g * static_cast<uint32_t>(a.pool.v_slot) + 4 * (VW < 4 ? VW : 4) * col;
   const char* kbase = a.pool.k + h * a.pool.k_head;
   const char* vbase = a.pool.v + h * a.pool.v_head;
   auto pages_of = [&](int i) {
@@ -223,7 +231,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttnA
       const char* base = kbase + p.page[t] * a.pool.k_page + ((k0 + 16 * t) & mask) * a.pool.k_slot;
 #pragma unroll
       for (int s = 0; s < KW / 4; ++s)
-        load_dwords<4>(reinterpret_cast<uint32_t(&)[4]>(kf[t][4 * s]), base, koff + 64 * s);
+        load_dwords<16>(reinterpret_cast<uint32_t(&)[4]>(kf[t][4 * s]), base, koff + 64 * s);
     }
   };
   auto load_v = [&](int i, const Pages& p) {
@@ -232,7 +240,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttnA
     for (int t = 0; t < kTiles; ++t) {
       const char* base = vbase + p.page[t] * a.pool.v_page + ((k0 + 16 * t) & mask) * a.pool.v_slot;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) load_dwords<VW>(vf[4 * t + j], base + j * a.pool.v_slot, voff);
+      for (int j = 0; j < 4; ++j) load_dwords<256>(vf[4 * t + j], base + j * a.pool.v_slot, voff);
     }
   };
 
@@ -348,7 +356,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttnA
     step(i, false);
   }
 
-  // The waves' parts in one: output row e of lane (col, g): columns (4 g + i) E + e of head col.
+  // The waves' parts in one: o[e][i] is head col's column (4 g + i) C + e % C of run e / C.
   l = sum_over_groups(l);
   if (g == 0) {
     ms[wave][col] = m;
@@ -362,7 +370,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttnA
   // the upper half of the waves leaves its rows in LDS, the lower half adds its own
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] *= keep;
-  float* mine = &os[wave % (kWaves / 2)][col][4 * g * E];
+  float* mine = &os[wave % (kWaves / 2)][col][4 * g * C];
 #pragma unroll
   for (int turn = 1; turn >= 0; --turn) {
     if (wave / (kWaves / 2) == turn && col < heads) {
@@ -371,7 +379,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttnA
 #pragma unroll
         for (int e = 0; e < E; e += 4) {
           float4 y = make_float4(o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]);
-          float4* at = reinterpret_cast<float4*>(mine + i * E + e);
+          float4* at = reinterpret_cast<float4*>(mine + 16 * C * (e / C) + i * C + e % C);
           if (turn == 0) {
             const float4 v = *at;
             y = make_float4(y.x + v.x, y.y + v.y, y.z + v.z, y.w + v.w);
@@ -381,6 +389,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttnA
     }
     __syncthreads();
   }
+  if (column == 0 && part.part == 0 && a.work && threadIdx.x == 0)
+    reinterpret_cast<int2*>(a.work)[part.b] = make_int2(part.first, part.parts);
   const float vs = E4M3 && a.pool.vscale ? a.pool.vscale[h] : 1.0f;
   for (int x = threadIdx.x; x < heads * (D / 4); x += 64 * kWaves) {
     const int hh = x / (D / 4), d = 4 * (x % (D / 4));
@@ -405,7 +415,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttnA
       store4<T>(a.y + part.b * a.ldy, (head0 + hh) * D + d, a.out_f32, y.x * r, y.y * r, y.z * r, y.w * r);
     } else {
       const int64_t at = static_cast<int64_t>(number) * a.heads + head0 + hh;
-      float* ws = a.work + at * (D + 4);
+      float* ws = parts_at(a) + at * (D + 4);
       *reinterpret_cast<float4*>(ws + d) = y;
       if (d == 0) *reinterpret_cast<float2*>(ws + D) = make_float2(t, sum);
     }
@@ -414,51 +424,42 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttnA
 
 // Joins the parts of a sequence: a workgroup per head, D / 4 lanes for a part's row.
 template <class T, int D>
-__global__ __launch_bounds__(64 * kWaves) void paged_join_kernel(PagedAttnArgs a, Deal deal) {
+__global__ __launch_bounds__(64 * kWaves) void paged_join_kernel(PagedAttnArgs a) {
   constexpr int L = D / 4, R = 64 * kWaves / L;     // lanes of a row, rows at a time
   __shared__ float4 os[R][L];
-  __shared__ float ls[R];
-  const int c = share<step_of(D)>(a.seqs, a.window, a.sinks, deal);
-  const Part part = find_part<step_of(D)>(a.seqs, a.window, a.sinks, c, -1, blockIdx.y);
-  if (part.parts <= 1) return;
-  const int head = blockIdx.x, lane = threadIdx.x & 63, r = threadIdx.x / L, d = 4 * (threadIdx.x % L);
-  const float* ws = a.work + (static_cast<int64_t>(part.first) * a.heads + head) * (D + 4);
+  __shared__ float ms[R], ls[R];
+  const int b = blockIdx.y, head = blockIdx.x, r = threadIdx.x / L, at = threadIdx.x % L, d = 4 * at;
+  const int2 own = reinterpret_cast<const int2*>(a.work)[b];
+  if (own.y <= 1) return;
+  const float* ws = parts_at(a) + (static_cast<int64_t>(own.x) * a.heads + head) * (D + 4);
   const int64_t ld = static_cast<int64_t>(a.heads) * (D + 4);
-  float top = -INFINITY;
-  for (int p = lane; p < part.parts; p += 64) top = fmaxf(top, ws[p * ld + D]);
-#pragma unroll
-  for (int i = 1; i < 64; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
-  const float base = top == -INFINITY ? 0.0f : top;
   float4 y = make_float4(0, 0, 0, 0);
-  float sum = 0;
+  float m = -INFINITY, sum = 0;
+  auto add = [&](float m1, float l1, float4 v) {
+    const float top = fmaxf(m, m1), base = top == -INFINITY ? 0.0f : top;
+    const float k0 = __builtin_amdgcn_exp2f(m - base), k1 = __builtin_amdgcn_exp2f(m1 - base);
+    m = top;
+    y = make_float4(y.x * k0 + v.x * k1, y.y * k0 + v.y * k1, y.z * k0 + v.z * k1, y.w * k0 + v.w * k1);
+    sum = sum * k0 + l1 * k1;
+  };
 #pragma unroll 4
-  for (int p = r; p < part.parts; p += R) {
+  for (int p = r; p < own.y; p += R) {
     const float4 v = *reinterpret_cast<const float4*>(ws + p * ld + d);
     const float2 ml = *reinterpret_cast<const float2*>(ws + p * ld + D);
-    const float w = __builtin_amdgcn_exp2f(ml.x - base);
-    y.x += w * v.x;
-    y.y += w * v.y;
-    y.z += w * v.z;
-    y.w += w * v.w;
-    sum += w * ml.y;
+    add(ml.x, ml.y, v);
   }
-  os[r][threadIdx.x % L] = y;
-  if (d == 0) ls[r] = sum;
+  os[r][at] = y;
+  if (at == 0) {
+    ms[r] = m;
+    ls[r] = sum;
+  }
   __syncthreads();
   if (r) return;
 #pragma unroll
-  for (int i = 1; i < R; ++i) {
-    const float4 v = os[i][threadIdx.x];
-    y.x += v.x;
-    y.y += v.y;
-    y.z += v.z;
-    y.w += v.w;
-    sum += ls[i];
-  }
-  sum = __shfl(sum, 0);
+  for (int i = 1; i < R; ++i) add(ms[i], ls[i], os[i][at]);
   const float vs = a.pool.vscale ? a.pool.vscale[head / a.group] : 1.0f;
   const float k = sum == 0 ? 0.0f : vs * __builtin_amdgcn_rcpf(sum);
-  store4<T>(a.y + part.b * a.ldy, head * D + d, a.out_f32, y.x * k, y.y * k, y.z * k, y.w * k);
+  store4<T>(a.y + b * a.ldy, head * D + d, a.out_f32, y.x * k, y.y * k, y.z * k, y.w * k);
 }
 
 // The deal of a call and the most parts it can come to: the shares' and one more for each sequence, or every sequence
@@ -472,10 +473,10 @@ Plan plan(int kv_heads, int group, int hd, int seqs, int cap, int window, int si
   const int columns = kv_heads * ceil_div(group, kHeads);
   Plan p;
   const int step = step_of(hd);
-  p.deal = {std::max(kSlots / columns, 1), kMinShare / step};
+  p.deal = {std::max(kSlots / columns, 1), std::max(kFew / columns, 1), kLeast / step, kShort / step};
   int64_t longest = ceil_div(cap, step);
   if (window > 0) longest = std::min<int64_t>(longest, window / step + 2 + ceil_div(std::min(sinks, cap), step));
-  const int64_t most = (longest + p.deal.min_share - 1) / p.deal.min_share;
+  const int64_t most = (longest + p.deal.least - 1) / p.deal.least;
   p.split = most > 1;
   p.parts = std::min<int64_t>(int64_t{p.deal.slots} + seqs, most * seqs);
   return p;
@@ -487,7 +488,7 @@ hipError_t go(const PagedAttnArgs& a, hipStream_t s) {
   const Plan p = plan(a.pool.kv_heads, a.group, D, a.seqs.seqs, a.seqs.cap, a.window, a.sinks);
   const dim3 grid(static_cast<uint32_t>(a.pool.kv_heads * tiles * p.parts)), block(64 * kWaves);
   hipLaunchKernelGGL((paged_decode_kernel<T, E4M3, D>), grid, block, 0, s, a, p.deal, tiles);
-  if (p.split) hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3(a.heads, a.seqs.seqs), block, 0, s, a, p.deal);
+  if (p.split) hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3(a.heads, a.seqs.seqs), block, 0, s, a);
   return hipGetLastError();
 }
 
@@ -500,7 +501,7 @@ hipError_t by_hd(const PagedAttnArgs& a, hipStream_t s) {
 
 int64_t paged_decode_workspace(int heads, int kv_heads, int hd, int seqs, int cap) {
   const Plan p = plan(kv_heads, heads / kv_heads, hd, seqs, cap, 0, 0);
-  return p.split ? p.parts * heads * (hd + 4) * 4 : 0;
+  return p.split ? head_bytes(seqs) + p.parts * heads * (hd + 4) * 4 : 0;
 }
 
 hipError_t launch_paged_decode(const PagedAttnArgs& a, hipStream_t s) {
