@@ -53,6 +53,11 @@ __device__ __forceinline__ void ring_load16(const void* base, uint32_t off, uint
   asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "s"(dst) : "memory");
 }
 
+// The same, free to move past other memory accesses: for a stage that the kernel's barriers keep apart from them.
+__device__ __forceinline__ void ring_load16_free(const void* base, uint32_t off, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "s"(dst));
+}
+
 template <int N>
 __device__ __forceinline__ void wait_vmcnt() {
   static_assert(N >= 0 && N < 64, "vmcnt is a 6-bit count");

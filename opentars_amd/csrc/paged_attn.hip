@@ -14,10 +14,10 @@
 // in [0, 2^kSlack] and are rounded to q's type for the second product.
 //
 // Tiles at a row's own position, at a window's edge or with a page number outside the pool mask their scores. There a
-// hidden position may hold anything: the tile of V is searched for infinities and NaN; if it has any, they are added to
-// the rows that see them and zeroed before the product.
+// hidden position may hold anything: the tile of V is searched for infinities and NaN, which are zeros in the product and
+// are added to the rows that see them at the end.
 //
-// A workgroup's rows are NW * 32; the last rows of a sequence, which see most, start first. With few rows their tiles
+// A workgroup has 128 rows, a wave 32; the last rows of a sequence, which see most, start first. With few rows their tiles
 // are split over workgroups and joined by a second launch.
 #include <algorithm>
 
@@ -29,6 +29,7 @@ namespace {
 constexpr int tile_of(int hd) { return hd == 256 ? 32 : 64; }  // positions of a tile
 constexpr float kLog2e = 1.44269504f;
 constexpr float kSlack = 6.0f;
+constexpr int kRowsWg = 128;       // rows of a workgroup
 
 struct Tile {
   int b, first, rows, len;         // the sequence, its first row, its rows, its length
@@ -46,7 +47,6 @@ __device__ __forceinline__ int inclusive_sum(int x) {
   return x;
 }
 
-template <int M>
 __device__ __forceinline__ Tile find_tile(const KvSeqs& s, int group, int number) {
   const int lane = threadIdx.x & 63;
   int before = 0;
@@ -54,7 +54,7 @@ __device__ __forceinline__ Tile find_tile(const KvSeqs& s, int group, int number
     const int b = b0 + lane;
     RowSpan r{0, 0};
     if (b < s.seqs) r = seq_rows(s.starts, b, s.rows);
-    const int tiles = ceil_div(r.n * group, M);
+    const int tiles = ceil_div(r.n * group, kRowsWg);
     const int upto = before + inclusive_sum(tiles);
     const uint64_t hit = __ballot(upto > number);
     if (hit) {
@@ -63,7 +63,7 @@ __device__ __forceinline__ Tile find_tile(const KvSeqs& s, int group, int number
       t.b = __builtin_amdgcn_readfirstlane(b0 + at);
       t.first = __builtin_amdgcn_readlane(r.first, at);
       t.rows = __builtin_amdgcn_readlane(r.n, at);
-      t.r0 = (__builtin_amdgcn_readlane(upto, at) - 1 - number) * M;
+      t.r0 = (__builtin_amdgcn_readlane(upto, at) - 1 - number) * kRowsWg;
       t.len = __builtin_amdgcn_readfirstlane(seq_len(s.lens, t.b, s.cap));
       return t;
     }
@@ -82,6 +82,33 @@ __device__ __forceinline__ Steps steps_of(const Tile& t, int m, const PagedAttnA
 // Tiles of a part, and the parts of n tiles.
 __device__ __forceinline__ int parts_of(int n, int splits, int least) { return max(min(splits, n / least), 1); }
 
+// Rows of a wave, columns of its products. 32 read each operand of K and V half as often, and heads of 256 at 32 rows need
+// 128 registers for the output alone: they take 16 rows, on twice the waves.
+constexpr int wave_rows(int hd) { return hd == 256 ? 16 : 32; }
+template <class T, int R>
+struct Product;
+template <class T>
+struct Product<T, 32> {  // 32 x 32 x 16
+  typedef v16f Acc;
+  static __device__ __forceinline__ Acc go(uint4 a, uint4 b, Acc c) { return T::mfma_32x32x16(a, b, c); }
+};
+template <class T>
+struct Product<T, 16> {  // 16 x 16 x 32
+  typedef v4f Acc;
+  static __device__ __forceinline__ Acc go(uint4 a, uint4 b, Acc c) { return T::mfma_16x16x32(a, b, c); }
+};
+
+// Over the lanes of one row: l % R.
+template <int R, class Op>
+__device__ __forceinline__ float over_row(float x, Op op) {
+  if constexpr (R == 16) {
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = op(__uint_as_float(s[0]), __uint_as_float(s[1]));
+  }
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return op(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+
 // Byte offset of 16-byte chunk c of row k in a tile.
 template <int D>
 __device__ __forceinline__ int k_at(int k, int c) {
@@ -89,7 +116,7 @@ __device__ __forceinline__ int k_at(int k, int c) {
 }
 template <int D>
 __device__ __forceinline__ int v_at(int k, int c) {
-  return k * 2 * D + ((c ^ (D == 64 ? (k & 2) << 1 : (k & 3) << 2)) << 4);
+  return k * 2 * D + ((c ^ (D == 64 ? (k & 2) << 1 : D == 128 ? (k & 3) << 2 : (k & 7) << 1)) << 4);
 }
 
 template <class T>
@@ -98,17 +125,27 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t x) {  // 0xFFFF in each 
   return ((x & e) == e ? 0xFFFFu : 0) | ((x >> 16 & e) == e ? 0xFFFF0000u : 0);
 }
 
-template <class T, bool E4M3, int D, int NW>
-__global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void paged_prompt_kernel(PagedAttnArgs a, int splits, int least) {
-  constexpr int M = 32 * NW, KS = D / 16, NT = D / 32;
-  constexpr int kTile = tile_of(D), kBlocks = kTile / 16, kHalves = kTile / 32;
+__device__ __forceinline__ uint32_t max_halves(uint32_t x, uint32_t y) {
+  typedef uint16_t v2s __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(v2s, x), __builtin_bit_cast(v2s, y)));
+}
+
+template <class T, bool E4M3, int D>
+__global__ __launch_bounds__(64 * kRowsWg / wave_rows(D), 2) void paged_prompt_kernel(PagedAttnArgs a, int splits, int least) {
+  // R rows of a wave, N values of an accumulator; products of R x R x G, whose R positions make kHalves of a tile's scores,
+  // NT of the columns, and whose G make KS of the columns and kSteps of the positions.
+  constexpr int M = kRowsWg, R = wave_rows(D), kWaves = M / R, G = 512 / R, N = R * R / 64, KS = D / G, NT = D / R;
+  constexpr int kTile = tile_of(D), kBlocks = kTile / 16, kHalves = kTile / R, kSteps = kTile / G;
+  typedef Product<T, R> Mul;
+  typedef typename Mul::Acc Acc;
   constexpr int kBytes = kTile * D * 2;                 // a tile of K or V
-  __shared__ __attribute__((aligned(1024))) char lds[2][2][kBytes];  // [stage][K, V]
-  __shared__ int flags[2];
-  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+  // K's stages, V's, and for e4m3 what the loads bring: of K, of V
+  __shared__ __attribute__((aligned(1024))) char lds[4 + E4M3][kBytes];
+  bool spoiled = false;
+  const int lane = threadIdx.x & 63, col = lane % R, part = lane / R;  // of N / 4 fours of positions, columns: 4 part + e
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = blockIdx.x % a.pool.kv_heads, rest = blockIdx.x / a.pool.kv_heads, split = rest % splits;
-  const Tile tile = find_tile<M>(a.seqs, a.group, rest / splits);
+  const Tile tile = find_tile(a.seqs, a.group, rest / splits);
   if (tile.b < 0) return;
   const Steps steps = steps_of<D>(tile, M, a);
   const int n = steps.n(), parts = parts_of(n, splits, least);
@@ -116,279 +153,375 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void paged_prompt_kernel
   const int per = ceil_div(n, parts), t0 = min(split * per, n), t1 = min(t0 + per, n);
 
   // the rows of this wave: row r of the sequence's rows * group is token r / group, query head r % group
-  const int total = tile.rows * a.group, w0 = tile.r0 + 32 * wave, r = min(w0 + col, total - 1);
+  const int total = tile.rows * a.group, w0 = tile.r0 + R * wave, r = min(w0 + col, total - 1);
   const int token = r / a.group, head = h * a.group + r - token * a.group;
   const int p0 = tile.len - tile.rows, p = p0 + token;
   const int plo = p0 + tile.r0 / a.group, phi = p0 + (min(tile.r0 + M, total) - 1) / a.group;
-  const bool mine = w0 < total;
-  const int wlo = __builtin_amdgcn_readfirstlane(p), whi = __builtin_amdgcn_readlane(p, 31);
 
   uint4 qf[KS];
-  const char* q = a.q + (tile.first + token) * a.ldq + 2 * D * head + 16 * half;
+  const char* q = a.q + (tile.first + token) * a.ldq + 2 * D * head + 16 * part;
 #pragma unroll
-  for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const uint4*>(q + 32 * s);
+  for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const uint4*>(q + 2 * G * s);
   const float sc = a.scale * kLog2e * (E4M3 && a.pool.kscale ? a.pool.kscale[h] : 1.0f);
 
   const int shift = a.pool.page_shift, mask = (1 << shift) - 1, last = max(tile.len - 1, 0) >> shift;
-  const __attribute__((address_space(4))) int32_t* table = reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(
-      reinterpret_cast<uintptr_t>(a.seqs.table + tile.b * a.seqs.ld_table));
   const char* kbase = a.pool.k + h * a.pool.k_head;
   const char* vbase = a.pool.v + h * a.pool.v_head;
 
-  // the pages of a tile's four blocks of 16 positions; the ones outside the pool are read as page 0 and masked
-  struct Pages {
-    int p0, p1, p2, p3, ok;
-    __device__ __forceinline__ int of(int block) const {
-      const int x0 = p0, x1 = p1, x2 = p2, x3 = p3;
-      const int even = block & 2 ? x2 : x0, odd = block & 2 ? x3 : x1;
-      return block & 1 ? odd : even;
-    }
+  // Where the blocks of 16 positions lie: lane x holds the addresses of block x % kBlocks of tile from + x / kBlocks, of
+  // page 0 for a page number outside the pool, whose bit of `in` is 0. The loads go at most two tiles past the one
+  // computed; the addresses move on by half their tiles, the page numbers asked for two tiles before.
+  constexpr int kHeld = 64 / kBlocks, kMove = kHeld / 2;
+  int from = 0, coming = 0;
+  uint64_t k_held = 0, v_held = 0, in = 0;
+  auto position_of = [&](int i) __attribute__((always_inline)) {
+    return steps.at(min(i + lane / kBlocks, t1 - 1)) * kTile + 16 * (lane % kBlocks);
   };
-  auto pages_of = [&](int i) {
-    const int k0 = steps.at(i) * kTile;
-    return Pages{table[min(k0 >> shift, last)], table[min((k0 + 16) >> shift, last)], table[min((k0 + 32) >> shift, last)],
-                 table[min((k0 + 48) >> shift, last)], 0};
+  auto numbers = [&](int i) __attribute__((always_inline)) {
+    return a.seqs.table[tile.b * a.seqs.ld_table + min(position_of(i) >> shift, last)];
   };
-  auto in_pool = [&](int& page, int bit) {
-    const bool in = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pool.pages);
-    page = in ? page : 0;
-    return in ? bit : 0;
+  auto hold = [&](int i, int number) __attribute__((always_inline)) {
+    const bool good = static_cast<uint32_t>(number) < static_cast<uint32_t>(a.pool.pages);
+    const int64_t page = good ? number : 0, slot = position_of(i) & mask;
+    from = i;
+    in = __ballot(good);
+    k_held = reinterpret_cast<uint64_t>(kbase) + page * a.pool.k_page + slot * a.pool.k_slot;
+    v_held = reinterpret_cast<uint64_t>(vbase) + page * a.pool.v_page + slot * a.pool.v_slot;
   };
-  auto check = [&](Pages g) {
-    int p0 = g.p0, p1 = g.p1, p2 = g.p2, p3 = g.p3;
-    const int ok = in_pool(p0, 1) | in_pool(p1, 2) | (kBlocks > 2 ? in_pool(p2, 4) | in_pool(p3, 8) : 0);
-    return Pages{p0, p1, p2, p3, ok};
+  auto block_of = [&](uint64_t held, int i, int block) __attribute__((always_inline)) {
+    const int x = (i - from) * kBlocks + block;
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(held), x);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(held >> 32), x);
+    return reinterpret_cast<const char*>(static_cast<uint64_t>(hi) << 32 | lo);
+  };
+  auto in_pool = [&](int i) __attribute__((always_inline)) {
+    return static_cast<int>(in >> ((i - from) * kBlocks)) & ((1 << kBlocks) - 1);
   };
 
-  // Loading a tile. 16-bit: a load instruction moves 1 KiB = kRows rows, lane l the 16 bytes at 16 l.
-  constexpr int kRows = 512 / D, kLoads = kTile / kRows;                    // of one of K, V
-  constexpr int kHold = E4M3 ? kTile * D / 16 / (64 * NW) : 1;              // e4m3: 16-byte loads of a thread
-  uint4 hold[2][kHold];
-  auto load = [&](int i, Pages g, int stage) __attribute__((always_inline)) {
-    const int k0 = steps.at(i) * kTile;
+  // Loading a tile: a load instruction moves 1 KiB = kRows rows, lane l the 16 bytes at 16 l; a
+  // wave's loads are kSpan rows apart. Rows of e4m3 come as they are and are widened into the stage by the wave that
+  // loaded them, a tile later.
+  constexpr int kRow = E4M3 ? D : 2 * D, kRows = 1024 / kRow, kSpan = kWaves * kRows, kTake = kTile / kSpan;
+  constexpr int kSame = kSpan >= 16 ? 1 : 16 / kSpan;                        // loads with offsets of their own
+  uint32_t k_off[kSame], v_off[kSame];
+#pragma unroll
+  for (int x = 0; x < kSame; ++x) {
+    const int row = (wave * kRows + x * kSpan) % 16 + lane / (kRow / 16), c = lane % (kRow / 16);
+    k_off[x] = row * static_cast<uint32_t>(a.pool.k_slot) + (E4M3 ? 16 * c : k_at<D>(row, c) & (2 * D - 1));
+    v_off[x] = row * static_cast<uint32_t>(a.pool.v_slot) + (E4M3 ? 16 * c : v_at<D>(row, c) & (2 * D - 1));
+  }
+  const uint32_t stages = lds_addr(lds[0]) + 1024 * wave;
+  // Piece x of K's (V's) tile to byte `to` of LDS; behind the last tile, of the last one again, to where nobody reads it.
+  auto load = [&](int tile, uint32_t to, bool is_v, int x) __attribute__((always_inline)) {
+    const char* at = block_of(is_v ? v_held : k_held, min(tile, t1 - 1), (wave * kRows + x * kSpan) >> 4);
+    ring_load16_free(at, is_v ? v_off[x % kSame] : k_off[x % kSame], stages + to + 1024 * kWaves * x);
+  };
+  constexpr int kRaw = 4 * kBytes;                              // e4m3: where K arrives; V kBytes / 2 behind
+  auto widen = [&](int stage, bool is_v) __attribute__((always_inline)) {
     if constexpr (E4M3) {
+      int thread = threadIdx.x;
+      asm volatile("" : "+v"(thread) : : "memory");  // addresses formed here, rather than in registers all the way
 #pragma unroll
-      for (int x = 0; x < kHold; ++x) {
-        const int at = x * 64 * NW + threadIdx.x, k = at / (D / 16), c = at % (D / 16), page = g.of(k >> 4);
-        const int64_t slot = (k0 + k) & mask;
-        hold[0][x] = *reinterpret_cast<const uint4*>(kbase + page * a.pool.k_page + slot * a.pool.k_slot + 16 * c);
-        hold[1][x] = *reinterpret_cast<const uint4*>(vbase + page * a.pool.v_page + slot * a.pool.v_slot + 16 * c);
+      for (int x = 0; x < kTake; ++x) {
+        const int at = x * 64 * kWaves + thread, k = at / (D / 16), c = at % (D / 16);
+        const uint4 w = *reinterpret_cast<const uint4*>(lds[0] + kRaw + is_v * (kBytes / 2) + 16 * at);
+        char* to = lds[stage];
+        *reinterpret_cast<uint4*>(to + (is_v ? v_at<D>(k, 2 * c) : k_at<D>(k, 2 * c))) =
+            make_uint4(T::template from_e4m3<false>(w.x), T::template from_e4m3<true>(w.x),
+                       T::template from_e4m3<false>(w.y), T::template from_e4m3<true>(w.y));
+        *reinterpret_cast<uint4*>(to + (is_v ? v_at<D>(k, 2 * c + 1) : k_at<D>(k, 2 * c + 1))) =
+            make_uint4(T::template from_e4m3<false>(w.z), T::template from_e4m3<true>(w.z),
+                       T::template from_e4m3<false>(w.w), T::template from_e4m3<true>(w.w));
       }
-    } else {
-#pragma unroll
-      for (int x = 0; x < 2 * kLoads / NW; ++x) {
-        const int j = wave + NW * (x % (kLoads / NW)), kk = j * kRows;
-        const bool is_v = x >= kLoads / NW;
-        const int k = lane / (D / 8), c = lane % (D / 8);                   // within the instruction's rows
-        const int page = g.of(kk >> 4);
-        const int64_t slot = (k0 + kk) & mask;
-        const int swz = is_v ? v_at<D>(kk + k, c) : k_at<D>(kk + k, c);
-        const uint32_t off = k * static_cast<uint32_t>(is_v ? a.pool.v_slot : a.pool.k_slot) + (swz & (2 * D - 1));
-        const char* base = is_v ? vbase + page * a.pool.v_page + slot * a.pool.v_slot
-                                : kbase + page * a.pool.k_page + slot * a.pool.k_slot;
-        ring_load16(base, off, lds_addr(lds[stage][is_v]) + 1024 * j);
-      }
+      wait_lgkm0();
+      asm volatile("" : : : "memory");
     }
   };
-  auto land = [&](int stage) __attribute__((always_inline)) {  // e4m3: the held rows widened into the stage
-    if constexpr (E4M3) {
-#pragma unroll
-      for (int x = 0; x < kHold; ++x) {
-        const int at = x * 64 * NW + threadIdx.x, k = at / (D / 16), c = at % (D / 16);
-#pragma unroll
-        for (int is_v = 0; is_v < 2; ++is_v) {
-          const uint32_t w[4] = {hold[is_v][x].x, hold[is_v][x].y, hold[is_v][x].z, hold[is_v][x].w};
-          uint32_t f[8];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            f[2 * i] = T::template from_e4m3<false>(w[i]);
-            f[2 * i + 1] = T::template from_e4m3<true>(w[i]);
-          }
-          char* to = lds[stage][is_v];
-          *reinterpret_cast<uint4*>(to + (is_v ? v_at<D>(k, 2 * c) : k_at<D>(k, 2 * c))) = make_uint4(f[0], f[1], f[2], f[3]);
-          *reinterpret_cast<uint4*>(to + (is_v ? v_at<D>(k, 2 * c + 1) : k_at<D>(k, 2 * c + 1))) = make_uint4(f[4], f[5], f[6], f[7]);
-        }
-      }
-    }
-  };
-  auto meet = [&]() {
+  auto meet = [&]() __attribute__((always_inline)) {
     asm volatile("" : : : "memory");
-    wait_lgkm0();
     __builtin_amdgcn_s_barrier();
     asm volatile("" : : : "memory");
   };
 
   // m: the maximum taken off, in units of the raw scores; bound: a score (with m taken off) above it moves m
   float l = 0, bound = -INFINITY;
-  v16f minus, o[NT];
+  Acc minus, o[NT];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) minus[i] = 0;
+  for (int i = 0; i < N; ++i) minus[i] = 0;
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[t][i] = 0;
+  for (int t = 0; t < NT; ++t) o[t] = minus;
   const float slack = kSlack * __builtin_amdgcn_rcpf(sc);
-  // lane offsets of the reads: row col, chunk 2 s + half of K; V's transposing read of 4 rows x 16 columns
-  const int vrow = 4 * half + ((lane & 15) >> 2), vchunk = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), vbyte = (lane & 1) * 8;
+  // Lane offsets of the reads, the permutation of the chunks included: row col, chunk `part` of K (product k's is that
+  // offset with 2 G k turned over); V's transposing read of 4 rows x 16 columns (column tile t: with 2 R t turned over).
+  const uint32_t k_lane = lds_addr(lds[0]) + k_at<D>(col, part);
+  const uint32_t v_lane = lds_addr(lds[0]) + v_at<D>(4 * part + (lane % 16 >> 2), lane % R / 16 * 2 + (lane % 4 >> 1)) + lane % 2 * 8;
+  Acc s0[kHalves], s1[kHalves];
+  uint32_t pf[kTile * R / 128];
 
-  auto compute = [&](int i, int ok, int stage) __attribute__((always_inline)) {
-    const int k0 = steps.at(i) * kTile;
-    const char* kt = lds[stage][0];
-    char* vt = lds[stage][1];
-    const bool whole = k0 + kTile - 1 <= plo && (a.window == 0 || k0 > phi - a.window || k0 + kTile <= a.sinks) && ok == (1 << kBlocks) - 1;
-    if (!whole) {
-      // hidden positions may hold anything: 16 bytes of V's tile per thread and turn
-      uint32_t bad = 0;
-      for (int x = threadIdx.x; x < kBytes / 16; x += 64 * NW) {
-        const uint4 v = *reinterpret_cast<const uint4*>(vt + 16 * x);
-        bad |= not_finite<T>(v.x) | not_finite<T>(v.y) | not_finite<T>(v.z) | not_finite<T>(v.w);
-      }
-      if (bad) flags[i & 1] = 1;
-      meet();
-      const bool any = __builtin_amdgcn_readfirstlane(flags[i & 1]) != 0;
-      if (threadIdx.x == 0) flags[(i & 1) ^ 1] = 0;
-      if (any) {
-        for (int k = 0; k < kTile; ++k) {
-          const int j = k0 + k;
-          const bool seen = sees(p, j, a.window, a.sinks) && (ok >> (k >> 4) & 1);
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int d = 32 * t + 8 * (e >> 2) + 4 * half + (e & 3);
-              const uint32_t v = *reinterpret_cast<const uint16_t*>(vt + v_at<D>(k, d >> 3) + 2 * (d & 7));
-              o[t][e] += seen && not_finite<T>(v) ? T::wide(v) : 0.0f;
-            }
-        }
-        meet();
-        for (int x = threadIdx.x; x < kBytes / 16; x += 64 * NW) {
-          uint4 v = *reinterpret_cast<uint4*>(vt + 16 * x);
-          v.x &= ~not_finite<T>(v.x);
-          v.y &= ~not_finite<T>(v.y);
-          v.z &= ~not_finite<T>(v.z);
-          v.w &= ~not_finite<T>(v.w);
-          *reinterpret_cast<uint4*>(vt + 16 * x) = v;
-        }
-        meet();
+  // The steps [whole0, whole0 + wholes) are the ones that every row of the workgroup sees whole, their pages being in the
+  // pool (with a window, the steps of the first tokens count as not whole).
+  const int whole0 = steps.a + (a.window == 0 ? 0 : max(phi - a.window + kTile - steps.b0 * kTile, 0) / kTile);
+  const int wholes = max(steps.a + (plo + 1) / kTile - steps.b0 - whole0, 0);
+  auto is_whole = [&](int i) __attribute__((always_inline)) {
+    return static_cast<uint32_t>(i - whole0) < static_cast<uint32_t>(wholes) && (~in == 0 || in_pool(i) == (1 << kBlocks) - 1);
+  };
+  // one operand of V^T: positions G k + (G / 2) x + 4 part + 0 .. 3 for x = 0, 1, column col of column tile t
+  auto v_operand = [&](uint32_t vt, int k, int t) __attribute__((always_inline)) {
+    typedef __attribute__((address_space(3))) v4s* P;
+    const uint32_t at = (vt ^ (2 * R * t)) + 2 * G * k * D;
+    const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(at)));
+    const uint2 hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(at + G * D)));
+    return make_uint4(lo.x, lo.y, hi.x, hi.y);
+  };
+  auto numerators = [&](int k) __attribute__((always_inline)) {
+    return make_uint4(pf[4 * k], pf[4 * k + 1], pf[4 * k + 2], pf[4 * k + 3]);
+  };
+
+  // Hidden positions of a tile that is not whole may hold anything: V's infinities and NaN become zeros (whichever wave
+  // meets them), to be added at the end to the rows that see them.
+  auto clean = [&](int i) __attribute__((always_inline)) {
+    char* vt = lds[2 + (i & 1)];
+    uint32_t bad = 0;
+#pragma unroll 2
+    for (int x = 0; x < kBytes / 1024; ++x) {
+      const uint4 v = *reinterpret_cast<const uint4*>(vt + 1024 * x + 16 * lane);
+      bad = max_halves(max_halves(bad, max_halves(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu)),
+                       max_halves(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
+    }
+    if (__ballot(not_finite<T>(bad) != 0)) {
+      spoiled = true;
+#pragma unroll 1
+      for (int x = lane; x < kBytes / 4; x += 64) {
+        uint32_t* at = reinterpret_cast<uint32_t*>(vt) + x;
+        *at &= ~not_finite<T>(*at);
       }
     }
-    if (!mine || k0 > whi || (a.window != 0 && k0 + kTile - 1 <= wlo - a.window && k0 >= a.sinks)) return;  // nothing seen
-    v16f s[kHalves];
-#pragma unroll
-    for (int t = 0; t < kHalves; ++t) {
-      s[t] = minus;
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const uint4 f = *reinterpret_cast<const uint4*>(kt + k_at<D>(32 * t + col, 2 * k + half));
-        s[t] = T::mfma_32x32x16(f, qf[k], s[t]);
-      }
-    }
+  };
+  // S^T = K Q^T, the maximum taken off: kQk products, whose operands are read kLead ahead.
+  constexpr int kPv = kSteps * NT, kQk = KS * kHalves, kLead = D == 256 ? 8 : 4, kPairs = kTile * R / 128;
+  auto k_operand = [&](uint32_t kt, int x) __attribute__((always_inline)) {
+    typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+    const v4u v = *(__attribute__((address_space(3))) const v4u*)((kt ^ (2 * G * (x / kHalves))) + 2 * R * D * (x % kHalves));
+    return make_uint4(v[0], v[1], v[2], v[3]);
+  };
+  auto score = [&](Acc (&s)[kHalves], int x, uint4 f) __attribute__((always_inline)) {
+    s[x % kHalves] = Mul::go(f, qf[x / kHalves], x < kHalves ? minus : s[x % kHalves]);
+  };
+  // The softmax of tile i's scores s, and between its steps the products for the next tile's scores (behind the last
+  // tile: of whatever the stage holds, not used).
+  auto softmax_and_scores = [&](int i, bool whole, Acc (&s)[kHalves], Acc (&next)[kHalves]) __attribute__((always_inline)) {
+    const uint32_t kt = k_lane + ((i + 1) & 1) * kBytes;
     if (!whole) {
+      const int k0 = steps.at(i) * kTile, ok = in_pool(i);
 #pragma unroll
       for (int t = 0; t < kHalves; ++t)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int k = 32 * t + 8 * (e >> 2) + 4 * half + (e & 3);
+        for (int e = 0; e < N; ++e) {
+          const int k = R * t + (e >> 2) * (256 / R) + 4 * part + (e & 3);
           const bool seen = sees(p, k0 + k, a.window, a.sinks) && (ok >> (k >> 4) & 1);
           s[t][e] = seen ? s[t][e] : -INFINITY;
         }
     }
-    float top = s[0][0];
+    issue_fence();
+    uint4 f[kLead];
 #pragma unroll
-    for (int e = 1; e < kTile / 2; ++e) top = fmaxf(top, s[e >> 4][e & 15]);
-    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-    top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-    if (__ballot(top > bound)) {
-      const bool up = top > bound;
-      // the first scores that a row sees set m from nothing: its sum and output are 0 (or not finite) then
-      const float by = up ? top : 0.0f, keep = bound == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(-by * sc);
-      l *= keep;
-      bound = up ? slack : bound;
+    for (int x = 0; x < kLead; ++x) f[x] = k_operand(kt, x);
+    auto at = [&](Acc (&v)[kHalves], int e) __attribute__((always_inline)) -> float { return v[e / N][e % N]; };
+    constexpr int kValues = kTile * R / 64;  // of a lane
+    float top = at(s, 0);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) minus[e] -= by;
+    for (int x = 0; x < kQk; ++x) {
+      score(next, x, f[x % kLead]);
+      if (x + kLead < kQk) f[x % kLead] = k_operand(kt, x + kLead);
+      constexpr int kTop = kHalves;  // the maximum: once every half's products are under way
+      if (x == kTop - 1) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+        for (int e = 1; e < kValues / 2; ++e) top = fmaxf(top, at(s, e));
+      } else if (x == kTop) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[t][e] *= keep;
+        for (int e = kValues / 2; e < kValues; ++e) top = fmaxf(top, at(s, e));
+        top = over_row<R>(top, [](float x, float y) { return fmaxf(x, y); });
+        // By row, not for the wave as a whole: the compiler then scales the output in place, where it copied all of it on
+        // the way past a uniform branch.
+        if (top > bound) {
+          // the first scores that a row sees set m from nothing: its sum and output are 0 (or not finite) then
+          const float by = top, keep = bound == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(-by * sc);
+          l *= keep;
+          bound = slack;
 #pragma unroll
-      for (int e = 0; e < kTile / 2; ++e) s[e >> 4][e & 15] -= by;
-    }
-    uint32_t pf[kTile / 4];
+          for (int e = 0; e < N; ++e) minus[e] -= by;
 #pragma unroll
-    for (int e = 0; e < kTile / 4; ++e) {
-      const float x = __builtin_amdgcn_exp2f(s[e >> 3][2 * e & 15] * sc), y = __builtin_amdgcn_exp2f(s[e >> 3][(2 * e & 15) + 1] * sc);
-      l += x + y;
-      pf[e] = T::pair(x, y);
-    }
+          for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int k = 0; k < kBlocks; ++k) {
-      const uint4 pk = make_uint4(pf[4 * k], pf[4 * k + 1], pf[4 * k + 2], pf[4 * k + 3]);
+            for (int e = 0; e < N; ++e) o[t][e] *= keep;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        uint32_t f[4];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const char* at = vt + v_at<D>(16 * k + 8 * x + vrow, 4 * t + vchunk) + vbyte;
-          const v4s v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(at));
-          const uint2 w = __builtin_bit_cast(uint2, v);
-          f[2 * x] = w.x;
-          f[2 * x + 1] = w.y;
+          for (int e = 0; e < kValues; ++e) {
+            s[e / N][e % N] -= by;
+            next[e / N][e % N] -= by;  // under way since the old maximum
+          }
         }
-        o[t] = T::mfma_32x32x16(make_uint4(f[0], f[1], f[2], f[3]), pk, o[t]);
+      } else if (x > kTop) {
+#pragma unroll
+        for (int e = (x - kTop - 1) * kPairs / (kQk - kTop - 1); e < (x - kTop) * kPairs / (kQk - kTop - 1); ++e) {
+          const float y = __builtin_amdgcn_exp2f(at(s, 2 * e) * sc), z = __builtin_amdgcn_exp2f(at(s, 2 * e + 1) * sc);
+          l += y + z;
+          pf[e] = T::pair(y, z);
+          asm volatile("" : "+v"(pf[e]));  // here, not where it is used
+        }
       }
+      constexpr int kEvery = kQk / (2 * kTake);
+      static_assert(kEvery > 0, "a load or none behind each product");
+      if (!E4M3 && x % kEvery == kEvery - 1 && x / kEvery < 2 * kTake) {
+        if (x / kEvery < kTake) load(i + 2, (i & 1) * kBytes, false, x / kEvery);
+        else load(i + 1, (2 + ((i + 1) & 1)) * kBytes, true, x / kEvery - kTake);
+      }
+      issue_fence();
+    }
+  };
+  // O^T += V^T P^T of tile i
+  auto output = [&](int i) __attribute__((always_inline)) {
+    const uint32_t vt = v_lane + (2 + (i & 1)) * kBytes;
+    uint4 f[kLead];
+    issue_fence();
+#pragma unroll
+    for (int x = 0; x < kLead; ++x) f[x] = v_operand(vt, x / NT, x % NT);
+#pragma unroll
+    for (int x = 0; x < kPv; ++x) {
+      o[x % NT] = Mul::go(f[x % kLead], numerators(x / NT), o[x % NT]);
+      if (x + kLead < kPv) f[x % kLead] = v_operand(vt, (x + kLead) / NT, (x + kLead) % NT);
+      issue_fence();
     }
   };
 
-  if (threadIdx.x < 2) flags[threadIdx.x] = 0;
+  // A tile's softmax runs between the products for the next tile's scores: vector work that hides half the matrix work.
+  // Its product with V is matrix work alone, next to which the SIMD runs the other workgroup's wave. Between the barriers
+  // of tiles i - 1 and i K's tile i + 1 and V's tile i are read, K's i + 2 and V's i + 1 loaded, into the stages read
+  // before.
   if (t0 < t1) {
-    Pages cur = pages_of(t0), next = pages_of(min(t0 + 1, t1 - 1));
-    cur = check(cur);
-    load(t0, cur, 0);
-    if constexpr (E4M3) land(0);
-    for (int i = t0; i < t1; ++i) {
-      const int stage = (i - t0) & 1;
-      if constexpr (!E4M3) wait_vmcnt<0>();
-      meet();
-      next = check(next);
-      if (i + 1 < t1) load(i + 1, next, stage ^ 1);
-      const Pages after = pages_of(min(i + 2, t1 - 1));
-      compute(i, cur.ok, stage);
-      if constexpr (E4M3) {
-        if (i + 1 < t1) land(stage ^ 1);
-      }
-      cur = next;
-      next = after;
+    hold(t0, numbers(t0));
+    auto arrive = [&](int k_tile, int v_tile) __attribute__((always_inline)) {  // e4m3
+#pragma unroll
+      for (int x = 0; x < kTake; ++x) load(k_tile, kRaw, false, x);
+#pragma unroll
+      for (int x = 0; x < kTake; ++x) load(v_tile, kRaw + kBytes / 2, true, x);
+    };
+    // K's tiles t0 and t0 + 1, V's tile t0
+    if constexpr (E4M3) {
+      arrive(t0, t0);
+      wait_vmcnt<0>();
+      widen(t0 & 1, false);
+      widen(2 + (t0 & 1), true);
+      arrive(t0 + 1, t0 + 1);
+      wait_vmcnt<0>();
+      widen((t0 + 1) & 1, false);
+      arrive(t0 + 2, t0 + 1);
+    } else {
+#pragma unroll
+      for (int x = 0; x < kTake; ++x) load(t0, (t0 & 1) * kBytes, false, x);
+#pragma unroll
+      for (int x = 0; x < kTake; ++x) load(t0 + 1, ((t0 + 1) & 1) * kBytes, false, x);
+#pragma unroll
+      for (int x = 0; x < kTake; ++x) load(t0, (2 + (t0 & 1)) * kBytes, true, x);
+      wait_vmcnt<0>();
     }
+    meet();
+#pragma unroll
+    for (int x = 0; x < kQk; ++x) score(s0, x, k_operand(k_lane + (t0 & 1) * kBytes, x));
+    meet();
+    auto turn = [&](int i, Acc (&s)[kHalves], Acc (&next)[kHalves]) __attribute__((always_inline)) {
+      if (i - from == kMove - 2) coming = numbers(from + kMove);
+      if (i - from == kMove) hold(i, coming);
+      const bool whole = is_whole(i);
+      if constexpr (E4M3) {
+        wait_vmcnt<0>();
+        widen(i & 1, false);
+        widen(2 + ((i + 1) & 1), true);
+        arrive(i + 3, i + 2);
+      }
+      softmax_and_scores(i, whole, s, next);
+      if (!whole) clean(i);
+      output(i);
+      if constexpr (!E4M3) wait_vmcnt<0>();
+      else wait_lgkm0();
+      meet();
+    };
+    for (int i = t0;;) {
+      turn(i, s0, s1);
+      if (++i == t1) break;
+      turn(i, s1, s0);
+      if (++i == t1) break;
+    }
+    wait_vmcnt<0>();  // the loads behind the last tile, before the workgroup's LDS goes to another
   }
 
-  // row r: columns 32 t + 8 (e / 4) + 4 half + e % 4
-  const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
-  l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
-  if (w0 + col >= total) return;
-  if (parts == 1) {
-    const float vs = E4M3 && a.pool.vscale ? a.pool.vscale[h] : 1.0f;
-    const float k = l == 0 ? 0.0f : vs * __builtin_amdgcn_rcpf(l);
-    char* y = a.y + (tile.first + token) * a.ldy;
+  l = over_row<R>(l, [](float x, float y) { return x + y; });
+  int r_out = w0 + col;
+  asm volatile("" : "+v"(r_out));  // the row's numbers again, rather than in registers all the way
+  const int token_out = r_out / a.group, head_out = h * a.group + r_out - token_out * a.group;
+  float* ws = a.work + static_cast<int64_t>(split) * a.seqs.rows * a.heads * (D + 4);
+  if (r_out < total) {
+    if (parts == 1) {
+      const float vs = E4M3 && a.pool.vscale ? a.pool.vscale[h] : 1.0f;
+      const float k = l == 0 ? 0.0f : vs * __builtin_amdgcn_rcpf(l);
+      char* y = a.y + (tile.first + token_out) * a.ldy;
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int e = 0; e < 16; e += 4)
-        store4<T>(y, head * D + 32 * t + 2 * e + 4 * half, a.out_f32, o[t][e] * k, o[t][e + 1] * k, o[t][e + 2] * k, o[t][e + 3] * k);
-  } else {
-    float* ws = a.work + ((static_cast<int64_t>(split) * a.seqs.rows + tile.first + token) * a.heads + head) * (D + 4);
+        for (int e = 0; e < N; e += 4)
+          store4<T>(y, head_out * D + R * t + e * (64 / R) + 4 * part, a.out_f32, o[t][e] * k, o[t][e + 1] * k, o[t][e + 2] * k, o[t][e + 3] * k);
+    } else {
+      float* at = ws + (static_cast<int64_t>(tile.first + token_out) * a.heads + head_out) * (D + 4);
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int e = 0; e < 16; e += 4)
-        *reinterpret_cast<float4*>(ws + 32 * t + 2 * e + 4 * half) = make_float4(o[t][e], o[t][e + 1], o[t][e + 2], o[t][e + 3]);
-    // the maximum in the exponent's units; none seen: the sum is 0 and the maximum counts for nothing
-    if (half == 0) *reinterpret_cast<float2*>(ws + D) = make_float2(l == 0 ? -INFINITY : -minus[0] * sc, l);
+        for (int e = 0; e < N; e += 4)
+          *reinterpret_cast<float4*>(at + R * t + e * (64 / R) + 4 * part) = make_float4(o[t][e], o[t][e + 1], o[t][e + 2], o[t][e + 3]);
+      // the maximum in the exponent's units; none seen: the sum is 0 and the maximum counts for nothing
+      if (part == 0) *reinterpret_cast<float2*>(at + D) = make_float2(l == 0 ? -INFINITY : -minus[0] * sc, l);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) *reinterpret_cast<volatile int*>(lds[0]) = 0;
+  __syncthreads();
+  if (spoiled) *reinterpret_cast<volatile int*>(lds[0]) = 1;
+  __syncthreads();
+  if (*reinterpret_cast<volatile int*>(lds[0]) == 0) return;
+
+  // The infinities and NaN that were left out, added to the outputs of the rows that see them: a thread per column.
+  for (int d = threadIdx.x; d < D; d += 64 * kWaves) {
+#pragma unroll 1
+    for (int i = t0; i < t1; ++i) {
+      const int k0 = steps.at(i) * kTile;
+      if (static_cast<uint32_t>(i - whole0) < static_cast<uint32_t>(wholes)) continue;
+#pragma unroll 1
+      for (int j = k0; j < min(k0 + kTile, tile.len); ++j) {
+        const int page = a.seqs.table[tile.b * a.seqs.ld_table + (j >> shift)];
+        if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pool.pages)) continue;
+        const char* at = vbase + page * a.pool.v_page + (j & mask) * a.pool.v_slot;
+        const uint32_t v = E4M3 ? T::template from_e4m3<false>(reinterpret_cast<const uint8_t*>(at)[d]) & 0xFFFFu
+                                : reinterpret_cast<const uint16_t*>(at)[d];
+        if (!not_finite<T>(v)) continue;
+#pragma unroll 1
+        for (int x = tile.r0; x < min(tile.r0 + M, total); ++x) {
+          const int t = x / a.group, hh = h * a.group + x - t * a.group;
+          if (!sees(p0 + t, j, a.window, a.sinks)) continue;
+          if (parts > 1) {
+            ws[(static_cast<int64_t>(tile.first + t) * a.heads + hh) * (D + 4) + d] += T::wide(v);
+          } else if (a.out_f32) {
+            reinterpret_cast<float*>(a.y + (tile.first + t) * a.ldy)[hh * D + d] += T::wide(v);
+          } else {
+            uint16_t* y = reinterpret_cast<uint16_t*>(a.y + (tile.first + t) * a.ldy) + hh * D + d;
+            *y = static_cast<uint16_t>(T::pair(T::wide(*y) + T::wide(v), 0.0f));
+          }
+        }
+      }
+    }
   }
 }
 
 // Joins the parts of rows whose tiles were split: a workgroup per row and 4 heads, D / 4 lanes of a wave for a head's
 // row, the wave's other lanes for other parts.
-template <class T, int D, int M>
+template <class T, int D>
 __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedAttnArgs a, int splits, int least) {
   constexpr int L = D / 4, R = 64 / L;
   const int row = blockIdx.x, lane = threadIdx.x & 63;
@@ -398,8 +531,8 @@ __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedAttnArgs a,
   const RowSpan span = seq_rows(a.seqs.starts, b, a.seqs.rows);
   if (row < span.first || row >= span.first + span.n) return;
   const int h = head / a.group, r = (row - span.first) * a.group + head % a.group;
-  const Tile tile{b, span.first, span.n, seq_len(a.seqs.lens, b, a.seqs.cap), r / M * M};
-  const int parts = parts_of(steps_of<D>(tile, M, a).n(), splits, least);
+  const Tile tile{b, span.first, span.n, seq_len(a.seqs.lens, b, a.seqs.cap), r / kRowsWg * kRowsWg};
+  const int parts = parts_of(steps_of<D>(tile, kRowsWg, a).n(), splits, least);
   if (parts == 1) return;
   const int64_t ld = static_cast<int64_t>(a.seqs.rows) * a.heads * (D + 4);
   const float* ws = a.work + (static_cast<int64_t>(row) * a.heads + head) * (D + 4);
@@ -436,39 +569,31 @@ __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedAttnArgs a,
 }
 
 struct Plan {
-  int waves, splits;
+  int splits;
   int64_t tiles;
 };
 constexpr int kLeast = 4;          // tiles of a part at least
 Plan plan(int heads, int kv_heads, int hd, int rows, int seqs, int cap) {
   const int group = heads / kv_heads;
-  Plan p;
-  p.waves = 4;
-  if (hd != 256 && (static_cast<int64_t>(rows) * heads) / 256 >= 512) p.waves = 8;
-  const int m = 32 * p.waves;
-  p.tiles = (static_cast<int64_t>(rows) * group + m - 1) / m + seqs;
-  const int64_t wgs = std::max<int64_t>((static_cast<int64_t>(rows) * group + m - 1) / m, std::min(rows, seqs)) * kv_heads;
+  const int64_t full = (static_cast<int64_t>(rows) * group + kRowsWg - 1) / kRowsWg;
+  const int64_t wgs = std::max<int64_t>(full, std::min(rows, seqs)) * kv_heads;
   const int64_t most = std::max(ceil_div(cap, tile_of(hd)) / kLeast, 1);
-  p.splits = static_cast<int>(std::clamp<int64_t>(512 / wgs, 1, std::min<int64_t>(most, 64)));
-  return p;
+  return {static_cast<int>(std::clamp<int64_t>(512 / wgs, 1, std::min<int64_t>(most, 64))), full + seqs};
 }
 
-template <class T, bool E4M3, int D, int NW>
-hipError_t run(const PagedAttnArgs& a, const Plan& p, hipStream_t s) {
+template <class T, bool E4M3, int D>
+hipError_t run(const PagedAttnArgs& a, hipStream_t s) {
+  const Plan p = plan(a.heads, a.pool.kv_heads, D, a.seqs.rows, a.seqs.seqs, a.seqs.cap);
   const dim3 grid(static_cast<uint32_t>(p.tiles * p.splits * a.pool.kv_heads));
-  hipLaunchKernelGGL((paged_prompt_kernel<T, E4M3, D, NW>), grid, dim3(64 * NW), 0, s, a, p.splits, kLeast);
+  hipLaunchKernelGGL((paged_prompt_kernel<T, E4M3, D>), grid, dim3(64 * kRowsWg / wave_rows(D)), 0, s, a, p.splits, kLeast);
   if (p.splits > 1)
-    hipLaunchKernelGGL((paged_prompt_join_kernel<T, D, 32 * NW>), dim3(a.seqs.rows, ceil_div(a.heads, 4)), dim3(256), 0, s, a,
-                       p.splits, kLeast);
+    hipLaunchKernelGGL((paged_prompt_join_kernel<T, D>), dim3(a.seqs.rows, ceil_div(a.heads, 4)), dim3(256), 0, s, a, p.splits, kLeast);
   return hipGetLastError();
 }
 
 template <class T, bool E4M3>
 hipError_t go(const PagedAttnArgs& a, hipStream_t s) {
-  const Plan p = plan(a.heads, a.pool.kv_heads, a.pool.hd, a.seqs.rows, a.seqs.seqs, a.seqs.cap);
-  if (a.pool.hd == 256) return run<T, E4M3, 256, 4>(a, p, s);
-  if (a.pool.hd == 128) return p.waves == 8 ? run<T, E4M3, 128, 8>(a, p, s) : run<T, E4M3, 128, 4>(a, p, s);
-  return p.waves == 8 ? run<T, E4M3, 64, 8>(a, p, s) : run<T, E4M3, 64, 4>(a, p, s);
+  return a.pool.hd == 64 ? run<T, E4M3, 64>(a, s) : a.pool.hd == 128 ? run<T, E4M3, 128>(a, s) : run<T, E4M3, 256>(a, s);
 }
 
 }  // namespace
