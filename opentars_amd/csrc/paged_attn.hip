@@ -217,24 +217,35 @@ __global__ __launch_bounds__(64 * kRowsWg / wave_rows(D), 2) void paged_prompt_k
     ring_load16_free(at, is_v ? v_off[x % kSame] : k_off[x % kSame], stages + to + 1024 * kWaves * x);
   };
   constexpr int kRaw = 4 * kBytes;                              // e4m3: where K arrives; V kBytes / 2 behind
-  auto widen = [&](int stage, bool is_v) __attribute__((always_inline)) {
+  // What has arrived of K (and of V) into their stages; the arrival rows are free for the next loads then.
+  auto widen = [&](int k_stage, int v_stage, bool with_v) __attribute__((always_inline)) {
     if constexpr (E4M3) {
       int thread = threadIdx.x;
       asm volatile("" : "+v"(thread) : : "memory");  // addresses formed here, rather than in registers all the way
+      uint4 w[2][kTake];
 #pragma unroll
-      for (int x = 0; x < kTake; ++x) {
-        const int at = x * 64 * kWaves + thread, k = at / (D / 16), c = at % (D / 16);
-        const uint4 w = *reinterpret_cast<const uint4*>(lds[0] + kRaw + is_v * (kBytes / 2) + 16 * at);
-        char* to = lds[stage];
-        *reinterpret_cast<uint4*>(to + (is_v ? v_at<D>(k, 2 * c) : k_at<D>(k, 2 * c))) =
-            make_uint4(T::template from_e4m3<false>(w.x), T::template from_e4m3<true>(w.x),
-                       T::template from_e4m3<false>(w.y), T::template from_e4m3<true>(w.y));
-        *reinterpret_cast<uint4*>(to + (is_v ? v_at<D>(k, 2 * c + 1) : k_at<D>(k, 2 * c + 1))) =
-            make_uint4(T::template from_e4m3<false>(w.z), T::template from_e4m3<true>(w.z),
-                       T::template from_e4m3<false>(w.w), T::template from_e4m3<true>(w.w));
-      }
-      wait_lgkm0();
-      asm volatile("" : : : "memory");
+      for (int v = 0; v < 1 + with_v; ++v)
+#pragma unroll
+        for (int x = 0; x < kTake; ++x)
+          w[v][x] = *reinterpret_cast<const uint4*>(lds[0] + kRaw + v * (kBytes / 2) + 16 * (x * 64 * kWaves + thread));
+#pragma unroll
+      for (int v = 0; v < 1 + with_v; ++v)
+#pragma unroll
+        for (int x = 0; x < kTake; ++x) asm volatile("" : "+v"(w[v][x].x), "+v"(w[v][x].y), "+v"(w[v][x].z), "+v"(w[v][x].w));
+#pragma unroll
+      for (int v = 0; v < 1 + with_v; ++v)
+#pragma unroll
+        for (int x = 0; x < kTake; ++x) {
+          const int at = x * 64 * kWaves + thread, k = at / (D / 16), c = at % (D / 16);
+          const uint4 u = w[v][x];
+          char* to = lds[v ? v_stage : k_stage];
+          *reinterpret_cast<uint4*>(to + (v ? v_at<D>(k, 2 * c) : k_at<D>(k, 2 * c))) =
+              make_uint4(T::template from_e4m3<false>(u.x), T::template from_e4m3<true>(u.x),
+                         T::template from_e4m3<false>(u.y), T::template from_e4m3<true>(u.y));
+          *reinterpret_cast<uint4*>(to + (v ? v_at<D>(k, 2 * c + 1) : k_at<D>(k, 2 * c + 1))) =
+              make_uint4(T::template from_e4m3<false>(u.z), T::template from_e4m3<true>(u.z),
+                         T::template from_e4m3<false>(u.w), T::template from_e4m3<true>(u.w));
+        }
     }
   };
   auto meet = [&]() __attribute__((always_inline)) {
@@ -409,11 +420,11 @@ __global__ __launch_bounds__(64 * kRowsWg / wave_rows(D), 2) void paged_prompt_k
     if constexpr (E4M3) {
       arrive(t0, t0);
       wait_vmcnt<0>();
-      widen(t0 & 1, false);
-      widen(2 + (t0 & 1), true);
+      widen(t0 & 1, 2 + (t0 & 1), true);
       arrive(t0 + 1, t0 + 1);
       wait_vmcnt<0>();
-      widen((t0 + 1) & 1, false);
+      widen((t0 + 1) & 1, 0, false);
+      wait_lgkm0();
       arrive(t0 + 2, t0 + 1);
     } else {
 #pragma unroll
@@ -434,8 +445,7 @@ __global__ __launch_bounds__(64 * kRowsWg / wave_rows(D), 2) void paged_prompt_k
       const bool whole = is_whole(i);
       if constexpr (E4M3) {
         wait_vmcnt<0>();
-        widen(i & 1, false);
-        widen(2 + ((i + 1) & 1), true);
+        widen(i & 1, 2 + ((i + 1) & 1), true);
         arrive(i + 3, i + 2);
       }
       softmax_and_scores(i, whole, s, next);
