@@ -27,7 +27,7 @@ LIB = PKG / "libopentars_amd.so"
 OBJ = PKG / "_build"
 SOURCES = ["abi.hip", "queue.hip", "quant_rows.hip", "gemv_w8a8.hip", "gemm_w8a8_mfma.hip", "w4a16.hip",
            "rowops.hip", "attn_rows.hip", "embed.hip", "kv_append.hip", "paged_attn.hip",
-           "paged_decode.hip"]
+           "paged_rows.hip"]
 ARCH = "gfx950"
 
 

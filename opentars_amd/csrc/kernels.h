@@ -396,7 +396,7 @@ struct EmbedArgs {
 };
 hipError_t launch_embed_rows(const EmbedArgs& a, hipStream_t s);
 
-// The paged key / value cache (kv_append.hip, paged_attn.hip). A pool's strides are in bytes.
+// The paged key / value cache (kv_append.hip, paged_attn.hip, paged_rows.hip). A pool's strides are in bytes.
 enum KvType : int { KV_BF16 = 0, KV_FP16 = 1, KV_E4M3 = 2 };
 struct KvPool {
   char* k;
@@ -437,9 +437,10 @@ struct PagedAttnArgs {
 };
 // Bytes of scratch that a call needs: for the partial results of a sequence split over workgroups.
 int64_t paged_workspace(int heads, int kv_heads, int hd, int rows, int seqs, int cap, bool decode);
-int64_t paged_decode_workspace(int heads, int kv_heads, int hd, int seqs, int cap);
+int64_t paged_rows_workspace(int heads, int kv_heads, int hd, int rows, int seqs, int cap);
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t s);
-hipError_t launch_paged_decode(const PagedAttnArgs& a, hipStream_t s);
+// Few rows for each sequence (paged_rows.hip), one where seqs.starts is null.
+hipError_t launch_paged_rows(const PagedAttnArgs& a, hipStream_t s);
 
 hipError_t launch_attention(const AttnArgs& a, hipStream_t s);
 // Prompt rows (attn_rows.hip): 16 query rows of a head per workgroup; the arguments of launch_attention

@@ -37,16 +37,6 @@ struct Tile {
 };
 
 // The workgroup's rows: `number` counts M-row tiles over the sequences; within one the last comes first.
-__device__ __forceinline__ int inclusive_sum(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast 15 to rows 1 and 3
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast 31 to rows 2 and 3
-  return x;
-}
-
 __device__ __forceinline__ Tile find_tile(const KvSeqs& s, int group, int number) {
   const int lane = threadIdx.x & 63;
   int before = 0;
@@ -63,7 +53,8 @@ __device__ __forceinline__ Tile find_tile(const KvSeqs& s, int group, int number
       t.b = __builtin_amdgcn_readfirstlane(b0 + at);
       t.first = __builtin_amdgcn_readlane(r.first, at);
       t.rows = __builtin_amdgcn_readlane(r.n, at);
-      t.r0 = (__builtin_amdgcn_readlane(upto, at) - 1 - number) * kRowsWg;
+      // clamped, for starts that do not ascend: their sums may be anything
+      t.r0 = iclamp(__builtin_amdgcn_readlane(upto, at) - 1 - number, 0, __builtin_amdgcn_readlane(tiles, at) - 1) * kRowsWg;
       t.len = __builtin_amdgcn_readfirstlane(seq_len(s.lens, t.b, s.cap));
       return t;
     }
@@ -98,17 +89,6 @@ struct Product<T, 16> {  // 16 x 16 x 32
   static __device__ __forceinline__ Acc go(uint4 a, uint4 b, Acc c) { return T::mfma_16x16x32(a, b, c); }
 };
 
-// Over the lanes of one row: l % R.
-template <int R, class Op>
-__device__ __forceinline__ float over_row(float x, Op op) {
-  if constexpr (R == 16) {
-    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = op(__uint_as_float(s[0]), __uint_as_float(s[1]));
-  }
-  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return op(__uint_as_float(s[0]), __uint_as_float(s[1]));
-}
-
 // Byte offset of 16-byte chunk c of row k in a tile.
 template <int D>
 __device__ __forceinline__ int k_at(int k, int c) {
@@ -117,12 +97,6 @@ __device__ __forceinline__ int k_at(int k, int c) {
 template <int D>
 __device__ __forceinline__ int v_at(int k, int c) {
   return k * 2 * D + ((c ^ (D == 64 ? (k & 2) << 1 : D == 128 ? (k & 3) << 2 : (k & 7) << 1)) << 4);
-}
-
-template <class T>
-__device__ __forceinline__ uint32_t not_finite(uint32_t x) {  // 0xFFFF in each half that is infinite or NaN
-  const uint32_t e = T::kExponent;
-  return ((x & e) == e ? 0xFFFFu : 0) | ((x >> 16 & e) == e ? 0xFFFF0000u : 0);
 }
 
 __device__ __forceinline__ uint32_t max_halves(uint32_t x, uint32_t y) {
@@ -497,36 +471,15 @@ __global__ __launch_bounds__(64 * kRowsWg / wave_rows(D), 2) void paged_prompt_k
   __syncthreads();
   if (*reinterpret_cast<volatile int*>(lds[0]) == 0) return;
 
-  // The infinities and NaN that were left out, added to the outputs of the rows that see them: a thread per column.
-  for (int d = threadIdx.x; d < D; d += 64 * kWaves) {
 #pragma unroll 1
-    for (int i = t0; i < t1; ++i) {
-      const int k0 = steps.at(i) * kTile;
-      if (static_cast<uint32_t>(i - whole0) < static_cast<uint32_t>(wholes)) continue;
-#pragma unroll 1
-      for (int j = k0; j < min(k0 + kTile, tile.len); ++j) {
-        const int page = a.seqs.table[tile.b * a.seqs.ld_table + (j >> shift)];
-        if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pool.pages)) continue;
-        const char* at = vbase + page * a.pool.v_page + (j & mask) * a.pool.v_slot;
-        const uint32_t v = E4M3 ? T::template from_e4m3<false>(reinterpret_cast<const uint8_t*>(at)[d]) & 0xFFFFu
-                                : reinterpret_cast<const uint16_t*>(at)[d];
-        if (!not_finite<T>(v)) continue;
-#pragma unroll 1
-        for (int x = tile.r0; x < min(tile.r0 + M, total); ++x) {
-          const int t = x / a.group, hh = h * a.group + x - t * a.group;
-          if (!sees(p0 + t, j, a.window, a.sinks)) continue;
-          if (parts > 1) {
-            ws[(static_cast<int64_t>(tile.first + t) * a.heads + hh) * (D + 4) + d] += T::wide(v);
-          } else if (a.out_f32) {
-            reinterpret_cast<float*>(a.y + (tile.first + t) * a.ldy)[hh * D + d] += T::wide(v);
-          } else {
-            uint16_t* y = reinterpret_cast<uint16_t*>(a.y + (tile.first + t) * a.ldy) + hh * D + d;
-            *y = static_cast<uint16_t>(T::pair(T::wide(*y) + T::wide(v), 0.0f));
-          }
-        }
-      }
-    }
-  }
+  for (int i = t0; i < t1; ++i)
+    if (static_cast<uint32_t>(i - whole0) >= static_cast<uint32_t>(wholes))
+      add_unfinite<T, E4M3, D>(a, tile.b, h, tile.len, steps.at(i) * kTile, kTile, p0, tile.first, tile.r0, min(M, total - tile.r0),
+                               [&](int x) {
+                                 const int t = x / a.group;
+                                 return parts > 1 ? ws + (static_cast<int64_t>(tile.first + t) * a.heads + h * a.group + x - t * a.group) * (D + 4)
+                                                  : nullptr;
+                               });
 }
 
 // Joins the parts of rows whose tiles were split: a workgroup per row and 4 heads, D / 4 lanes of a wave for a head's
@@ -608,13 +561,17 @@ hipError_t go(const PagedAttnArgs& a, hipStream_t s) {
 
 }  // namespace
 
+// Sequences of 32 columns or fewer on average go to the kernel for few rows.
+static bool few_rows(int group, int rows, int seqs) { return static_cast<int64_t>(rows) * group <= 32ll * seqs; }
+
 int64_t paged_workspace(int heads, int kv_heads, int hd, int rows, int seqs, int cap, bool decode) {
-  if (decode) return paged_decode_workspace(heads, kv_heads, hd, seqs, cap);
+  if (decode || few_rows(heads / kv_heads, rows, seqs)) return paged_rows_workspace(heads, kv_heads, hd, rows, seqs, cap);
   const Plan p = plan(heads, kv_heads, hd, rows, seqs, cap);
   return p.splits > 1 ? int64_t{4} * p.splits * rows * heads * (hd + 4) : 0;
 }
 
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t s) {
+  if (few_rows(a.group, a.seqs.rows, a.seqs.seqs)) return launch_paged_rows(a, s);
   const bool e4m3 = a.pool.dtype == KV_E4M3;
   if (a.dtype == KV_BF16) return e4m3 ? go<Bf16, true>(a, s) : go<Bf16, false>(a, s);
   return e4m3 ? go<Fp16, true>(a, s) : go<Fp16, false>(a, s);

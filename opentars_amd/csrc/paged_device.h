@@ -62,6 +62,41 @@ struct Fp16 {
   }
 };
 
+__device__ __forceinline__ int inclusive_sum(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast 15 to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast 31 to rows 2 and 3
+  return x;
+}
+
+// Over the lanes of one row: l % R.
+template <int R, class Op>
+__device__ __forceinline__ float over_row(float x, Op op) {
+  if constexpr (R == 16) {
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = op(__uint_as_float(s[0]), __uint_as_float(s[1]));
+  }
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return op(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+
+template <class T>
+__device__ __forceinline__ uint32_t not_finite(uint32_t x) {  // 0xFFFF in each half that is infinite or NaN
+  const uint32_t e = T::kExponent;
+  return ((x & e) == e ? 0xFFFFu : 0) | ((x >> 16 & e) == e ? 0xFFFF0000u : 0);
+}
+
+// The same for four e4m3 values: 0xFF for a NaN.
+__device__ __forceinline__ uint32_t nan_e4m3(uint32_t x) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r |= (x >> 8 * i & 0x7F) == 0x7F ? 0xFFu << 8 * i : 0;
+  return r;
+}
+
 // Four neighbouring values of an output row, rounded once: fp32 or T.
 template <class T>
 __device__ __forceinline__ void store4(char* row, int at, int f32, float a, float b, float c, float d) {
@@ -81,6 +116,39 @@ __device__ __forceinline__ int seq_of_row(const KvSeqs& s, int row) {
     if (here < 64) break;
   }
   return __builtin_amdgcn_readfirstlane(n);
+}
+
+// V's infinities and NaN at the positions [k0, k0 + count) of sequence b, which the products left out, added to the outputs
+// of the columns [c0, c0 + cols) of K / V head h that see them; column x is query head h * group + x % group of row
+// first + x / group, at position p0 + x / group. part(x): the column's row of a part in the workspace, or null where its
+// output is final. A thread per column of V; all of the workgroup's outputs are written, and the barrier behind that passed.
+template <class T, bool E4M3, int D, class F>
+__device__ void add_unfinite(const PagedAttnArgs& a, int b, int h, int len, int k0, int count, int p0, int first, int c0, int cols,
+                             F part) {
+  for (int d = threadIdx.x; d < D; d += blockDim.x) {
+#pragma unroll 1
+    for (int j = k0; j < min(k0 + count, len); ++j) {
+      const int page = a.seqs.table[b * a.seqs.ld_table + (j >> a.pool.page_shift)];
+      if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pool.pages)) continue;
+      const char* at = a.pool.v + h * a.pool.v_head + page * a.pool.v_page + (j & ((1 << a.pool.page_shift) - 1)) * a.pool.v_slot;
+      const uint32_t v = E4M3 ? T::template from_e4m3<false>(reinterpret_cast<const uint8_t*>(at)[d]) & 0xFFFFu
+                              : reinterpret_cast<const uint16_t*>(at)[d];
+      if (!not_finite<T>(v)) continue;
+#pragma unroll 1
+      for (int x = c0; x < c0 + cols; ++x) {
+        const int t = x / a.group, head = h * a.group + x - t * a.group;
+        if (!sees(p0 + t, j, a.window, a.sinks)) continue;
+        if (float* to = part(x)) {
+          to[d] += T::wide(v);
+        } else if (a.out_f32) {
+          reinterpret_cast<float*>(a.y + (first + t) * a.ldy)[head * D + d] += T::wide(v);
+        } else {
+          uint16_t* y = reinterpret_cast<uint16_t*>(a.y + (first + t) * a.ldy) + head * D + d;
+          *y = static_cast<uint16_t>(T::pair(T::wide(*y) + T::wide(v), 0.0f));
+        }
+      }
+    }
+  }
 }
 
 }  // namespace tars

@@ -139,6 +139,23 @@ def test_prompt_rows_over_longer_caches(rows, past, heads, kv):
     prompt(Layer(rows, [past + rows, past // 2 + rows], [rows, rows], heads, kv, 128, page=32), window=0)
 
 
+@pytest.mark.parametrize("qt,cache", [("bf16", "same"), ("fp16", "same"), ("bf16", "e4m3"), ("fp16", "e4m3")])
+@pytest.mark.parametrize("heads,kv,hd,page", [(4, 4, 64, 16), (16, 4, 128, 16), (12, 2, 128, 64), (4, 1, 256, 32), (7, 1, 64, 128)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (50, 6)])
+def test_few_rows_of_each_sequence(qt, cache, heads, kv, hd, page, window, sinks):
+    """32 columns (rows times query heads of a K / V head) a sequence or fewer on average, some sequences with none, some
+    with more."""
+    rows = [1, 5, 0, 3, 40, 2, 1, 4, 0, 0, 1, 1, 0, 0, 2, 1, 1, 1, 1, 0]
+    lens = [1, 70, 9, 500, 48, 1, 300, 4, 0, 55, 16, 17, 3, 0, 1000, 129, 128, 127, 33, 31]
+    prompt(Layer(hd + heads, lens, rows, heads, kv, hd, page=page, qt=qt, cache=cache, spare=3), window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("hd,kv", [(64, 2), (128, 8), (256, 1)])
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+def test_few_rows_over_split_lengths(hd, kv, cache):
+    prompt(Layer(hd, [6000, 700, 3, 2500], [5, 6, 4, 7], 4 * kv, kv, hd, page=32, cache=cache))
+
+
 def test_prompt_output_types_and_scale():
     layer = Layer(5, [50, 20], [31, 20], 4, 2, 64, spare=1)
     prompt(layer, torch.float32, scale=0.3)
@@ -224,6 +241,54 @@ def test_hidden_positions_never_change_a_row(hd, cache, window, sinks):
     dirty = got[~clean][:, :2 * hd]                                    # the K / V head that holds them: 2 query heads
     assert not bool(torch.isfinite(dirty).all(1).any())
     compare(got[:, 2 * hd:], want[:, 2 * hd:], tol[:, 2 * hd:])        # the other K / V head's
+
+
+@pytest.mark.parametrize("hd,cache", [(128, "same"), (64, "e4m3"), (256, "same"), (128, "e4m3")])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (20, 2)])
+@pytest.mark.parametrize("n", [70, 1300])
+def test_hidden_positions_never_change_one_of_few_rows(hd, cache, window, sinks, n):
+    """The same for eight rows of a sequence, the hidden positions among their own, in one part and in several."""
+    layer = Layer(7, [n, n], [8, 8], 4, 2, hd, qt="fp16", cache=cache)
+    bad = {n - 3: float("inf"), n - 5: float("nan")}
+    if window:
+        bad[n - 27] = float("-inf")                                    # the first row's window alone holds it
+    for p, value in bad.items():
+        page, slot = layer.where[0][p]
+        for pool, col in ((layer.kpool, 3), (layer.vpool, 9)):
+            if pool.dtype == E4M3:
+                pool.view(torch.uint8)[page, 0, slot, col] = 0x7F
+            else:
+                pool[page, 0, slot, col] = value
+    cache_, q, table, lens, starts = layer.dev(ops)
+    got = ops.paged_attention(cache_, q, table, lens, starts, window=window, sinks=sinks, out=OUT_FP32).cpu()
+    want, tol = layer.want(torch.zeros(got.shape), window=window, sinks=sinks)
+    p = torch.arange(n - 8, n)
+    clean = torch.ones(8, dtype=torch.bool)
+    for j in bad:
+        clean &= ~((j <= p) & ((j > p - window) if window else True))
+    assert int(clean.sum()) == (2 if window else 3)
+    compare(got[:8][clean], want[:8][clean], tol[:8][clean])
+    assert not bool(torch.isfinite(got[:8][~clean][:, :2 * hd]).all(1).any())
+    compare(got[:, 2 * hd:], want[:, 2 * hd:], tol[:, 2 * hd:])
+    compare(got[8:], want[8:], tol[8:])
+
+
+def test_an_infinity_in_v_reaches_its_own_column_of_the_rows_that_see_it():
+    """V alone holds an infinity, ahead of some rows: the rows that see it are infinite in its column and nowhere else."""
+    for rows in (8, 100):
+        layer = Layer(rows, [200], [rows], 4, 2, 64, qt="bf16")
+        page, slot = layer.where[0][196]
+        layer.vpool[page, 1, slot, 20] = float("inf")
+        cache, q, table, lens, starts = layer.dev(ops)
+        got = ops.paged_attention(cache, q, table, lens, starts, out=OUT_FP32).cpu()
+        want, tol = layer.want(torch.zeros(got.shape))
+        see = torch.arange(200 - rows, 200) >= 196
+        cols = [2 * 64 + 20, 3 * 64 + 20]
+        assert bool(torch.isposinf(got[see][:, cols]).all())
+        rest = torch.ones(256, dtype=torch.bool)
+        rest[cols] = False
+        compare(got[:, rest], want[:, rest], tol[:, rest])
+        compare(got[~see], want[~see], tol[~see])
 
 
 @pytest.mark.parametrize("hd,cache", [(128, "same"), (64, "e4m3")])
