@@ -83,18 +83,16 @@ __device__ __forceinline__ float over_row(float x, Op op) {
   return op(__uint_as_float(s[0]), __uint_as_float(s[1]));
 }
 
+// Masks without comparisons, whose results would crowd the scalar registers.
 template <class T>
 __device__ __forceinline__ uint32_t not_finite(uint32_t x) {  // 0xFFFF in each half that is infinite or NaN
-  const uint32_t e = T::kExponent;
-  return ((x & e) == e ? 0xFFFFu : 0) | ((x >> 16 & e) == e ? 0xFFFF0000u : 0);
+  const uint32_t e = T::kExponent << 16 | T::kExponent, rest = (x & e) ^ e;  // 0 where the exponent is all ones
+  const uint32_t top = ~(rest + 0x7FFF7FFFu) & 0x80008000u;
+  return (top << 1) - (top >> 15);
 }
-
-// The same for four e4m3 values: 0xFF for a NaN.
-__device__ __forceinline__ uint32_t nan_e4m3(uint32_t x) {
-  uint32_t r = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) r |= (x >> 8 * i & 0x7F) == 0x7F ? 0xFFu << 8 * i : 0;
-  return r;
+__device__ __forceinline__ uint32_t nan_e4m3(uint32_t x) {    // 0xFF in each byte that is an e4m3 NaN
+  const uint32_t top = ((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+  return (top << 1) - (top >> 7);
 }
 
 // Four neighbouring values of an output row, rounded once: fp32 or T.

@@ -34,7 +34,7 @@ namespace {
 // Positions that a wave takes at a time: 16 for heads of 256, whose K and V rows fill the registers.
 constexpr int step_of(int hd) { return hd == 256 ? 16 : 32; }
 constexpr int kWaves = 4;
-constexpr int kSlots = 1536;     // workgroups that long work is dealt to: two rounds of the three on every CU
+constexpr int kSlots = 512;      // workgroups that long work is dealt to, for each that a CU holds: two rounds
 constexpr int kFew = 512;        // and short work, in shares of kLeast to kShort positions: one round
 constexpr int kLeast = 64, kShort = 512;
 
@@ -54,14 +54,14 @@ struct Part {
 };
 
 template <int STEP>
-__device__ __forceinline__ Work work_of(const PagedAttnArgs& a, int b, int wide) {
+__device__ __forceinline__ Work work_of(const PagedAttnArgs& a, int b, int wide) {  // wide: a constant
   Work w{0, 0, 0, 0, {0, 0, 0}};
   if (b >= a.seqs.seqs) return w;
   w.len = seq_len(a.seqs.lens, b, a.seqs.cap);
   const RowSpan r = a.seqs.starts ? seq_rows(a.seqs.starts, b, a.seqs.rows) : RowSpan{b, 1};
   w.first = r.first;
   w.rows = r.n;
-  w.tiles = ceil_div(r.n * a.group, wide);
+  w.tiles = static_cast<uint32_t>(r.n * a.group + wide - 1) / static_cast<uint32_t>(wide);
   w.steps = visible_steps(w.len - r.n, w.len - 1, w.len, a.window, a.sinks, STEP);
   return w;
 }
@@ -103,7 +103,7 @@ __device__ __forceinline__ Part find_part(const PagedAttnArgs& a, int wide, int 
       p.work = {of(w.len), of(w.first), of(w.rows), of(w.tiles), {of(w.steps.a), of(w.steps.b0), of(w.steps.b1)}};
       p.first = of(upto) - p.parts * p.work.tiles;
       // clamped, for starts that do not ascend: their sums may be anything
-      const int part = (idx - p.first) / p.work.tiles;
+      const int part = p.work.tiles == 1 ? idx - p.first : (idx - p.first) / p.work.tiles;
       p.part = iclamp(part, 0, p.parts - 1);
       p.tile = iclamp(idx - p.first - part * p.work.tiles, 0, p.work.tiles - 1);
       return p;
@@ -193,10 +193,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(PagedAttnArg
   const int n = steps.n(), per = (n + part.parts - 1) / part.parts;
   const int t0 = min(part.part * per, n), t1 = min(n, t0 + per);
   // positions of the workgroup's first and last column, and of this lane's
-  const int plo = p0 + c0 / a.group, phi = p0 + (c0 + cols - 1) / a.group;
+  const auto token_of = [&](int x) { return part.work.rows == 1 ? 0 : x / a.group; };
+  const int plo = p0 + token_of(c0), phi = p0 + token_of(c0 + cols - 1);
   int at[CT];
 #pragma unroll
-  for (int u = 0; u < CT; ++u) at[u] = p0 + (c0 + min(16 * u + col, cols - 1)) / a.group;
+  for (int u = 0; u < CT; ++u) at[u] = p0 + token_of(c0 + min(16 * u + col, cols - 1));
 
   // Q^T. Heads of 256 keep it in LDS (every wave's own copy, 16 bytes of a lane at a time), where the registers are needed
   // for K and V.
@@ -207,7 +208,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(PagedAttnArg
   static_assert(!kQLds || 1024 * KS * kWaves <= sizeof(os), "Q's copies fit the rows that join the waves");
 #pragma unroll
   for (int u = 0; u < CT; ++u) {
-    const int x = c0 + min(16 * u + col, cols - 1), token = x / a.group;
+    const int x = c0 + min(16 * u + col, cols - 1), token = token_of(x);
     const char* q = a.q + (part.work.first + token) * a.ldq + 2 * D * (h * a.group + x - token * a.group);
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
@@ -334,14 +335,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(PagedAttnArg
 #pragma unroll
         for (int j = 0; j < NK; ++j)
 #pragma unroll
-          for (int w = 0; w < VW; ++w) bad |= E4M3 ? nan_e4m3(vf[j][w]) : not_finite<T>(vf[j][w]);
-        if (__ballot(bad != 0)) {
-          spoiled = true;
-#pragma unroll
-          for (int j = 0; j < NK; ++j)
-#pragma unroll
-            for (int w = 0; w < VW; ++w) vf[j][w] &= ~(E4M3 ? nan_e4m3(vf[j][w]) : not_finite<T>(vf[j][w]));
-        }
+          for (int w = 0; w < VW; ++w) {
+            const uint32_t out = E4M3 ? nan_e4m3(vf[j][w]) : not_finite<T>(vf[j][w]);
+            bad |= out;
+            vf[j][w] &= ~out;
+            asm volatile("" : "+v"(bad), "+v"(vf[j][w]));  // one mask at a time in the registers
+          }
+        spoiled |= bad != 0;
       }
     }
     uint32_t hi[CT][NK / 2], lo[CT][NK / 2];
@@ -478,7 +478,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(PagedAttnArg
     }
     if (part.parts == 1) {
       const float r = sum == 0 ? 0.0f : vs * __builtin_amdgcn_rcpf(sum);
-      const int token = (c0 + cc) / a.group, head = h * a.group + c0 + cc - token * a.group;
+      const int token = token_of(c0 + cc), head = h * a.group + c0 + cc - token * a.group;
       store4<T>(a.y + (part.work.first + token) * a.ldy, head * D + d, a.out_f32, y.x * r, y.y * r, y.z * r, y.w * r);
     } else {
       float* to = ws + cc * (D + 4);
@@ -557,7 +557,7 @@ Plan plan(int kv_heads, int group, int hd, int rows, int seqs, int cap, bool one
   const int step = step_of(hd);
   Plan p;
   p.wide = hd != 256 && static_cast<int64_t>(rows) * group > 16ll * seqs ? 32 : 16;
-  p.deal = {std::max(kSlots / kv_heads, 1), std::max(kFew / kv_heads, 1), kLeast / step, kShort / step};
+  p.deal = {std::max(kSlots * (p.wide == 32 ? 2 : 3) / kv_heads, 1), std::max(kFew / kv_heads, 1), kLeast / step, kShort / step};
   int64_t longest = ceil_div(cap, step);
   if (window > 0 && one_each)
     longest = std::min<int64_t>(longest, window / step + 2 + ceil_div(std::min(sinks, cap), step));
