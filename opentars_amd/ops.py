@@ -32,6 +32,7 @@ There is no CPU path: without the built library or a GPU every call raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Sequence
 
 import numpy as np
@@ -551,29 +552,46 @@ class PagedCache:
         self._ref = ctypes.byref(self._pool)
 
 
-def _paged_rows(cache: PagedCache, t: torch.Tensor, what: str) -> int:
-    """The element code of a call's packed rows, which must lie on the cache's GPU, the current one."""
+def _paged_rows(cache: PagedCache, t: torch.Tensor, what: str):
+    """The element code, shape and row stride (bytes) of a call's packed rows, which must lie on the cache's GPU."""
     code = _KV_DTYPES.get(t.dtype)
     if code is None or code == 2:
         raise ValueError(f"{what} must be bf16 or fp16")
-    if t.get_device() != cache.index or cache.index != torch.cuda.current_device():
-        raise ValueError(f"{what} must live on the cache's GPU, and that must be the current device")
-    return code
+    if t.get_device() != cache.index:
+        raise ValueError(f"{what} must live on the cache's GPU")
+    if t.dim() != 2:
+        raise ValueError("expected a 2-D tensor with contiguous rows")
+    (rows, cols), (ld, one) = t.shape, t.stride()
+    if one != 1 and cols > 1:
+        raise ValueError("expected a 2-D tensor with contiguous rows")
+    return code, rows, cols, 2 * ld
 
 
 def _paged_meta(cache: PagedCache, table: torch.Tensor, lens: torch.Tensor, starts: torch.Tensor | None):
-    seqs = lens.shape[0]
-    if table.dtype != torch.int32 or lens.dtype != torch.int32 or (starts is not None and starts.dtype != torch.int32):
+    i32, index = torch.int32, cache.index
+    if table.dtype != i32 or lens.dtype != i32 or (starts is not None and starts.dtype != i32):
         raise ValueError("table, lens and starts must be int32")
-    if table.get_device() != cache.index or lens.get_device() != cache.index or (
-            starts is not None and starts.get_device() != cache.index):
+    if table.get_device() != index or lens.get_device() != index or (starts is not None and starts.get_device() != index):
         raise ValueError("table, lens and starts must live on the cache's GPU")
+    if torch._C._cuda_getDevice() != index:
+        raise ValueError("the cache's GPU must be the current device")
+    if table.dim() != 2 or lens.dim() != 1:
+        raise ValueError("table must be [seqs, table_pages] and lens [seqs]")
+    (seqs, pages), (ld, one) = table.shape, table.stride()
+    if one != 1 and pages > 1:
+        raise ValueError("expected a 2-D tensor with contiguous rows")
+    if lens.shape[0] != seqs:
+        raise ValueError("table must have a row for each sequence")
     _vec(lens, seqs, "lens")
     if starts is not None:
         _vec(starts, seqs + 1, "starts")
-    if table.shape[0] != seqs:
-        raise ValueError("table must have a row for each sequence")
-    return table.data_ptr(), _ld(table), table.shape[1], lens.data_ptr(), _ptr(starts), seqs
+        return table.data_ptr(), 4 * ld, pages, lens.data_ptr(), starts.data_ptr(), seqs
+    return table.data_ptr(), 4 * ld, pages, lens.data_ptr(), None, seqs
+
+
+@functools.lru_cache(maxsize=1024)
+def _paged_workspace(*sizes: int) -> int:
+    return _lib.lib().tars_paged_workspace(*sizes)
 
 
 def kv_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
@@ -583,22 +601,20 @@ def kv_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torch.
     [seqs, table_pages]: its page numbers; starts int32 [seqs + 1]: its rows are starts[b] .. starts[b + 1] - 1, its
     last positions (without it, one row per sequence). Rows behind the last sequence, at negative positions (an idle
     slot's, length 0) or on pages outside the pool are not stored. No rows: nothing is done."""
-    code = _paged_rows(cache, k, "k")
-    if _paged_rows(cache, v, "v") != code or k.shape != v.shape:
+    code, rows, cols, ldk = _paged_rows(cache, k, "k")
+    vcode, vrows, vcols, ldv = _paged_rows(cache, v, "v")
+    if vcode != code or vrows != rows or vcols != cols:
         raise ValueError("k and v must have one shape and type")
-    ldk, ldv = _ld(k), _ld(v)
-    if k.shape[1] != cache.kv_heads * cache.hd:
+    if cols != cache.kv_heads * cache.hd:
         raise ValueError("k and v must be [rows, kv_heads * hd]")
     meta = _paged_meta(cache, table, lens, starts)
-    if k.shape[0] == 0 or (starts is not None and meta[5] == 0):
+    if rows == 0 or (starts is not None and meta[5] == 0):
         return
-    _check(_lib.lib().tars_kv_append(cache._ref, k.data_ptr(), ldk, v.data_ptr(), ldv, code, k.shape[0], *meta, _stream()))
+    _check(_lib.lib().tars_kv_append(cache._ref, k.data_ptr(), ldk, v.data_ptr(), ldv, code, rows, *meta, _stream()))
 
 
 def _paged(cache: PagedCache, q: torch.Tensor, table, lens, starts, scale, window: int, sinks: int, out, y):
-    code = _paged_rows(cache, q, "q")
-    ldq = _ld(q)
-    rows, cols = q.shape
+    code, rows, cols, ldq = _paged_rows(cache, q, "q")
     hd = cache.hd
     heads = cols // hd
     if heads * hd != cols or heads < 1 or heads % cache.kv_heads:
@@ -611,7 +627,8 @@ def _paged(cache: PagedCache, q: torch.Tensor, table, lens, starts, scale, windo
         if out is None:
             out = _KV_OUT[code]
         dtype = torch.float32 if out == OUT_FP32 else q.dtype
-        y = (torch.zeros if starts is not None else torch.empty)((rows, cols), dtype=dtype, device=q.device)
+        y = (torch.zeros if starts is not None else torch.empty)((rows, cols), dtype=dtype, device=cache.device)
+        ldy = y.element_size() * cols
     else:
         if y.shape != q.shape or y.get_device() != cache.index or (y.dtype != torch.float32 and _KV_DTYPES.get(y.dtype) != code):
             raise ValueError("y must have q's shape and place, fp32 or q's type")
@@ -620,12 +637,13 @@ def _paged(cache: PagedCache, q: torch.Tensor, table, lens, starts, scale, windo
             out = OUT_FP32 if is_f32 else _KV_OUT[code]
         elif is_f32 != (out == OUT_FP32):
             raise ValueError("y must have the type that out names")
+        ldy = _ld(y)
     if rows == 0 or seqs == 0:
         return y
     lib = _lib.lib()
-    need = lib.tars_paged_workspace(heads, cache.kv_heads, hd, rows, seqs, meta[2], cache.page, starts is None)
-    work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    args = (cache._ref, q.data_ptr(), ldq, code, heads, rows, y.data_ptr(), _ld(y), out,
+    need = _paged_workspace(heads, cache.kv_heads, hd, rows, seqs, meta[2], cache.page, starts is None)
+    work = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
+    args = (cache._ref, q.data_ptr(), ldq, code, heads, rows, y.data_ptr(), ldy, out,
             hd ** -0.5 if scale is None else scale, window, sinks, *meta[:4])
     if starts is None:
         _check(lib.tars_paged_decode(*args, _ptr(work), need, _stream()))
