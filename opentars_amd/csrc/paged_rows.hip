@@ -35,8 +35,8 @@ namespace {
 constexpr int step_of(int hd) { return hd == 256 ? 16 : 32; }
 constexpr int kWaves = 4;
 constexpr int kSlots = 512;      // workgroups that long work is dealt to, for each that a CU holds: two rounds
-constexpr int kFew = 512;        // and short work, in shares of kLeast to kShort positions: one round
-constexpr int kLeast = 64, kShort = 512;
+constexpr int kFew = 512;        // and short work, in shares of up to kShort positions: one round
+constexpr int kShort = 512;
 
 struct Deal {
   int slots, few;        // workgroups for a K / V head, of long and of short work
@@ -557,7 +557,7 @@ Plan plan(int kv_heads, int group, int hd, int rows, int seqs, int cap, bool one
   const int step = step_of(hd);
   Plan p;
   p.wide = hd != 256 && static_cast<int64_t>(rows) * group > 16ll * seqs ? 32 : 16;
-  p.deal = {std::max(kSlots * (p.wide == 32 ? 2 : 3) / kv_heads, 1), std::max(kFew / kv_heads, 1), kLeast / step, kShort / step};
+  p.deal = {std::max(kSlots * (p.wide == 32 ? 2 : 3) / kv_heads, 1), std::max(kFew / kv_heads, 1), kWaves, kShort / step};
   int64_t longest = ceil_div(cap, step);
   if (window > 0 && one_each)
     longest = std::min<int64_t>(longest, window / step + 2 + ceil_div(std::min(sinks, cap), step));
