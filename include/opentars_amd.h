@@ -14,8 +14,9 @@
  * golden model's "every check before any write" rule (tars_mini/golden.py:450-472).
  *
  * Results are bit-exact against the golden model's arithmetic (tars_mini/golden.py,
- * tars_mini/numerics.py; the paged cache's attention is outside that contract): exact int32 dot products, then the fp32 epilogue one rounded step at a
- * time (round-to-nearest-even, subnormals flushed on the way in and out, canonical NaN, no FMA).
+ * tars_mini/numerics.py; the paged cache is outside that contract): exact int32 dot products, then
+ * the fp32 epilogue one rounded step at a time (round-to-nearest-even, subnormals flushed on the way
+ * in and out, canonical NaN, no FMA).
  * Results never depend on launch geometry.
  */
 #ifndef OPENTARS_AMD_H
@@ -298,8 +299,9 @@ int tars_attention_noalloc(const float* const* q, int64_t ldq, const float* cons
  * A serving cache of 16- or 8-bit K and V rows in pages that many sequences share, and the attention
  * that reads it. It has no counterpart in the reference, whose attention reads one sequence's dense
  * fp32 / binary16 rows (tars_attention above), and it is not part of the golden contract: results
- * are rounded once at the end from fp32 sums whose order is the kernels' own (they do not depend on
- * the stream, on other calls or on time; which kernel runs depends on the call's sizes).
+ * are rounded once at the end from fp32 sums whose order is the kernels' own. The order depends on
+ * the call's sizes, and for few rows on the lengths of all its sequences, over which the work is
+ * split; never on the stream, on other calls or on time, so a repeated call gives the same bits.
  *
  * A pool holds `pages` pages of `page` positions (a power of two, 16 or more) for kv_heads heads of
  * hd (64, 128 or 256) elements. K of page i, head h, slot t is the row at
@@ -315,7 +317,9 @@ int tars_attention_noalloc(const float* const* q, int64_t ldq, const float* cons
  * may be 0) are the last ones of sequence b, so row i of its n is at position lens[b] - n + i.
  * Device arrays are not checked on the host; whatever they hold, nothing outside the call's buffers is
  * read or written: lens is clamped to [0, table_pages * page], starts to [0, rows], a page number
- * outside the pool means that its positions hold nothing. */
+ * outside the pool means that its positions hold nothing.
+ * Limits (TARS_E_FIELD / TARS_E_RANGE past them): 1024 heads, 65535 sequences, 2^22 rows, seqs * heads
+ * 2^22, rows * heads 2^28, slots 2^26 bytes apart. */
 #define TARS_KV_BF16  0
 #define TARS_KV_FP16  1
 #define TARS_KV_E4M3  2
@@ -360,7 +364,8 @@ int64_t tars_paged_workspace(int32_t heads, int32_t kv_heads, int32_t hd, int32_
  * 0; rows behind the last sequence are left as they were.
  *   q [rows, heads * hd] at ldq, BF16 or FP16; query head h reads K / V head h / (heads / kv_heads).
  *   y [rows, heads * hd] at ldy, out = FP32 or q's type (BF16 / FP16). fp32 scores, maxima and sums;
- *   the softmax's numerators are rounded to q's type for the product with V.
+ *   the softmax's numerators are rounded to q's type for the product with V (where a sequence's rows
+ *   times heads / kv_heads come to 32 or fewer on average, to the sum of two values of it).
  *   0 < scale <= 1e30; work: tars_paged_workspace bytes, 16-byte aligned, for this call until it is done.
  */
 int tars_paged_attention(const tars_kv_pool* pool, const void* q, int64_t ldq, int32_t dtype,

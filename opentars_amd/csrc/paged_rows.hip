@@ -24,6 +24,13 @@
 // its own (sequence, tile, part) in the prefix sums. So one long cache fills the GPU as well as many short ones, whatever
 // the batch's longest is. A sequence of one part is written at once; the parts of the others go to the workspace as
 // (maximum, sum, unscaled output) in fp32 and a second launch joins them in order.
+//
+// What bounds it: reading the cache once. Measured with 8 K / V heads of 128: three caches of 90k to 131k 231 us, 6.4 TB/s
+// (a plain read of memory comes to 6.0 to 6.4); 64 of up to 8k 174 to 180 us, 5.7 TB/s; 32 of 9k to 17k in e4m3 with
+// 64 query heads 162 us, 5.4 TB/s, the widening of K and V beside the loads; 16 of 3k to 16k with five rows each (32
+// columns, two workgroups on a CU instead of three) 134 us, 4.8 TB/s. Short work is bound by the chain launch -> lengths
+// -> page numbers -> K and V -> second launch: one cache of 2k 10.8 us, of 300 10.0 us; 100 windows of 512, one K / V
+// head of 256, 19.7 us.
 #include <algorithm>
 
 #include "paged_device.h"
@@ -34,9 +41,12 @@ namespace {
 // Positions that a wave takes at a time: 16 for heads of 256, whose K and V rows fill the registers.
 constexpr int step_of(int hd) { return hd == 256 ? 16 : 32; }
 constexpr int kWaves = 4;
-constexpr int kSlots = 512;      // workgroups that long work is dealt to, for each that a CU holds: two rounds
-constexpr int kFew = 512;        // and short work, in shares of up to kShort positions: one round
-constexpr int kShort = 512;
+// Long work is dealt to two rounds of the workgroups that the CUs hold, kSlots for each that a CU holds: three to a CU
+// 64 caches of up to 8k 174 us and three of 110k 231 us (one round less 175 and 246, one more 177 and 241). Short work,
+// shares of up to kShort positions, is dealt to two workgroups on a CU: 100 windows of 512 13.9 us (16.4 with one, which
+// is better for one long cache: 8k 15.0 and 13.1). A share has a step for each wave at least: one cache of 4k 10.9 us
+// (12.8 with half of that).
+constexpr int kSlots = 512, kFew = 512, kShort = 512;
 
 struct Deal {
   int slots, few;        // workgroups for a K / V head, of long and of short work
@@ -547,6 +557,8 @@ __global__ __launch_bounds__(64 * kWaves) void paged_rows_join_kernel(PagedAttnA
 
 // Column tiles of a workgroup, the deal, and the most parts it can come to: the shares' and one more for each column tile
 // of each sequence, or everyone's at the longest in the smallest shares.
+// 32 columns where a sequence has more than 16 on average: five rows of four query heads over 16 caches 134 us, and 206 in
+// tiles of 16, which read the cache twice. 16 columns leave room for a third workgroup on a CU; heads of 256 for no more.
 struct Plan {
   int wide;
   Deal deal;
