@@ -505,9 +505,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(PagedAttnArg
                                [&](int x) { return part.parts > 1 ? ws + (x - c0) * (D + 4) : nullptr; });
 }
 
-// Joins the parts of a row: a workgroup per row and head, D / 4 lanes for a part's row.
+// Joins the parts of a row, of `all`: a workgroup per row and head, D / 4 lanes for a part's row.
 template <class T, int D, int CT>
-__global__ __launch_bounds__(64 * kWaves) void paged_rows_join_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(64 * kWaves) void paged_rows_join_kernel(PagedAttnArgs a, int all) {
   constexpr int L = D / 4, R = 64 * kWaves / L, kWide = 16 * CT;  // lanes of a row, rows at a time
   __shared__ float4 os[R][L];
   __shared__ float ms[R], ls[R];
@@ -524,8 +524,11 @@ __global__ __launch_bounds__(64 * kWaves) void paged_rows_join_kernel(PagedAttnA
   const int2 own = reinterpret_cast<const int2*>(a.work)[b];
   if (own.y <= 1) return;
   const int h = head / a.group, x = token * a.group + head - h * a.group;
+  // Within the workspace: with starts that do not ascend nobody may have written the sequence's numbers, or not all its parts.
+  const int first = own.x + x / kWide, n = min(own.y, (all - 1 - first) / tiles + 1);
+  if (own.x < 0 || first < 0 || first >= all) return;
   const int64_t ld = static_cast<int64_t>(tiles) * a.pool.kv_heads * kWide * (D + 4);
-  const float* ws = parts_at(a) + ((static_cast<int64_t>(own.x + x / kWide) * a.pool.kv_heads + h) * kWide + x % kWide) * (D + 4);
+  const float* ws = parts_at(a) + ((static_cast<int64_t>(first) * a.pool.kv_heads + h) * kWide + x % kWide) * (D + 4);
   float4 y = make_float4(0, 0, 0, 0);
   float m = -INFINITY, sum = 0;
   auto add = [&](float m1, float l1, float4 v) {
@@ -536,7 +539,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_rows_join_kernel(PagedAttnA
     sum = sum * k0 + l1 * k1;
   };
 #pragma unroll 4
-  for (int p = r; p < own.y; p += R) {
+  for (int p = r; p < n; p += R) {
     const float4 v = *reinterpret_cast<const float4*>(ws + p * ld + d);
     const float2 ml = *reinterpret_cast<const float2*>(ws + p * ld + D);
     add(ml.x, ml.y, v);
@@ -584,7 +587,7 @@ template <class T, bool E4M3, int D, int CT>
 hipError_t run(const PagedAttnArgs& a, const Plan& p, hipStream_t s) {
   const dim3 block(64 * kWaves);
   hipLaunchKernelGGL((paged_rows_kernel<T, E4M3, D, CT>), dim3(static_cast<uint32_t>(a.pool.kv_heads * p.parts)), block, 0, s, a, p.deal);
-  if (p.split) hipLaunchKernelGGL((paged_rows_join_kernel<T, D, CT>), dim3(a.seqs.rows, a.heads), block, 0, s, a);
+  if (p.split) hipLaunchKernelGGL((paged_rows_join_kernel<T, D, CT>), dim3(a.seqs.rows, a.heads), block, 0, s, a, static_cast<int>(p.parts));
   return hipGetLastError();
 }
 

@@ -335,6 +335,29 @@ def test_lengths_and_starts_out_of_range_are_clamped():
     assert torch.equal(bits(cache.k), bits(before))
 
 
+@pytest.mark.parametrize("seqs", [40, 200])
+@pytest.mark.parametrize("rows", [1, 12, 40])
+def test_starts_that_do_not_ascend_stay_inside_the_calls_buffers(seqs, rows):
+    """Row spans that overlap come to more parts than the sizes allow for; what surrounds the buffers keeps its bits, and a
+    right call after it its results."""
+    layer = Layer(13, [1200] * 3, [rows] * 3, 4, 2, 64)
+    cache, q, table, lens, _ = layer.dev(ops)
+    table, lens = (t.repeat(seqs // 3 + 1, *[1] * (t.dim() - 1))[:seqs].contiguous() for t in (table, lens))
+    q = q.repeat(seqs // 3 + 1, 1)[:rows * seqs].contiguous()
+    good = torch.arange(seqs + 1, dtype=torch.int32).cuda() * rows
+    want = ops.paged_attention(cache, q, table, lens, good).clone()
+    around = torch.full((rows * seqs + 64, q.shape[1]), SENTINEL, dtype=q.dtype, device="cuda")
+    y = around[32:32 + rows * seqs]
+    before = cache.k.clone(), cache.v.clone()
+    ends = torch.tensor([0, rows * seqs], dtype=torch.int32).repeat(seqs // 2 + 1)[:seqs + 1].cuda()
+    for starts in (ends, good.flip(0), ends.flip(0), good * -3, good * 5 - 7):
+        ops.paged_attention(cache, q, table, lens, starts.contiguous(), y=y)
+        torch.cuda.synchronize()
+        assert bool((around[:32] == SENTINEL).all()) and bool((around[32 + rows * seqs:] == SENTINEL).all())
+    assert torch.equal(bits(cache.k), bits(before[0])) and torch.equal(bits(cache.v), bits(before[1]))
+    assert torch.equal(bits(ops.paged_attention(cache, q, table, lens, good)), bits(want))
+
+
 # ------------------------------------------------------------------------------------------------ how calls are made
 def test_empty_calls_do_nothing():
     layer = Layer(1, [5], [5], 2, 1, 64)
