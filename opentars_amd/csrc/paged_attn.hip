@@ -45,31 +45,16 @@ struct Tile {
   int r0;                          // the first of the workgroup's rows among rows * group
 };
 
-// The workgroup's rows: `number` counts M-row tiles over the sequences; within one the last comes first.
+// The workgroup's rows: `number` counts kRowsWg-row tiles over the sequences; within one the last comes first.
 __device__ __forceinline__ Tile find_tile(const KvSeqs& s, int group, int number) {
-  const int lane = threadIdx.x & 63;
-  int before = 0;
-  for (int b0 = 0; b0 < s.seqs; b0 += 64) {
-    const int b = b0 + lane;
-    RowSpan r{0, 0};
-    if (b < s.seqs) r = seq_rows(s.starts, b, s.rows);
-    const int tiles = ceil_div(r.n * group, kRowsWg);
-    const int upto = before + inclusive_sum(tiles);
-    const uint64_t hit = __ballot(upto > number);
-    if (hit) {
-      const int at = __builtin_ctzll(hit);
-      Tile t;
-      t.b = __builtin_amdgcn_readfirstlane(b0 + at);
-      t.first = __builtin_amdgcn_readlane(r.first, at);
-      t.rows = __builtin_amdgcn_readlane(r.n, at);
-      // clamped, for starts that do not ascend: their sums may be anything
-      t.r0 = iclamp(__builtin_amdgcn_readlane(upto, at) - 1 - number, 0, __builtin_amdgcn_readlane(tiles, at) - 1) * kRowsWg;
-      t.len = __builtin_amdgcn_readfirstlane(seq_len(s.lens, t.b, s.cap));
-      return t;
-    }
-    before = __builtin_amdgcn_readlane(upto, 63);
-  }
-  return {-1, 0, 0, 0, 0};
+  Tile t{-1, 0, 0, 0, 0};
+  const int b = count_first(s.seqs, [&](int i) { return tile_first(s.starts, i + 1, s.rows, group, kRowsWg) <= number; });
+  if (b >= s.seqs) return t;
+  const RowSpan r = seq_rows(s.starts, b, s.rows);
+  // among its tiles, also for starts that do not ascend
+  const int tiles = ceil_div(r.n * group, kRowsWg), at = number - tile_first(s.starts, b, s.rows, group, kRowsWg);
+  if (at < 0 || at >= tiles) return t;
+  return {b, r.first, r.n, seq_len(s.lens, b, s.cap), (tiles - 1 - at) * kRowsWg};
 }
 
 template <int D>

@@ -102,18 +102,23 @@ __device__ __forceinline__ void store4(char* row, int at, int f32, float a, floa
   else *reinterpret_cast<uint2*>(row + 2 * at) = make_uint2(T::pair(a, b), T::pair(c, d));
 }
 
-// The sequence that packed row `row` belongs to (seqs: none), the same in every lane: the number of sequences that
-// end at or before it, 64 at a time.
-__device__ __forceinline__ int seq_of_row(const KvSeqs& s, int row) {
+// The number of sequences, of `seqs`, that ended(b) holds for, which holds for the first ones: 64 of every 4096, 64 and 1
+// at a time. Where it does not, any number up to seqs.
+template <class F>
+__device__ __forceinline__ int count_first(int seqs, F ended) {
+  const int lane = threadIdx.x & 63;
   int n = 0;
-  for (int b = 0; b < s.seqs; b += 64) {
-    const int i = b + static_cast<int>(threadIdx.x & 63);
-    const bool ended = i < s.seqs && iclamp(s.starts[i + 1], 0, s.rows) <= row;
-    const int here = __popcll(__ballot(ended));
-    n += here;
-    if (here < 64) break;
+  for (int step = seqs > 4096 ? 4096 : seqs > 64 ? 64 : 1; step; step >>= 6) {
+    const int b = n + (lane + 1) * step - 1;
+    n += step * __popcll(__ballot(b < seqs && ended(min(b, seqs - 1))));
   }
   return __builtin_amdgcn_readfirstlane(n);
+}
+
+// The sequence that packed row `row` belongs to (seqs: none), the same in every lane: the number of sequences that end at
+// or before it.
+__device__ __forceinline__ int seq_of_row(const KvSeqs& s, int row) {
+  return count_first(s.seqs, [&](int b) { return iclamp(s.starts[b + 1], 0, s.rows) <= row; });
 }
 
 // V's infinities and NaN at the positions [k0, k0 + count) of sequence b, which the products left out, added to the outputs

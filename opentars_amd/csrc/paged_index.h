@@ -32,6 +32,13 @@ TARS_HD RowSpan seq_rows(const int32_t* starts, int b, int rows) {
   return {r0, imax(iclamp(starts[b + 1], 0, rows) - r0, 0)};
 }
 
+// Tiles of m rows over the packed rows, each row `group` deep, none with rows of two sequences: those of sequence b are
+// numbered from tile_first(b) on. A closed form, in place of a sum over the sequences before: floor(s group / m) + b
+// leaves ceil(n group / m) numbers or one more to a sequence of n rows.
+TARS_HD int tile_first(const int32_t* starts, int b, int rows, int group, int m) {
+  return iclamp(starts[b], 0, rows) * group / m + b;
+}
+
 // Whether the row at position p sees position j >= 0: not ahead of it, and within the window (0: none) or a first token.
 TARS_HD bool sees(int p, int j, int window, int sinks) {
   return j <= p && (window == 0 || j > p - window || j < sinks);

@@ -64,7 +64,7 @@ struct Part {
 };
 
 template <int STEP>
-__device__ __forceinline__ Work work_of(const PagedAttnArgs& a, int b, int wide) {  // wide: a constant
+__device__ __forceinline__ Work work_of(const PagedAttnArgs& a, int b, int wide) {  // wide: a constant; of no sequence: no rows
   Work w{0, 0, 0, 0, {0, 0, 0}};
   if (b >= a.seqs.seqs) return w;
   w.len = seq_len(a.seqs.lens, b, a.seqs.cap);
@@ -76,16 +76,8 @@ __device__ __forceinline__ Work work_of(const PagedAttnArgs& a, int b, int wide)
   return w;
 }
 
-// The share C of a workgroup, the same in every wave.
-template <int STEP>
-__device__ __forceinline__ int share(const PagedAttnArgs& a, int wide, const Deal& deal) {
-  uint64_t mine = 0;
-  for (int b = threadIdx.x & 63; b < a.seqs.seqs; b += 64) {
-    const Work w = work_of<STEP>(a, b, wide);
-    mine += static_cast<uint64_t>(w.steps.n()) * w.tiles;
-  }
-  const auto sum = [&](int from) -> uint64_t { return group_sum<64>(static_cast<int>(mine >> from & 0xFFFFF)); };
-  const uint64_t total = sum(0) + (sum(20) << 20) + (sum(40) << 40);
+// The share C of a workgroup for `total` steps.
+__device__ __forceinline__ int share_of(uint64_t total, const Deal& deal) {
   // in units of 2^20 steps where the sum has more than 31 bits (a share too long is no harm; no sequence has more than
   // 2^26 steps)
   const int up = total < (1ull << 31) ? 0 : 20;
@@ -94,33 +86,86 @@ __device__ __forceinline__ int share(const PagedAttnArgs& a, int wide, const Dea
   const int c = max(static_cast<int>(per(deal.slots)), min(static_cast<int>(per(deal.few)), deal.most_few));
   return max(c, deal.least);
 }
+__device__ __forceinline__ uint64_t steps_of(const Work& w) { return static_cast<uint64_t>(w.steps.n()) * w.tiles; }
+__device__ __forceinline__ uint64_t wave_sum(uint64_t x) {
+  const auto sum = [&](int from) -> uint64_t { return group_sum<64>(static_cast<int>(x >> from & 0xFFFFF)); };
+  return sum(0) + (sum(20) << 20) + (sum(40) << 40);
+}
+__device__ __forceinline__ int parts_of(const Work& w, int c) { return max((w.steps.n() + c - 1) / c, 1); }
 
-// The part numbered idx among all (b < 0: none): a sequence's tiles side by side, then its next part.
+// The part numbered idx of the wave's 64 sequences from b0 on, w a lane's, whose parts end at `upto`.
+__device__ __forceinline__ Part pick(const Work& w, int parts, int upto, int b0, int idx) {
+  const int at = __builtin_ctzll(__ballot(upto > idx));
+  const auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
+  Part p;
+  p.b = __builtin_amdgcn_readfirstlane(b0 + at);
+  p.parts = of(parts);
+  p.work = {of(w.len), of(w.first), of(w.rows), of(w.tiles), {of(w.steps.a), of(w.steps.b0), of(w.steps.b1)}};
+  p.first = of(upto) - p.parts * p.work.tiles;
+  // clamped, for starts that do not ascend: their sums may be anything
+  const int part = p.work.tiles == 1 ? idx - p.first : (idx - p.first) / p.work.tiles;
+  p.part = iclamp(part, 0, p.parts - 1);
+  p.tile = iclamp(idx - p.first - part * p.work.tiles, 0, p.work.tiles - 1);
+  return p;
+}
+
+// The part numbered idx among all (b < 0: none), the same in every wave: a sequence's tiles side by side, then its next
+// part. Up to 64 sequences are every wave's, a lane to each; of more, each wave takes its 64 in turn (250k positions of one
+// K / V head of 128 in 64 caches 28.7 us, in 1024 39 us, in 4096 92 us; 54 and 181 us where every wave went through all).
 template <int STEP>
-__device__ __forceinline__ Part find_part(const PagedAttnArgs& a, int wide, int c, int idx) {
-  const int lane = threadIdx.x & 63;
+__device__ __forceinline__ Part find_part(const PagedAttnArgs& a, int wide, const Deal& deal, int idx) {
+  const Part none{-1, 0, 0, 0, 0, {0, 0, 0, 0, {0, 0, 0}}};
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (a.seqs.seqs <= 64) {
+    const Work w = work_of<STEP>(a, lane, wide);
+    const int c = share_of(wave_sum(steps_of(w)), deal);
+    const int parts = parts_of(w, c), upto = inclusive_sum(parts * w.tiles);
+    return idx < __builtin_amdgcn_readlane(upto, 63) ? pick(w, parts, upto, 0, idx) : none;
+  }
+  __shared__ uint64_t sums[kWaves];
+  __shared__ int counts[2][kWaves];
+  __shared__ Part found;
+  uint64_t mine = 0;
+  for (int b0 = 64 * wave; b0 < a.seqs.seqs; b0 += 64 * kWaves) mine += steps_of(work_of<STEP>(a, b0 + lane, wide));
+  mine = wave_sum(mine);
+  if (lane == 0) sums[wave] = mine;
+  __syncthreads();
+  uint64_t total = 0;
+#pragma unroll
+  for (int x = 0; x < kWaves; ++x) total += sums[x];
+  const int c = share_of(total, deal);
   int before = 0;
-  for (int b0 = 0; b0 < a.seqs.seqs; b0 += 64) {
-    const Work w = work_of<STEP>(a, b0 + lane, wide);
-    const int parts = max((w.steps.n() + c - 1) / c, 1), upto = before + inclusive_sum(parts * w.tiles);
-    const uint64_t hit = __ballot(upto > idx);
-    if (hit) {
-      const int at = __builtin_ctzll(hit);
-      const auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
+  for (int b0 = 0, turn = 0; b0 < a.seqs.seqs; b0 += 64 * kWaves, turn ^= 1) {
+    const Work w = work_of<STEP>(a, b0 + 64 * wave + lane, wide);
+    const int parts = parts_of(w, c), own = inclusive_sum(parts * w.tiles);
+    if (lane == 63) counts[turn][wave] = own;
+    __syncthreads();
+    // the wave whose parts hold it, alike in all of them whatever the counts (starts that do not ascend)
+    int upto = before, start = 0, owner = -1;
+#pragma unroll
+    for (int x = 0; x < kWaves; ++x) {
+      const int n = counts[turn][x];
+      if (owner < 0 && upto <= idx && idx < upto + n) {
+        owner = x;
+        start = upto;
+      }
+      upto += n;
+    }
+    before = upto;
+    owner = __builtin_amdgcn_readfirstlane(owner);
+    if (owner >= 0) {
+      if (wave == owner) {
+        const Part p = pick(w, parts, start + own, b0 + 64 * wave, idx);
+        if (lane == 0) found = p;
+      }
+      __syncthreads();
       Part p;
-      p.b = __builtin_amdgcn_readfirstlane(b0 + at);
-      p.parts = of(parts);
-      p.work = {of(w.len), of(w.first), of(w.rows), of(w.tiles), {of(w.steps.a), of(w.steps.b0), of(w.steps.b1)}};
-      p.first = of(upto) - p.parts * p.work.tiles;
-      // clamped, for starts that do not ascend: their sums may be anything
-      const int part = p.work.tiles == 1 ? idx - p.first : (idx - p.first) / p.work.tiles;
-      p.part = iclamp(part, 0, p.parts - 1);
-      p.tile = iclamp(idx - p.first - part * p.work.tiles, 0, p.work.tiles - 1);
+      for (int x = 0; x < static_cast<int>(sizeof(Part) / 4); ++x)
+        reinterpret_cast<int*>(&p)[x] = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(&found)[x]);
       return p;
     }
-    before = __builtin_amdgcn_readlane(upto, 63);
   }
-  return {-1, 0, 0, 0, 0, {0, 0, 0, 0, {0, 0, 0}}};
+  return none;
 }
 
 __device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
@@ -193,9 +238,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(PagedAttnArg
   __shared__ float ms[kWaves][kWide], ls[kWaves][kWide];
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c = share<kStep>(a, kWide, deal);
   const int number = blockIdx.x / a.pool.kv_heads, h = blockIdx.x % a.pool.kv_heads;
-  const Part part = find_part<kStep>(a, kWide, c, number);
+  const Part part = find_part<kStep>(a, kWide, deal, number);
   if (part.b < 0) return;
   const Steps steps = part.work.steps;
   const int len = part.work.len, p0 = len - part.work.rows;       // the first row's position

@@ -213,6 +213,43 @@ def test_many_sequences():
     prompt(Layer(1, lens, rows, 2, 1, 64))
 
 
+def test_prompts_of_many_sequences():
+    """More sequences than a wave has lanes, some without rows."""
+    g = torch.Generator().manual_seed(5)
+    lens = torch.randint(0, 70, (150,), generator=g).tolist()
+    rows = [0 if i % 7 == 3 else min(n, 20 + i % 30) for i, n in enumerate(lens)]
+    prompt(Layer(2, lens, rows, 4, 1, 64, spare=3))
+
+
+def test_the_slices_of_a_long_batch_give_the_same_rows():
+    """9000 sequences of up to 60 positions, five new rows each (none for some), stored and attended at once, and 30 at a
+    time: no sequence is split here, so every row has the same bits."""
+    seqs, kv, hd, group, page = 9000, 1, 64, 8, 16
+    g = torch.Generator().manual_seed(6)
+    lens = torch.randint(5, 61, (seqs,), generator=g, dtype=torch.int32)
+    rows = torch.where(torch.arange(seqs) % 11 == 5, 0, 5)
+    starts = torch.cat([torch.zeros(1, dtype=torch.int64), rows.cumsum(0)]).to(torch.int32)
+    total = int(starts[-1])
+    table = torch.randperm(4 * seqs, generator=g).to(torch.int32).view(seqs, 4).cuda()
+    k, v = (torch.randn(4 * seqs, kv, page, hd, generator=g).to(torch.bfloat16).cuda() for _ in range(2))
+    new, q = (torch.randn(total + 9, n, generator=g).to(torch.bfloat16).cuda() for n in (2 * kv * hd, group * hd))
+    whole, parts = (ops.PagedCache(k.clone(), v.clone()) for _ in range(2))
+    y = torch.full(q.shape, SENTINEL, dtype=q.dtype, device="cuda")
+    z = y.clone()
+    ld, sd = lens.cuda(), starts.cuda()
+    ops.kv_append(whole, new[:, :hd], new[:, hd:], table, ld, sd)
+    ops.paged_attention(whole, q, table, ld, sd, y=y)
+    for b in list(range(0, 300, 30)) + list(range(4000, 4300, 30)) + list(range(seqs - 300, seqs, 30)):
+        r0, r1 = int(starts[b]), int(starts[b + 30])
+        ops.kv_append(parts, new[r0:r1, :hd], new[r0:r1, hd:], table[b:b + 30], ld[b:b + 30], sd[b:b + 31] - r0)
+        ops.paged_attention(parts, q[r0:r1], table[b:b + 30], ld[b:b + 30], sd[b:b + 31] - r0, y=z[r0:r1])
+        t = table[b:b + 30].flatten().long()
+        assert torch.equal(bits(whole.k[t]), bits(parts.k[t])) and torch.equal(bits(whole.v[t]), bits(parts.v[t]))
+        assert torch.equal(bits(y[r0:r1]), bits(z[r0:r1]))
+    assert bool((y[total:] == SENTINEL).all())
+    assert bool(torch.isfinite(y.float()).all()) and not bool((y[:total] == SENTINEL).all(1).any())
+
+
 # ------------------------------------------------------------------------------------------------ what must not be read
 @pytest.mark.parametrize("hd,cache", [(128, "same"), (64, "e4m3"), (256, "same")])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (20, 4)])

@@ -36,6 +36,9 @@ int main() {
     } else if (what == 'l') {
       const int32_t len = v[0];
       std::printf("%d 0 0\n", seq_len(&len, 0, v[1]));
+    } else if (what == 't') {
+      const int32_t starts[2] = {v[0], v[1]};
+      std::printf("%d %d 0\n", tile_first(starts, 0, v[2], v[3], v[4]), tile_first(starts, 1, v[2], v[3], v[4]));
     } else {
       std::printf("%d 0 0\n", sees(v[0], v[1], v[2], v[3]));
     }
@@ -99,6 +102,19 @@ def test_sees_rows_and_lengths(index):
         lo, hi = min(max(a, 0), n), min(max(b, 0), n)
         assert (first, count) == (lo, max(hi - lo, 0)) and first + count <= n
     assert index([("l", v, 8) for v in bad])[:, 0].tolist() == [min(max(v, 0), 8) for v in bad]
+
+
+def test_every_sequence_has_numbers_for_its_tiles(index):
+    rng = np.random.default_rng(2)
+    rows = 1 << 18
+    cases = [(int(a), int(a + n), rows, int(g), 128) for a, n, g in
+             zip(rng.integers(0, rows // 2, 3000), rng.integers(0, 600, 3000), rng.integers(1, 1025, 3000))]
+    cases += [(0, 1 << 22, 1 << 22, 64, 128), ((1 << 22) - 1, 1 << 22, 1 << 22, 64, 128), (0, 0, 1, 1024, 128)]
+    for (a, b, _, g, m), (first, after, _) in zip(cases, index([("t", *c) for c in cases])):
+        assert first == a * g // m                                     # of sequence 0: no numbers lost before it
+        assert -(-(b - a) * g // m) <= after - first <= -(-(b - a) * g // m) + 1
+    # numbers past the last tile are few: one for each sequence
+    assert index([("t", -5, 2 ** 31 - 1, 100, 3, 128)])[0].tolist() == [0, 300 // 128 + 1, 0]
 
 
 def pool(**kw):
