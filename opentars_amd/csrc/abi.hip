@@ -261,7 +261,7 @@ int paged_attention(const tars_kv_pool* pool, const void* q, int64_t ldq, int32_
     if (hit) return fail(TARS_E_OVERLAP, "the workspace overlaps an input or the output");
   }
   tars::PagedAttnArgs a{c.pool, c.seqs, static_cast<const char*>(q), static_cast<char*>(y), ldq, ldy, dtype, heads,
-                        heads / pool->kv_heads, out == TARS_OUT_FP32, scale, window, sinks, static_cast<float*>(work)};
+                        heads / pool->kv_heads, out == TARS_OUT_FP32, scale, window, sinks, need > 0 ? static_cast<float*>(work) : nullptr};
   hipStream_t s = static_cast<hipStream_t>(stream);
   return launched(decode ? tars::launch_paged_rows(a, s) : tars::launch_paged_attention(a, s));
 }

@@ -408,6 +408,25 @@ def test_empty_calls_do_nothing():
     ops.kv_append(cache, q[:, :64], q[:, :64], table[:0], lens[:0], none)
 
 
+@pytest.mark.parametrize("decode", [0, 1])
+def test_a_workspace_that_no_call_needs_is_left_alone(decode):
+    layer = Layer(2, [40, 17], [1, 1], 2, 1, 64)
+    cache, q, table, lens, starts = layer.dev(ops)
+    assert _lib.lib().tars_paged_workspace(2, 1, 64, 2, 2, table.shape[1], 16, decode) == 0
+    work = torch.full((64,), SENTINEL, device="cuda")
+    y = torch.empty_like(q)
+    args = (cache._ref, q.data_ptr(), 0, 0, 2, 2, y.data_ptr(), 0, OUT_BF16, 0.125, 0, 0, table.data_ptr(), 0, table.shape[1],
+            lens.data_ptr())
+    stream = torch.cuda.current_stream().cuda_stream
+    lib = _lib.lib()
+    if decode:
+        assert lib.tars_paged_decode(*args, work.data_ptr(), 0, stream) == 0
+    else:
+        assert lib.tars_paged_attention(*args, starts.data_ptr(), 2, work.data_ptr(), 0, stream) == 0
+    compare(y, *layer.want(torch.zeros(y.shape, dtype=y.dtype), scale=0.125))
+    assert bool((work == SENTINEL).all())
+
+
 def test_refusals_of_the_wrappers():
     layer = Layer(1, [5], [5], 4, 2, 64)
     cache, q, table, lens, starts = layer.dev(ops)
