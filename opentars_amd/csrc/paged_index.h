@@ -39,6 +39,15 @@ TARS_HD int tile_first(const int32_t* starts, int b, int rows, int group, int m)
   return iclamp(starts[b], 0, rows) * group / m + b;
 }
 
+// Of n rows' ceil(n group / m) tiles, rows at positions p0 .. p0 + n - 1: how many, the last ones, have their last row
+// behind the first s - 1 steps of `step` positions; all of them for s <= 0.
+TARS_HD int tiles_behind(int s, int p0, int n, int group, int m, int step) {
+  const int tiles = ceil_div(n * group, m);
+  if (s <= 0) return tiles;
+  const int token = imax((s - 1) * step - p0, 0);  // the first row that is
+  return token < n ? tiles - (ceil_div(token * group + 1, m) - 1) : 0;
+}
+
 // Whether the row at position p sees position j >= 0: not ahead of it, and within the window (0: none) or a first token.
 TARS_HD bool sees(int p, int j, int window, int sinks) {
   return j <= p && (window == 0 || j > p - window || j < sinks);

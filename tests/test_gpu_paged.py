@@ -221,6 +221,16 @@ def test_prompts_of_many_sequences():
     prompt(Layer(2, lens, rows, 4, 1, 64, spare=3))
 
 
+@pytest.mark.parametrize("window,sinks", [(0, 0), (70, 3)])
+def test_more_tiles_than_run_at_once(window, sinks):
+    """Prompts of several sequences that come to more workgroups than the GPU holds: they start in the order of their
+    length."""
+    rows = [3, 330, 0, 130, 64, 1, 210, 20, 0, 190, 65, 63]
+    lens = [r + (37 * i) % 90 for i, r in enumerate(rows)]
+    lens[4] = 40                                                        # more new rows than positions
+    prompt(Layer(7, lens, rows, 64, 32, 64, spare=2), window=window, sinks=sinks)
+
+
 def test_the_slices_of_a_long_batch_give_the_same_rows():
     """9000 sequences of up to 60 positions, five new rows each (none for some), stored and attended at once, and 30 at a
     time: no sequence is split here, so every row has the same bits."""

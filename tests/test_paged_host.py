@@ -39,6 +39,8 @@ int main() {
     } else if (what == 't') {
       const int32_t starts[2] = {v[0], v[1]};
       std::printf("%d %d 0\n", tile_first(starts, 0, v[2], v[3], v[4]), tile_first(starts, 1, v[2], v[3], v[4]));
+    } else if (what == 'b') {
+      std::printf("%d 0 0\n", tiles_behind(v[0], v[1], v[2], v[3], v[4], v[5]));
     } else {
       std::printf("%d 0 0\n", sees(v[0], v[1], v[2], v[3]));
     }
@@ -115,6 +117,19 @@ def test_every_sequence_has_numbers_for_its_tiles(index):
         assert -(-(b - a) * g // m) <= after - first <= -(-(b - a) * g // m) + 1
     # numbers past the last tile are few: one for each sequence
     assert index([("t", -5, 2 ** 31 - 1, 100, 3, 128)])[0].tolist() == [0, 300 // 128 + 1, 0]
+
+
+def test_tiles_behind_a_step(index):
+    rng = np.random.default_rng(3)
+    cases = [(int(s), int(p0), int(n), int(g), int(m), int(step)) for s, p0, n, g, m, step in
+             zip(rng.integers(-1, 20, 4000), rng.integers(-70, 300, 4000), rng.integers(0, 300, 4000),
+                 rng.choice([1, 2, 3, 8, 40, 200], 4000), rng.choice([16, 128], 4000), rng.choice([32, 64], 4000))]
+    for (s, p0, n, g, m, step), (got, _, _) in zip(cases, index([("b", *c) for c in cases])):
+        last = [min(((t + 1) * m - 1) // g, n - 1) for t in range(-(-n * g // m))]
+        assert got == (len(last) if s <= 0 else sum(p0 + x >= (s - 1) * step for x in last)), (s, p0, n, g, m, step)
+    top = 2 ** 30                                                       # the longest cache, the most rows
+    assert index([("b", top // 64, top - 2 ** 22, 2 ** 22, 64, 128, 64), ("b", top // 64 + 2, top - 2 ** 22, 2 ** 22, 64, 128, 64),
+                  ("b", 1, top - 2 ** 22, 2 ** 22, 64, 128, 64)])[:, 0].tolist() == [32, 0, 2 ** 21]
 
 
 def pool(**kw):
