@@ -562,15 +562,18 @@ struct Plan {
   int64_t tiles;
   bool sorted;
 };
-// Rows that make fewer than 256 workgroups are split until there are up to 512, two on every CU, in parts of kLeast tiles
-// or more: 256 rows of 16 heads behind 30000 85 us (up to 256: 100, 1024: 108), 40 behind 3000 20.3 us (8 tiles: 23.1).
+// Few workgroups are split until there are up to 512, two on every CU, in parts of kLeast tiles or more: 256 rows of 16
+// heads behind 30000 85 us (up to 256: 100, 1024: 108), 40 behind 3000 20.3 us (8 tiles: 23.1). Of heads of 256, whose
+// workgroups have twice the waves, a CU holds one: 128 rows of 16 heads behind 8000 41 us (up to 512: 58), 256 behind
+// 30000 175 us (193).
+constexpr int resident(int hd) { return hd == 256 ? 256 : 512; }
 constexpr int kLeast = 4;
 Plan plan(int heads, int kv_heads, int hd, int rows, int seqs, int cap) {
   const int group = heads / kv_heads;
   const int64_t full = (static_cast<int64_t>(rows) * group + kRowsWg - 1) / kRowsWg;
   const int64_t wgs = std::max<int64_t>(full, std::min(rows, seqs)) * kv_heads;
   const int64_t most = std::max(ceil_div(cap, tile_of(hd)) / kLeast, 1);
-  return {static_cast<int>(std::clamp<int64_t>(512 / wgs, 1, std::min<int64_t>(most, 64))), full + seqs, wgs > 512 && seqs > 1 && seqs <= 64};
+  return {static_cast<int>(std::clamp<int64_t>(resident(hd) / wgs, 1, std::min<int64_t>(most, 64))), full + seqs, wgs > 512 && seqs > 1 && seqs <= 64};
 }
 
 template <class T, bool E4M3, int D>
