@@ -47,6 +47,10 @@ constexpr int kWaves = 4;
 // is better for one long cache: 8k 15.0 and 13.1). A share has a step for each wave at least: one cache of 4k 10.9 us
 // (12.8 with half of that).
 constexpr int kSlots = 512, kFew = 512, kShort = 512;
+// Caches that may have up to kAlone steps are not split, which spares the second launch: one of 120 positions 7.3 us (8.8),
+// of 300 9.1 us (9.8), of 480 10.4 us (10.2; the host's work is 3 us less), 32 of up to 480 13.1 us (16.3); of 600, whose
+// 19 steps are split, 10.3 us (11.4).
+constexpr int kAlone = 16;
 
 struct Deal {
   int slots, few;        // workgroups for a K / V head, of long and of short work
@@ -620,6 +624,7 @@ Plan plan(int kv_heads, int group, int hd, int rows, int seqs, int cap, bool one
   int64_t longest = ceil_div(cap, step);
   if (window > 0 && one_each)
     longest = std::min<int64_t>(longest, window / step + 2 + ceil_div(std::min(sinks, cap), step));
+  if (longest <= kAlone) p.deal.least = std::max<int>(longest, p.deal.least);
   const int64_t most = (longest + p.deal.least - 1) / p.deal.least;
   p.split = most > 1;
   const int64_t tiles = rows == seqs ? int64_t{seqs} * ceil_div(group, p.wide) : static_cast<int64_t>(rows) * group / p.wide + seqs;
