@@ -552,6 +552,14 @@ class PagedCache:
         self._ref = ctypes.byref(self._pool)
 
 
+def _row_stride(t: torch.Tensor, rows: int, cols: int, size: int) -> int:
+    """_ld for a 2-D tensor of known shape; 0, dense, for one row, and refused for rows that are one and the same."""
+    ld, one = t.stride()
+    if (one != 1 and cols > 1) or (ld == 0 and rows > 1):
+        raise ValueError("expected a 2-D tensor with contiguous rows of their own")
+    return size * ld if rows > 1 else 0
+
+
 def _paged_rows(cache: PagedCache, t: torch.Tensor, what: str):
     """The element code, shape and row stride (bytes) of a call's packed rows, which must lie on the cache's GPU."""
     code = _KV_DTYPES.get(t.dtype)
@@ -561,10 +569,8 @@ def _paged_rows(cache: PagedCache, t: torch.Tensor, what: str):
         raise ValueError(f"{what} must live on the cache's GPU")
     if t.dim() != 2:
         raise ValueError("expected a 2-D tensor with contiguous rows")
-    (rows, cols), (ld, one) = t.shape, t.stride()
-    if one != 1 and cols > 1:
-        raise ValueError("expected a 2-D tensor with contiguous rows")
-    return code, rows, cols, 2 * ld
+    rows, cols = t.shape
+    return code, rows, cols, _row_stride(t, rows, cols, 2)
 
 
 def _paged_meta(cache: PagedCache, table: torch.Tensor, lens: torch.Tensor, starts: torch.Tensor | None):
@@ -577,16 +583,15 @@ def _paged_meta(cache: PagedCache, table: torch.Tensor, lens: torch.Tensor, star
         raise ValueError("the cache's GPU must be the current device")
     if table.dim() != 2 or lens.dim() != 1:
         raise ValueError("table must be [seqs, table_pages] and lens [seqs]")
-    (seqs, pages), (ld, one) = table.shape, table.stride()
-    if one != 1 and pages > 1:
-        raise ValueError("expected a 2-D tensor with contiguous rows")
+    seqs, pages = table.shape
+    ld = _row_stride(table, seqs, pages, 4)
     if lens.shape[0] != seqs:
         raise ValueError("table must have a row for each sequence")
     _vec(lens, seqs, "lens")
     if starts is not None:
         _vec(starts, seqs + 1, "starts")
-        return table.data_ptr(), 4 * ld, pages, lens.data_ptr(), starts.data_ptr(), seqs
-    return table.data_ptr(), 4 * ld, pages, lens.data_ptr(), None, seqs
+        return table.data_ptr(), ld, pages, lens.data_ptr(), starts.data_ptr(), seqs
+    return table.data_ptr(), ld, pages, lens.data_ptr(), None, seqs
 
 
 @functools.lru_cache(maxsize=1024)
@@ -637,7 +642,7 @@ def _paged(cache: PagedCache, q: torch.Tensor, table, lens, starts, scale, windo
             out = OUT_FP32 if is_f32 else _KV_OUT[code]
         elif is_f32 != (out == OUT_FP32):
             raise ValueError("y must have the type that out names")
-        ldy = _ld(y)
+        ldy = _row_stride(y, rows, cols, 4 if is_f32 else 2)
     if rows == 0 or seqs == 0:
         return y
     lib = _lib.lib()

@@ -437,6 +437,27 @@ def test_a_workspace_that_no_call_needs_is_left_alone(decode):
     assert bool((work == SENTINEL).all())
 
 
+def test_rows_that_are_one_and_the_same_are_refused():
+    """A broadcast row has no stride of its own, which a stride of 0 (dense) would read past; one row alone is fine."""
+    layer = Layer(1, [5, 9, 7], [1, 1, 1], 2, 1, 64)
+    cache, q, table, lens, starts = layer.dev(ops)
+    same, pages = q[:1].expand(3, -1), table[:1].expand(3, -1)
+    for call in (lambda: ops.paged_decode(cache, same, table, lens), lambda: ops.paged_decode(cache, q, pages, lens),
+                 lambda: ops.paged_decode(cache, q, table, lens, y=same), lambda: ops.paged_decode(cache, q, table, lens[:1].expand(3)),
+                 lambda: ops.paged_attention(cache, same, table, lens, starts),
+                 lambda: ops.paged_attention(cache, q, table, lens, starts[:1].expand(4)),
+                 lambda: ops.kv_append(cache, same[:, :64], q[:, :64], table, lens),
+                 lambda: ops.kv_append(cache, q[:, :64], same[:, :64], table, lens),
+                 lambda: ops.kv_append(cache, q[:, :64], q[:, :64], pages, lens)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(ValueError):
+        ops.paged_decode(cache, q[0], table, lens)
+    want = ops.paged_decode(cache, q, table, lens)
+    one = torch.as_strided(q, (1, q.shape[1]), (1, 1)), torch.as_strided(table, (1, table.shape[1]), (0, 1))   # any stride
+    assert torch.equal(bits(ops.paged_decode(cache, *one, lens[:1])), bits(want[:1]))
+
+
 def test_refusals_of_the_wrappers():
     layer = Layer(1, [5], [5], 4, 2, 64)
     cache, q, table, lens, starts = layer.dev(ops)
