@@ -418,6 +418,30 @@ def test_empty_calls_do_nothing():
     ops.kv_append(cache, q[:, :64], q[:, :64], table[:0], lens[:0], none)
 
 
+@pytest.mark.parametrize("window", [0, 300])
+@pytest.mark.parametrize("rows,heads,kv,hd", [
+    ([1, 1, 1, 1], 8, 2, 128), ([4, 0, 0, 0], 24, 2, 64), ([0, 3, 0, 1], 12, 1, 128), ([9, 1, 17, 0], 8, 8, 64),
+    ([6, 2, 5, 8], 16, 4, 256), ([40, 0, 90, 3], 8, 2, 64), ([200, 130, 1, 0], 4, 2, 128), ([70, 0, 0, 66], 6, 3, 256)])
+def test_the_workspace_is_as_large_as_the_calls_use(rows, heads, kv, hd, window):
+    """What lies behind it keeps its bits, however the rows are spread over the sequences."""
+    layer = Layer(14, [2600, 700, 3300, 90], rows, heads, kv, hd)
+    cache, q, table, lens, starts = layer.dev(ops)
+    lib, n, stream = _lib.lib(), sum(rows), torch.cuda.current_stream().cuda_stream
+    y = torch.full(q.shape, SENTINEL, dtype=q.dtype, device="cuda")
+    for decode in [0, 1] if rows == [1, 1, 1, 1] else [0]:
+        need = lib.tars_paged_workspace(heads, kv, hd, n, 4, table.shape[1], 16, decode)
+        assert need % 16 == 0
+        work = torch.full((need // 4 + 4096,), SENTINEL, device="cuda")
+        args = (cache._ref, q.data_ptr(), 0, 0, heads, n, y.data_ptr(), 0, OUT_BF16, hd ** -0.5, window, 3, table.data_ptr(), 0,
+                table.shape[1], lens.data_ptr())
+        if decode:
+            assert lib.tars_paged_decode(*args, work.data_ptr(), need, stream) == 0
+        else:
+            assert lib.tars_paged_attention(*args, starts.data_ptr(), 4, work.data_ptr(), need, stream) == 0
+        assert bool((work[need // 4:] == SENTINEL).all())
+        compare(y, *layer.want(torch.zeros(y.shape, dtype=y.dtype), window=window, sinks=3 if window else 0))
+
+
 @pytest.mark.parametrize("decode", [0, 1])
 def test_a_workspace_that_no_call_needs_is_left_alone(decode):
     layer = Layer(2, [40, 17], [1, 1], 2, 1, 64)
@@ -510,6 +534,24 @@ def test_another_stream():
     for y in (a, b, c):
         compare(y, want, tol)
     assert torch.equal(a, c)
+
+
+def test_calls_on_two_streams_at_once():
+    layers = [Layer(15 + i, [3000 + 500 * i, 40, 1500], [1, 1, 1], 8, 2, 128) for i in range(2)]
+    prompts = [Layer(17 + i, [900, 2000], [5, 60 + i], 8, 2, 128) for i in range(2)]
+    calls = [(*a.dev(ops), *b.dev(ops)) for a, b in zip(layers, prompts)]
+    want = [(ops.paged_decode(*c[:4]), ops.paged_attention(*c[5:])) for c in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, (s, c) in enumerate(zip(streams, calls)):
+            with torch.cuda.stream(s):
+                got[i].append((ops.paged_decode(*c[:4]), ops.paged_attention(*c[5:])))
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        for pair in g:
+            assert all(torch.equal(bits(x), bits(y)) for x, y in zip(w, pair))
 
 
 def test_two_captured_graphs_replayed_between_eager_calls():
