@@ -364,8 +364,8 @@ int64_t tars_paged_workspace(int32_t heads, int32_t kv_heads, int32_t hd, int32_
  * 0; rows behind the last sequence are left as they were.
  *   q [rows, heads * hd] at ldq, BF16 or FP16; query head h reads K / V head h / (heads / kv_heads).
  *   y [rows, heads * hd] at ldy, out = FP32 or q's type (BF16 / FP16). fp32 scores, maxima and sums;
- *   the softmax's numerators are rounded to q's type for the product with V (where a sequence's rows
- *   times heads / kv_heads come to 32 or fewer on average, to the sum of two values of it).
+ *   the softmax's numerators are rounded to q's type for the product with V (for few rows, or few over
+ *   a short cache, to the sum of two values of it).
  *   0 < scale <= 1e30; work: tars_paged_workspace bytes, 16-byte aligned, for this call until it is done.
  */
 int tars_paged_attention(const tars_kv_pool* pool, const void* q, int64_t ldq, int32_t dtype,

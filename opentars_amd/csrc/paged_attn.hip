@@ -26,8 +26,8 @@
 // with zeros for data; the library's bf16 product of 8192 x 8192 x 8192 runs at 1.23 to 1.35); 2000 rows behind 14000 of
 // 16 heads 268 us, 0.92 PF/s; heads of 256, 16 of them, 619 us, 0.89 PF/s, the reads of K and V from LDS beside the
 // products, and 748 us over an e4m3 pool, whose widening adds to them. Few workgroups are bound by their number: two
-// chunks of 2000 to 3001 rows, heads of 256 with a window of 1024 in e4m3, 316 on 256 CUs, 126 us; 77 rows behind 300,
-// six tiles one after another, 13.3 us.
+// chunks of 2000 to 3001 rows, heads of 256 with a window of 1024 in e4m3, 316 on 256 CUs, 126 us; 400 rows of 16 heads
+// of 64, seven tiles one after another, 12.6 us.
 #include <algorithm>
 
 #include "paged_device.h"
@@ -563,7 +563,9 @@ struct Plan {
   bool sorted;
 };
 // Few workgroups are split until there are up to 512, two on every CU, in parts of kLeast tiles or more: 256 rows of 16
-// heads behind 30000 85 us (up to 256: 100, 1024: 108), 40 behind 3000 20.3 us (8 tiles: 23.1). Of heads of 256, whose
+// heads behind 30000 85 us (up to 256: 100, 1024: 108), 40 behind 3000 20.3 us (8 tiles: 23.1); two parts are not worth
+// the second launch (480 rows, 16 heads of 64: 14.0 us in one, 18.5 in two), three are (80 rows behind 600: 15.9, 18.1 in
+// one). Of heads of 256, whose
 // workgroups have twice the waves, a CU holds one: 128 rows of 16 heads behind 8000 41 us (up to 512: 58), 256 behind
 // 30000 175 us (193).
 constexpr int resident(int hd) { return hd == 256 ? 256 : 512; }
@@ -572,7 +574,8 @@ Plan plan(int heads, int kv_heads, int hd, int rows, int seqs, int cap) {
   const int group = heads / kv_heads;
   const int64_t full = (static_cast<int64_t>(rows) * group + kRowsWg - 1) / kRowsWg;
   const int64_t wgs = std::max<int64_t>(full, std::min(rows, seqs)) * kv_heads;
-  const int64_t most = std::max(ceil_div(cap, tile_of(hd)) / kLeast, 1);
+  const int tiles = ceil_div(cap, tile_of(hd));
+  const int64_t most = tiles <= 2 * kLeast ? 1 : tiles / kLeast;
   return {static_cast<int>(std::clamp<int64_t>(resident(hd) / wgs, 1, std::min<int64_t>(most, 64))), full + seqs, wgs > 512 && seqs > 1 && seqs <= 64};
 }
 
@@ -594,17 +597,25 @@ hipError_t go(const PagedAttnArgs& a, hipStream_t s) {
 }  // namespace
 
 // Sequences of 32 columns or fewer on average go to the kernel for few rows: 16 caches of 3k to 16k with 20 columns 134 us
-// and 148 here, with 32 143 and 150, with 64 233 and 157.
-static bool few_rows(int group, int rows, int seqs) { return static_cast<int64_t>(rows) * group <= 32ll * seqs; }
+// and 148 here, with 32 143 and 150, with 64 233 and 157. So do short caches of five tiles or more with rows for a quarter of
+// their positions at most, where this kernel's tiles follow one another in few workgroups and that one has one for each 32
+// (16) columns: 77 rows behind 300, 16 heads of 64, 10.5 us (13.4), of 128 13.4 us (17.8), 8 of 256 14.6 us (19.0). With
+// rows for all positions, or fewer tiles, it is the other way round (400 rows: 14.9 and 12.6 here, 20: 8.3 and 7.6).
+constexpr int kShort = 256, kShortCap = 512, kShortWgs = 512;
+static bool few_rows(int group, int kv_heads, int hd, int rows, int seqs, int cap) {
+  const int64_t columns = static_cast<int64_t>(rows) * group;
+  return columns <= 32ll * seqs || (cap > kShort && cap <= kShortCap && 4ll * rows <= static_cast<int64_t>(cap) * seqs &&
+                                    (columns / (hd == 256 ? 16 : 32) + seqs) * kv_heads <= kShortWgs);
+}
 
 int64_t paged_workspace(int heads, int kv_heads, int hd, int rows, int seqs, int cap, bool decode) {
-  if (decode || few_rows(heads / kv_heads, rows, seqs)) return paged_rows_workspace(heads, kv_heads, hd, rows, seqs, cap);
+  if (decode || few_rows(heads / kv_heads, kv_heads, hd, rows, seqs, cap)) return paged_rows_workspace(heads, kv_heads, hd, rows, seqs, cap);
   const Plan p = plan(heads, kv_heads, hd, rows, seqs, cap);
   return p.splits > 1 ? int64_t{4} * p.splits * rows * heads * (hd + 4) : 0;
 }
 
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t s) {
-  if (few_rows(a.group, a.seqs.rows, a.seqs.seqs)) return launch_paged_rows(a, s);
+  if (few_rows(a.group, a.pool.kv_heads, a.pool.hd, a.seqs.rows, a.seqs.seqs, a.seqs.cap)) return launch_paged_rows(a, s);
   const bool e4m3 = a.pool.dtype == KV_E4M3;
   if (a.dtype == KV_BF16) return e4m3 ? go<Bf16, true>(a, s) : go<Bf16, false>(a, s);
   return e4m3 ? go<Fp16, true>(a, s) : go<Fp16, false>(a, s);

@@ -1,5 +1,6 @@
-// Attention of few rows per sequence over the paged cache, split over the caches' lengths and joined: decode, and packed
-// rows that come to 32 columns or fewer a sequence (a column is a row of one query head of a K / V head).
+// Attention of few rows per sequence over the paged cache, split over the caches' lengths and joined: decode, packed rows
+// that come to 32 columns or fewer a sequence (a column is a row of one query head of a K / V head), and some over short
+// caches.
 //
 // Per sequence and K / V head the cache is read once for the columns that share it, 16 or 32 of them, a step of 32
 // positions at a time. Both products run on matrix instructions with the positions as rows, so that nothing passes

@@ -221,6 +221,14 @@ def test_prompts_of_many_sequences():
     prompt(Layer(2, lens, rows, 4, 1, 64, spare=3))
 
 
+@pytest.mark.parametrize("heads,kv,hd,qt,cache", [(16, 4, 64, "fp16", "same"), (16, 2, 128, "bf16", "same"),
+                                                  (6, 2, 128, "bf16", "e4m3"), (8, 2, 256, "bf16", "same"), (2, 2, 256, "fp16", "e4m3")])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (90, 3)])
+def test_some_rows_behind_short_caches(heads, kv, hd, qt, cache, window, sinks):
+    layer = Layer(21, [301, 77, 0, 290, 310, 5], [61, 77, 0, 1, 40, 9], heads, kv, hd, qt=qt, cache=cache, spare=2)
+    prompt(layer, window=window, sinks=sinks)
+
+
 @pytest.mark.parametrize("window,sinks", [(0, 0), (70, 3)])
 def test_more_tiles_than_run_at_once(window, sinks):
     """Prompts of several sequences that come to more workgroups than the GPU holds: they start in the order of their
