@@ -30,7 +30,7 @@
 // (a plain read of memory comes to 6.0 to 6.4); 64 of up to 8k 174 to 180 us, 5.7 TB/s; 32 of 9k to 17k in e4m3 with
 // 64 query heads 162 us, 5.4 TB/s, the widening of K and V beside the loads; 16 of 3k to 16k with five rows each (32
 // columns, two workgroups on a CU instead of three) 134 us, 4.8 TB/s. Short work is bound by the chain launch -> lengths
-// -> page numbers -> K and V -> second launch: one cache of 2k 10.8 us, of 300 10.0 us; 100 windows of 512, one K / V
+// -> page numbers -> K and V -> second launch: one cache of 2k 10.8 us, of 300 9.1 us; 100 windows of 512, one K / V
 // head of 256, 19.7 us.
 #include <algorithm>
 
