@@ -42,11 +42,11 @@ namespace {
 // Positions that a wave takes at a time: 16 for heads of 256, whose K and V rows fill the registers.
 constexpr int step_of(int hd) { return hd == 256 ? 16 : 32; }
 constexpr int kWaves = 4;
-// Long work is dealt to two rounds of the workgroups that the CUs hold, kSlots for each that a CU holds: three to a CU
-// 64 caches of up to 8k 174 us and three of 110k 231 us (one round less 175 and 246, one more 177 and 241). Short work,
-// shares of up to kShort positions, is dealt to two workgroups on a CU: 100 windows of 512 13.9 us (16.4 with one, which
-// is better for one long cache: 8k 15.0 and 13.1). A share has a step for each wave at least: one cache of 4k 10.9 us
-// (12.8 with half of that).
+// Long work is dealt to two rounds of three workgroups on every CU, of two with 32 columns (kSlots for each): 64 caches of
+// up to 8k 174 us and three of 110k 231 us (in 1024 workgroups 175 and 246, in 2048 173 and 234). Heads of 256, of which a
+// CU holds two, take the same: 172 and 235 us (in 1024: 176 and 225). Short work, shares of up to kShort positions, is
+// dealt to two workgroups on a CU: 100 windows of 512 13.9 us (16.4 with one, which is better for one long cache: 8k 15.0
+// and 13.1). A share has a step for each wave at least: one cache of 4k 10.9 us (12.8 with half of that).
 constexpr int kSlots = 512, kFew = 512, kShort = 512;
 // Caches that may have up to kAlone steps are not split, which spares the second launch: one of 120 positions 7.3 us (8.8),
 // of 300 9.1 us (9.8), of 480 10.4 us (10.2; the host's work is 3 us less), 32 of up to 480 13.1 us (16.3); of 600, whose
