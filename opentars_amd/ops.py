@@ -520,6 +520,14 @@ def embed_rows(table, ids, scale=None, y=None):
 # ---------------------------------------------------------------- paged key / value cache
 _KV_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.int16: 1, torch.float8_e4m3fn: 2}
 _KV_OUT = {0: OUT_BF16, 1: OUT_FP16}
+_INT32_MAX = 2 ** 31 - 1
+
+
+def _fit_int32(*values: int) -> None:
+    """The C ABI's sizes are 32 bits wide, and ctypes cuts a longer integer to its low 32 bits: a window of 2^32 + 5 to
+    one of 5, an out of 2^32 to OUT_FP32, whose rows would pass the end of a 16-bit y."""
+    if max(values) > _INT32_MAX or min(values) < -_INT32_MAX:
+        raise ValueError("sizes, window, sinks and out must fit in 32 bits")
 
 
 class PagedCache:
@@ -538,6 +546,7 @@ class PagedCache:
         if k.numel() == 0 or (k.shape[3] > 1 and (k.stride(3) != 1 or v.stride(3) != 1)):
             raise ValueError("k and v must not be empty and their rows contiguous")
         pages, kv_heads, page, hd = k.shape
+        _fit_int32(*k.shape)
         for t, what in ((kscale, "kscale"), (vscale, "vscale")):
             if t is not None:
                 if t.dtype != torch.float32 or t.device != k.device:
@@ -613,6 +622,7 @@ def kv_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torch.
     if cols != cache.kv_heads * cache.hd:
         raise ValueError("k and v must be [rows, kv_heads * hd]")
     meta = _paged_meta(cache, table, lens, starts)
+    _fit_int32(rows, meta[2], meta[5])
     if rows == 0 or (starts is not None and meta[5] == 0):
         return
     _check(_lib.lib().tars_kv_append(cache._ref, k.data_ptr(), ldk, v.data_ptr(), ldv, code, rows, *meta, _stream()))
@@ -626,6 +636,7 @@ def _paged(cache: PagedCache, q: torch.Tensor, table, lens, starts, scale, windo
         raise ValueError("q must be [rows, heads * hd], heads a multiple of kv_heads")
     meta = _paged_meta(cache, table, lens, starts)
     seqs = meta[5]
+    _fit_int32(rows, seqs, meta[2], window, sinks, 0 if out is None else out)
     if starts is None and rows != seqs:
         raise ValueError("q must have a row for each sequence")
     if y is None:
