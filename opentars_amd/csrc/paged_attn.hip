@@ -494,9 +494,18 @@ __global__ __launch_bounds__(64 * kRowsWg / wave_rows(D), 2) void paged_prompt_k
   __syncthreads();
   if (*reinterpret_cast<volatile int*>(lds[0]) == 0) return;
 
+  // the tiles that is_whole() was false for: by their positions, or by a page outside the pool
+  auto cleaned = [&](int i) {
+    bool whole = static_cast<uint32_t>(i - whole0) < static_cast<uint32_t>(wholes);
+    for (int x = 0; x < kBlocks && whole; ++x) {
+      const int page = a.seqs.table[tile.b * a.seqs.ld_table + min((steps.at(i) * kTile + 16 * x) >> shift, last)];
+      whole = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pool.pages);
+    }
+    return !whole;
+  };
 #pragma unroll 1
   for (int i = t0; i < t1; ++i)
-    if (static_cast<uint32_t>(i - whole0) >= static_cast<uint32_t>(wholes))
+    if (cleaned(i))
       add_unfinite<T, E4M3, D>(a, tile.b, h, tile.len, steps.at(i) * kTile, kTile, p0, tile.first, tile.r0, min(M, total - tile.r0),
                                [&](int x) {
                                  const int t = x / a.group;

@@ -548,10 +548,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(PagedAttnArg
   if (!any) return;
   __syncthreads();
 #pragma unroll 1
-  for (int i = t0; i < t1; ++i)
-    if (!is_whole(i, (1 << kTiles) - 1))
+  for (int i = t0; i < t1; ++i) {
+    Pages p = pages_of(i);
+    check(p);
+    if (!is_whole(i, p.ok))  // as above, the pages included
       add_unfinite<T, E4M3, D>(a, part.b, h, len, steps.at(i) * kStep, kStep, p0, part.work.first, c0, cols,
                                [&](int x) { return part.parts > 1 ? ws + (x - c0) * (D + 4) : nullptr; });
+  }
 }
 
 // Joins the parts of a row, of `all`: a workgroup per row and head, D / 4 lanes for a part's row.
