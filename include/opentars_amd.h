@@ -360,8 +360,10 @@ int64_t tars_paged_workspace(int32_t heads, int32_t kv_heads, int32_t hd, int32_
  * y = softmax(scale q K^T) V for packed rows (prompts, chunks of them, speculative rounds) over the
  * cache, which holds their own K and V already. The row at position p sees the positions j <= p with
  * window == 0, j > p - window or j < sinks (first tokens that stay visible). A position that a row
- * does not see never changes its result, whatever the cache holds there. A row that sees nothing is
- * 0; rows behind the last sequence are left as they were.
+ * does not see never changes its result, whatever the cache holds there. An infinity or NaN of V that
+ * it does see is the result in that column (the sum of them, if there are several), however small its
+ * weight; a NaN among its scores makes the row NaN. A row that sees nothing is 0; rows behind the last
+ * sequence are left as they were.
  *   q [rows, heads * hd] at ldq, BF16 or FP16; query head h reads K / V head h / (heads / kv_heads).
  *   y [rows, heads * hd] at ldy, out = FP32 or q's type (BF16 / FP16). fp32 scores, maxima and sums;
  *   the softmax's numerators are rounded to q's type for the product with V (for few rows, or few over

@@ -16,8 +16,8 @@
 // unrounded values, in fp32.
 //
 // Tiles at a row's own position, at a window's edge or with a page number outside the pool mask their scores. There a
-// hidden position may hold anything: the tile of V is searched for infinities and NaN, which are zeros in the product and
-// are added to the rows that see them at the end.
+// hidden position may hold anything: the tile of V is searched for infinities and NaN, which are zeros in the product. Where
+// one was found, or an output is not finite, the outputs that V's infinities and NaN reach are set to their sum at the end.
 //
 // A workgroup has 128 rows, a wave 32 (16 for heads of 256); the last rows of a sequence, which see most, start first.
 // With few rows their tiles are split over workgroups and joined by a second launch.
@@ -487,6 +487,9 @@ __global__ __launch_bounds__(64 * kRowsWg / wave_rows(D), 2) void paged_prompt_k
       if (part == 0) *reinterpret_cast<float2*>(at + D) = make_float2(l == 0 ? -INFINITY : -minus[0] * sc, l);
     }
   }
+  // In whole tiles V's infinities and NaN met the numerators, some of them rounded to 0: the outputs they reached are not finite.
+  const float mark = mark_of(o);
+  spoiled |= mark != mark;
   __syncthreads();
   if (threadIdx.x == 0) *reinterpret_cast<volatile int*>(lds[0]) = 0;
   __syncthreads();
@@ -494,24 +497,20 @@ __global__ __launch_bounds__(64 * kRowsWg / wave_rows(D), 2) void paged_prompt_k
   __syncthreads();
   if (*reinterpret_cast<volatile int*>(lds[0]) == 0) return;
 
-  // the tiles that is_whole() was false for: by their positions, or by a page outside the pool
-  auto cleaned = [&](int i) {
-    bool whole = static_cast<uint32_t>(i - whole0) < static_cast<uint32_t>(wholes);
-    for (int x = 0; x < kBlocks && whole; ++x) {
-      const int page = a.seqs.table[tile.b * a.seqs.ld_table + min((steps.at(i) * kTile + 16 * x) >> shift, last)];
-      whole = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pool.pages);
-    }
-    return !whole;
+  float* sums = reinterpret_cast<float*>(lds[1]);
+  sums[R * wave + col] = l;
+  __syncthreads();
+  const auto part_row = [&](int x) {
+    const int t = x / a.group;
+    return parts > 1 ? ws + (static_cast<int64_t>(tile.first + t) * a.heads + h * a.group + x - t * a.group) * (D + 4) : nullptr;
   };
+  const auto sound = [&](int x) { return parts > 1 || sums[x - tile.r0] < INFINITY; };
 #pragma unroll 1
-  for (int i = t0; i < t1; ++i)
-    if (cleaned(i))
-      add_unfinite<T, E4M3, D>(a, tile.b, h, tile.len, steps.at(i) * kTile, kTile, p0, tile.first, tile.r0, min(M, total - tile.r0),
-                               [&](int x) {
-                                 const int t = x / a.group;
-                                 return parts > 1 ? ws + (static_cast<int64_t>(tile.first + t) * a.heads + h * a.group + x - t * a.group) * (D + 4)
-                                                  : nullptr;
-                               });
+  for (int turn = 0; turn < 2; ++turn)
+#pragma unroll 1
+    for (int i = t0; i < t1; ++i)
+      add_unfinite<T, E4M3, D>(a, turn == 0, tile.b, h, tile.len, steps.at(i) * kTile, (steps.at(i) + 1) * kTile, p0, tile.first,
+                               tile.r0, min(M, total - tile.r0), part_row, sound);
 }
 
 // Joins the parts of rows whose tiles were split: a workgroup per row and 4 heads, D / 4 lanes of a wave for a head's
@@ -558,6 +557,7 @@ __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedAttnArgs a,
     y.w += __shfl_xor(y.w, i);
     sum += __shfl_xor(sum, i);
   }
+  join_unfinite(y, parts, [&](int p) { return *reinterpret_cast<const float4*>(ws + p * ld + d); });
   const float vs = a.pool.vscale ? a.pool.vscale[h] : 1.0f;
   const float k = sum == 0 ? 0.0f : vs * __builtin_amdgcn_rcpf(sum);
   if (lane < L) store4<T>(a.y + row * a.ldy, head * D + d, a.out_f32, y.x * k, y.y * k, y.z * k, y.w * k);

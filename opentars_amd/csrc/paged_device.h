@@ -121,33 +121,73 @@ __device__ __forceinline__ int seq_of_row(const KvSeqs& s, int row) {
   return count_first(s.seqs, [&](int b) { return iclamp(s.starts[b + 1], 0, s.rows) <= row; });
 }
 
-// V's infinities and NaN at the positions [k0, k0 + count) of sequence b, which the products left out, added to the outputs
-// of the columns [c0, c0 + cols) of K / V head h that see them; column x is query head h * group + x % group of row
-// first + x / group, at position p0 + x / group. part(x): the column's row of a part in the workspace, or null where its
-// output is final. A thread per column of V; all of the workgroup's outputs are written, and the barrier behind that passed.
-template <class T, bool E4M3, int D, class F>
-__device__ void add_unfinite(const PagedAttnArgs& a, int b, int h, int len, int k0, int count, int p0, int first, int c0, int cols,
-                             F part) {
+// NaN if one of the accumulators is not finite, else 0.
+template <class Acc, int N>
+__device__ __forceinline__ float mark_of(const Acc (&o)[N]) {
+  float z[4] = {0, 0, 0, 0};  // four chains
+#pragma unroll
+  for (int t = 0; t < N; ++t)
+#pragma unroll
+    for (int e = 0; e < static_cast<int>(sizeof(Acc) / 4); ++e) z[e & 3] = __builtin_fmaf(o[t][e], 0.0f, z[e & 3]);
+  return z[0] + z[1] + (z[2] + z[3]);
+}
+
+// Four columns y of a row joined from n parts, the parts' own v(p): an infinity of a part whose weight fp32 rounds to 0 made
+// NaN there. A weight is positive: such a column is the sum of the parts' infinities and NaN, if they have any.
+template <class F>
+__device__ __forceinline__ void join_unfinite(float4& y, int n, F v) {
+  if (y.x == y.x && y.y == y.y && y.z == y.z && y.w == y.w) return;
+  const auto add = [](float z, float x) { return x - x == 0 ? z : z + x; };
+  float4 z = make_float4(0, 0, 0, 0);
+#pragma unroll 1
+  for (int p = 0; p < n; ++p) {
+    const float4 x = v(p);
+    z = make_float4(add(z.x, x.x), add(z.y, x.y), add(z.z, x.z), add(z.w, x.w));
+  }
+  y = make_float4(z.x == 0 ? y.x : z.x, z.y == 0 ? y.y : z.y, z.z == 0 ? y.z : z.z, z.w == 0 ? y.w : z.w);
+}
+
+// V's infinities and NaN at the positions [k0, k1), k0 a multiple of 16, of sequence b, in the outputs of the columns [c0, c0 + cols)
+// of K / V head h that see them: clear, then add. What such a value made of an output in the products does not matter (nothing
+// where it was left out, an infinity or NaN otherwise): the output is the sum of those it sees. sound(x): column x has a
+// finite sum of numerators (an output of one that has not stays NaN), or is a row of a part. Column x is query head h *
+// group + x % group of row first + x / group, at position p0 + x / group; part(x): its row of a part in the workspace, or
+// null where its output is final. A thread per column of V, 16 positions of a page at a time; all of the workgroup's
+// outputs are written, and the barrier behind that passed.
+template <class T, bool E4M3, int D, class F, class G>
+__device__ void add_unfinite(const PagedAttnArgs& a, bool clear, int b, int h, int len, int k0, int k1, int p0, int first, int c0,
+                             int cols, F part, G sound) {
   for (int d = threadIdx.x; d < D; d += blockDim.x) {
 #pragma unroll 1
-    for (int j = k0; j < min(k0 + count, len); ++j) {
-      const int page = a.seqs.table[b * a.seqs.ld_table + (j >> a.pool.page_shift)];
+    for (int j0 = k0; j0 < min(k1, len); j0 += 16) {
+      const int page = a.seqs.table[b * a.seqs.ld_table + (j0 >> a.pool.page_shift)];
       if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pool.pages)) continue;
-      const char* at = a.pool.v + h * a.pool.v_head + page * a.pool.v_page + (j & ((1 << a.pool.page_shift) - 1)) * a.pool.v_slot;
-      const uint32_t v = E4M3 ? T::template from_e4m3<false>(reinterpret_cast<const uint8_t*>(at)[d]) & 0xFFFFu
-                              : reinterpret_cast<const uint16_t*>(at)[d];
-      if (!not_finite<T>(v)) continue;
+      const char* at = a.pool.v + h * a.pool.v_head + page * a.pool.v_page + (j0 & ((1 << a.pool.page_shift) - 1)) * a.pool.v_slot;
+      const auto value = [&](int i) {
+        const char* row = at + i * a.pool.v_slot;
+        return E4M3 ? T::template from_e4m3<false>(reinterpret_cast<const uint8_t*>(row)[d]) & 0xFFFFu
+                    : static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[d]);
+      };
+      uint32_t bad = 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) bad |= static_cast<uint32_t>(not_finite<T>(value(i)) != 0) << i;
 #pragma unroll 1
-      for (int x = c0; x < c0 + cols; ++x) {
-        const int t = x / a.group, head = h * a.group + x - t * a.group;
-        if (!sees(p0 + t, j, a.window, a.sinks)) continue;
-        if (float* to = part(x)) {
-          to[d] += T::wide(v);
-        } else if (a.out_f32) {
-          reinterpret_cast<float*>(a.y + (first + t) * a.ldy)[head * D + d] += T::wide(v);
-        } else {
-          uint16_t* y = reinterpret_cast<uint16_t*>(a.y + (first + t) * a.ldy) + head * D + d;
-          *y = static_cast<uint16_t>(T::pair(T::wide(*y) + T::wide(v), 0.0f));
+      for (; bad; bad &= bad - 1) {
+        const int i = __builtin_ctz(bad), j = j0 + i;
+        const float v = T::wide(value(i));
+#pragma unroll 1
+        for (int x = c0; x < c0 + cols; ++x) {
+          const int t = x / a.group, head = h * a.group + x - t * a.group;
+          if (j >= len || !sees(p0 + t, j, a.window, a.sinks) || !sound(x)) continue;
+          if (float* to = part(x)) {
+            to[d] = clear ? 0.0f : to[d] + v;
+          } else if (a.out_f32) {
+            float* y = reinterpret_cast<float*>(a.y + (first + t) * a.ldy) + head * D + d;
+            *y = clear ? 0.0f : *y + v;
+          } else {
+            uint16_t* y = reinterpret_cast<uint16_t*>(a.y + (first + t) * a.ldy) + head * D + d;
+            *y = clear ? 0 : static_cast<uint16_t>(T::pair(T::wide(*y) + v, 0.0f));
+          }
         }
       }
     }

@@ -17,8 +17,9 @@
 // The running maximum is kept per column; accumulators are rescaled only when it grows, which after a few steps is rare.
 // Positions that a column does not see get a numerator of 0, and what nobody in the workgroup sees zeros for V (which may
 // hold anything there). Where some columns see a position and others do not, its infinities and NaN are zeros in the
-// product and are added to the columns that see them at the end. Only steps at the rows' own positions, at the window's
-// edges or with a page number outside the pool pay for that.
+// product. Only steps at the rows' own positions, at the window's edges or with a page number outside the pool pay for that.
+// Where one was found, or an output is not finite, the outputs that V's infinities and NaN reach are set to their sum at the
+// end.
 //
 // The split is made on the device from the lengths: every workgroup adds up the steps of all sequences (those of a
 // sequence once for each of its column tiles), sets the share C of a workgroup so that the shares fill the GPU, and finds
@@ -469,6 +470,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(PagedAttnArg
     step(i, false);
   }
 
+  // V's infinities and NaN in whole steps met the numerators, second halves of 0 or less among them: the outputs they reached
+  // are not finite, and are put right at the end.
+#pragma unroll
+  for (int u = 0; u < CT; ++u) {
+    const float mark = mark_of(o[u]);
+    spoiled |= mark != mark;
+  }
+
   // The waves' parts in one: o[u][e][i] is column 16 u + col's (4 g + i) C + e % C of run e / C.
 #pragma unroll
   for (int u = 0; u < CT; ++u) {
@@ -547,14 +556,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(PagedAttnArg
   }
   if (!any) return;
   __syncthreads();
+  const auto sound = [&](int x) {
+    float sum = 0;
+    for (int w = 0; w < kWaves; ++w) sum += ls[w][x - c0];
+    return part.parts > 1 || sum < INFINITY;
+  };
 #pragma unroll 1
-  for (int i = t0; i < t1; ++i) {
-    Pages p = pages_of(i);
-    check(p);
-    if (!is_whole(i, p.ok))  // as above, the pages included
-      add_unfinite<T, E4M3, D>(a, part.b, h, len, steps.at(i) * kStep, kStep, p0, part.work.first, c0, cols,
-                               [&](int x) { return part.parts > 1 ? ws + (x - c0) * (D + 4) : nullptr; });
-  }
+  for (int turn = 0; turn < 2; ++turn)
+#pragma unroll 1
+    for (int i = t0; i < t1; ++i)
+      add_unfinite<T, E4M3, D>(a, turn == 0, part.b, h, len, steps.at(i) * kStep, (steps.at(i) + 1) * kStep, p0, part.work.first, c0,
+                               cols, [&](int x) { return part.parts > 1 ? ws + (x - c0) * (D + 4) : nullptr; }, sound);
 }
 
 // Joins the parts of a row, of `all`: a workgroup per row and head, D / 4 lanes for a part's row.
@@ -605,6 +617,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_rows_join_kernel(PagedAttnA
   if (r) return;
 #pragma unroll
   for (int i = 1; i < R; ++i) add(ms[i], ls[i], os[i][at]);
+  join_unfinite(y, n, [&](int p) { return *reinterpret_cast<const float4*>(ws + p * ld + d); });
   const float vs = a.pool.vscale ? a.pool.vscale[h] : 1.0f;
   const float k = sum == 0 ? 0.0f : vs * __builtin_amdgcn_rcpf(sum);
   store4<T>(a.y + row * a.ldy, head * D + d, a.out_f32, y.x * k, y.y * k, y.z * k, y.w * k);

@@ -23,13 +23,13 @@ def plant(layer, b, p, head, col, value):
         layer.vpool[page, head, slot, col] = value
 
 
-def check(got, layer, planted, window=0, sinks=0, hidden=()):
+def check(got, layer, planted, window=0, sinks=0, hidden=(), scale=None):
     """planted: (sequence, position, K / V head, column, value). The columns that hold one are the sum of those that the
     row sees; everything else is the definition's."""
     got = got.cpu()
-    want, tol = layer.want(torch.zeros(got.shape), window=window, sinks=sinks, hidden=hidden)
+    want, tol = layer.want(torch.zeros(got.shape, dtype=got.dtype), scale=scale, window=window, sinks=sinks, hidden=hidden)
     group, hd = layer.heads // layer.kv, layer.hd
-    extra = torch.zeros(got.shape)
+    extra = torch.zeros(got.shape, dtype=got.dtype)
     first = 0
     for b, (n, r) in enumerate(zip(layer.lens, layer.rows)):
         for i in range(r):
@@ -60,3 +60,93 @@ def test_beside_a_page_outside_the_pool(n, rows, hd, qt, cache, value):
     cache_, q, table, lens, starts = layer.dev(ops)
     got = ops.paged_attention(cache_, q, table, lens, starts, out=OUT_FP32)
     assert check(got, layer, [(0, 70, 1, 20, value)], hidden=[(0, p) for p in range(80, 96)]) == 2 * rows
+
+
+SHAPES = [(64, "fp16", "same"), (128, "bf16", "same"), (128, "fp16", "e4m3"), (256, "bf16", "same"), (64, "bf16", "e4m3"),
+          (256, "fp16", "same")]
+
+
+def run(layer, decode, dtype, **kw):
+    cache, q, table, lens, starts = layer.dev(ops)
+    y = torch.empty(layer.q.shape, dtype=dtype, device="cuda")
+    return ops.paged_decode(cache, q, table, lens, y=y, **kw) if decode else ops.paged_attention(cache, q, table, lens, starts, y=y, **kw)
+
+
+@pytest.mark.parametrize("hd,qt,cache", SHAPES)
+@pytest.mark.parametrize("n", [30, 300, 3000])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (200, 5)])
+def test_decode_gives_each_column_its_infinities(n, hd, qt, cache, window, sinks):
+    """First, last and middle positions, in one part and in several; two of one sign in a column, and of both."""
+    lens = [n, 1, n - 3]
+    layer = Layer(n + hd, lens, [1, 1, 1], 6, 2, hd, qt=qt, cache=cache)
+    planted = [(0, 0, 0, 3, INF), (0, n - 1, 1, 4, -INF), (0, n // 2, 0, 9, NAN), (0, n - 2, 0, 30, INF), (0, n - 9, 0, 30, INF),
+               (0, n - 2, 0, 31, INF), (0, n - 9, 0, 31, -INF), (2, n - 4, 1, hd - 1, -INF), (2, 7, 1, 0, INF)]
+    planted = [(*x, NAN if cache == "e4m3" else v) for *x, v in planted]
+    for x in planted:
+        plant(layer, *x)
+    for dtype in (torch.float32, layer.qt):
+        got = run(layer, True, dtype, window=window, sinks=sinks)
+        assert check(got, layer, planted, window=window, sinks=sinks) >= 15   # five of the columns at least, three heads each
+
+
+@pytest.mark.parametrize("hd,qt,cache", SHAPES)
+@pytest.mark.parametrize("rows", [3, 8, 100])
+@pytest.mark.parametrize("n", [300, 3000])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (150, 5)])
+def test_rows_give_each_column_its_infinities(n, rows, hd, qt, cache, window, sinks):
+    """The same wherever the position stands: one that every row sees, one of the rows' own, one that leaves the window."""
+    layer = Layer(n + rows + hd, [n, 40], [rows, 2], 4, 2, hd, qt=qt, cache=cache)
+    planted = [(0, 2, 0, 3, INF), (0, n - rows - 20, 1, 4, -INF), (0, n - 2, 0, 9, INF), (0, n - 151, 1, 20, INF), (0, n - 170, 0, 21, NAN),
+               (0, n - rows - 33, 0, 30, INF), (0, n - 1, 0, 30, -INF), (1, 38, 1, hd - 1, -INF)]
+    planted = [(*x, NAN if cache == "e4m3" else v) for *x, v in planted]
+    for x in planted:
+        plant(layer, *x)
+    for dtype in (torch.float32, layer.qt):
+        got = run(layer, False, dtype, window=window, sinks=sinks)
+        assert check(got, layer, planted, window=window, sinks=sinks) > 6 * rows
+
+
+@pytest.mark.parametrize("hd,qt,cache", SHAPES)
+@pytest.mark.parametrize("rows,n", [(1, 300), (1, 4000), (4, 300), (4, 4000), (100, 300), (100, 4000)])
+def test_weights_too_small_for_fp32_are_positive(rows, n, hd, qt, cache):
+    """One position outweighs all others by more than 2^150: the others' numerators, and the weights of the parts without
+    it, round to 0, and an infinity beside them is one all the same."""
+    layer = Layer(rows + n + hd, [n], [rows], 4, 2, hd, qt=qt, cache=cache)
+    u = torch.randn(hd, generator=torch.Generator().manual_seed(3)).sign() * 1.5
+    layer.q[:] = u.to(layer.qt).repeat(layer.heads)
+    loud, k = n - rows - 100, 10.0 * u
+    k = (k / layer.kscale[:, None]).clamp(-448, 448) if cache == "e4m3" else k.repeat(2, 1)
+    k = k.to(layer.ct)
+    page, slot = layer.where[0][loud]
+    layer.kpool.view(torch.uint8 if cache == "e4m3" else layer.ct)[page, :, slot] = k.view(torch.uint8) if cache == "e4m3" else k
+    layer.K[0][loud] = k.double() if cache != "e4m3" else k.double() * layer.kscale.double()[:, None]
+    s = 0.4 * (layer.K[0].transpose(0, 1) @ layer.q[0, :hd].double())
+    assert float(s[:, loud].min() - s[:, torch.arange(n) != loud].max()) > 105              # e^-105 < 2^-150
+    planted = [(0, 5, 0, 3, INF), (0, 40, 1, 4, -INF), (0, loud - 3, 0, 9, NAN), (0, loud, 1, 30, INF)]
+    planted = [(*x, NAN if cache == "e4m3" else v) for *x, v in planted]
+    for x in planted:
+        plant(layer, *x)
+    got = run(layer, rows == 1, torch.float32, scale=0.4)
+    assert check(got, layer, planted, scale=0.4) == 8 * rows
+
+
+@pytest.mark.parametrize("rows,n", [(1, 300), (1, 4000), (4, 300), (4, 4000), (100, 300), (100, 4000)])
+@pytest.mark.parametrize("hd,qt", [(64, "fp16"), (128, "bf16"), (256, "bf16")])
+def test_a_nan_in_k_is_the_rows_result(rows, n, hd, qt):
+    """A row that sees a NaN among its scores is NaN in every column, those with an infinity of V among them; the other K / V
+    head is not touched."""
+    layer = Layer(rows + n, [n], [rows], 4, 2, hd, qt=qt)
+    page, slot = layer.where[0][33]
+    layer.kpool[page, 0, slot, 7] = NAN
+    plant(layer, 0, 50, 0, 3, INF)
+    plant(layer, 0, 50, 1, 4, INF)
+    for dtype in (torch.float32, layer.qt):
+        got = run(layer, rows == 1, dtype).cpu()
+        assert bool(got[:, :2 * hd].isnan().all())
+        got[:, :2 * hd] = 0
+        want, tol = layer.want(torch.zeros(got.shape, dtype=dtype))
+        want[:, :2 * hd] = 0
+        cols = torch.arange(2, 4) * hd + 4
+        assert bool((got[:, cols] == INF).all())
+        got[:, cols], want[:, cols] = 0, 0
+        compare(got, want, tol)
