@@ -36,7 +36,6 @@ namespace tars {
 namespace {
 
 constexpr int tile_of(int hd) { return hd == 256 ? 32 : 64; }  // positions of a tile
-constexpr float kLog2e = 1.44269504f;
 constexpr float kSlack = 6.0f;     // numerators up to 64: their sums and products stay far from fp16's and fp32's limits
 constexpr int kRowsWg = 128;       // rows of a workgroup
 
@@ -159,7 +158,7 @@ __global__ __launch_bounds__(64 * kRowsWg / wave_rows(D), 2) void paged_prompt_k
   const char* q = a.q + (tile.first + token) * a.ldq + 2 * D * head + 16 * part;
 #pragma unroll
   for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const uint4*>(q + 2 * G * s);
-  const float sc = a.scale * kLog2e * (E4M3 && a.pool.kscale ? a.pool.kscale[h] : 1.0f);
+  const float sc = score_scale(a, h);
 
   const int shift = a.pool.page_shift, mask = (1 << shift) - 1, last = max(tile.len - 1, 0) >> shift;
   const char* kbase = a.pool.k + h * a.pool.k_head;
@@ -483,8 +482,8 @@ __global__ __launch_bounds__(64 * kRowsWg / wave_rows(D), 2) void paged_prompt_k
 #pragma unroll
         for (int e = 0; e < N; e += 4)
           *reinterpret_cast<float4*>(at + R * t + e * (64 / R) + 4 * part) = make_float4(o[t][e], o[t][e + 1], o[t][e + 2], o[t][e + 3]);
-      // the maximum in the exponent's units; none seen: the sum is 0 and the maximum counts for nothing
-      if (part == 0) *reinterpret_cast<float2*>(at + D) = make_float2(l == 0 ? -INFINITY : -minus[0] * sc, l);
+      // none seen: the sum is 0 and the maximum counts for nothing
+      if (part == 0) *reinterpret_cast<float2*>(at + D) = make_float2(l == 0 ? -INFINITY : -minus[0], l);
     }
   }
   // In whole tiles V's infinities and NaN met the numerators, some of them rounded to 0: the outputs they reached are not finite.
@@ -534,7 +533,7 @@ __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedAttnArgs a,
   for (int i = lane; i < parts; i += 64) top = fmaxf(top, ws[i * ld + D]);
 #pragma unroll
   for (int i = 1; i < 64; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
-  const float base = top == -INFINITY ? 0.0f : top;
+  const float base = top == -INFINITY ? 0.0f : top, sc = score_scale(a, h);
   const int d = 4 * (lane % L);
   float4 y = make_float4(0, 0, 0, 0);
   float sum = 0;
@@ -542,7 +541,7 @@ __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedAttnArgs a,
   for (int i = lane / L; i < parts; i += R) {
     const float4 v = *reinterpret_cast<const float4*>(ws + i * ld + d);
     const float2 ml = *reinterpret_cast<const float2*>(ws + i * ld + D);
-    const float w = __builtin_amdgcn_exp2f(ml.x - base);
+    const float w = __builtin_amdgcn_exp2f((ml.x - base) * sc);
     y.x += w * v.x;
     y.y += w * v.y;
     y.z += w * v.z;

@@ -83,6 +83,14 @@ __device__ __forceinline__ float over_row(float x, Op op) {
   return op(__uint_as_float(s[0]), __uint_as_float(s[1]));
 }
 
+// What a difference of K / V head h's raw scores is multiplied by to be an exponent of 2: scale times log2(e), and K's scale.
+// Within fp32's normal numbers: at 0 a hidden score, -inf, would be NaN, and at infinity the largest score's distance from
+// itself. The scores are kept raw, and only their differences, 0 or less, multiplied: scale q k itself may pass fp32.
+__device__ __forceinline__ float score_scale(const PagedAttnArgs& a, int h) {
+  const float sc = a.scale * 1.44269504f * (a.pool.kscale ? a.pool.kscale[h] : 1.0f);
+  return sc < 0x1p-126f ? 0x1p-126f : sc > 0x1.fffffep127f ? 0x1.fffffep127f : sc;
+}
+
 // Masks without comparisons, whose results would crowd the scalar registers.
 template <class T>
 __device__ __forceinline__ uint32_t not_finite(uint32_t x) {  // 0xFFFF in each half that is infinite or NaN

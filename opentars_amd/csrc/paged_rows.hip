@@ -276,7 +276,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(PagedAttnArg
       if constexpr (kQLds) *reinterpret_cast<uint4*>(qs + 1024 * s) = make_uint4(qf[0][0][0], qf[0][0][1], qf[0][0][2], qf[0][0][3]);
     }
   }
-  const float sc = a.scale * 1.44269504f * (E4M3 && a.pool.kscale ? a.pool.kscale[h] : 1.0f);
+  const float sc = score_scale(a, h);
 
   const int shift = a.pool.page_shift, mask = (1 << shift) - 1, last = max(len - 1, 0) >> shift;
   const __attribute__((address_space(4))) int32_t* table = reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(
@@ -376,7 +376,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(PagedAttnArg
 #pragma unroll
     for (int u = 0; u < CT; ++u)
 #pragma unroll
-      for (int j = 0; j < NK; ++j) x[u][j] = s[u][j >> 2][j & 3] * sc;
+      for (int j = 0; j < NK; ++j) x[u][j] = s[u][j >> 2][j & 3];
     if (!is_whole(i, cur.ok)) {
       const int k0 = steps.at(i) * kStep;
 #pragma unroll
@@ -413,7 +413,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(PagedAttnArg
       top = over_row<16>(top, [](float y, float z) { return fmaxf(y, z); });
       // by column, not for the wave as a whole: the compiler then scales in place
       if (top > m[u]) {
-        const float keep = __builtin_amdgcn_exp2f(m[u] - top);
+        const float keep = __builtin_amdgcn_exp2f((m[u] - top) * sc);
         m[u] = top;
         l[u] *= keep;
 #pragma unroll
@@ -422,7 +422,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(PagedAttnArg
       const float base = m[u] == -INFINITY ? 0.0f : m[u];   // nothing seen yet: every numerator is 0
 #pragma unroll
       for (int w = 0; w < NK / 2; ++w) {
-        const float y = __builtin_amdgcn_exp2f(x[u][2 * w] - base), z = __builtin_amdgcn_exp2f(x[u][2 * w + 1] - base);
+        const float y = __builtin_amdgcn_exp2f((x[u][2 * w] - base) * sc), z = __builtin_amdgcn_exp2f((x[u][2 * w + 1] - base) * sc);
         l[u] += y + z;
         hi[u][w] = T::pair(y, z);
         lo[u][w] = T::pair(y - T::wide(hi[u][w] & 0xFFFFu), z - T::wide(hi[u][w] >> 16));
@@ -493,7 +493,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(PagedAttnArg
     float top = ms[0][16 * u + col];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) top = fmaxf(top, ms[w][16 * u + col]);
-    const float keep = __builtin_amdgcn_exp2f(top == -INFINITY ? 0.0f : m[u] - top);
+    const float keep = __builtin_amdgcn_exp2f(top == -INFINITY ? 0.0f : (m[u] - top) * sc);
 #pragma unroll
     for (int e = 0; e < E; ++e) o[u][e] *= keep;
   }
@@ -542,7 +542,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(PagedAttnArg
         y.z += v.z;
         y.w += v.w;
       }
-      sum += ls[w][cc] * __builtin_amdgcn_exp2f(top == -INFINITY ? 0.0f : ms[w][cc] - top);
+      sum += ls[w][cc] * __builtin_amdgcn_exp2f(top == -INFINITY ? 0.0f : (ms[w][cc] - top) * sc);
     }
     if (part.parts == 1) {
       const float r = sum == 0 ? 0.0f : vs * __builtin_amdgcn_rcpf(sum);
@@ -595,9 +595,10 @@ __global__ __launch_bounds__(64 * kWaves) void paged_rows_join_kernel(PagedAttnA
   const float* ws = parts_at(a) + ((static_cast<int64_t>(first) * a.pool.kv_heads + h) * kWide + x % kWide) * (D + 4);
   float4 y = make_float4(0, 0, 0, 0);
   float m = -INFINITY, sum = 0;
+  const float sc = score_scale(a, h);
   auto add = [&](float m1, float l1, float4 v) {
     const float top = fmaxf(m, m1), base = top == -INFINITY ? 0.0f : top;
-    const float k0 = __builtin_amdgcn_exp2f(m - base), k1 = __builtin_amdgcn_exp2f(m1 - base);
+    const float k0 = __builtin_amdgcn_exp2f((m - base) * sc), k1 = __builtin_amdgcn_exp2f((m1 - base) * sc);
     m = top;
     y = make_float4(y.x * k0 + v.x * k1, y.y * k0 + v.y * k1, y.z * k0 + v.z * k1, y.w * k0 + v.w * k1);
     sum = sum * k0 + l1 * k1;

@@ -150,3 +150,34 @@ def test_a_nan_in_k_is_the_rows_result(rows, n, hd, qt):
         assert bool((got[:, cols] == INF).all())
         got[:, cols], want[:, cols] = 0, 0
         compare(got, want, tol)
+
+
+# ------------------------------------------------------------------------------------------------ scales
+@pytest.mark.parametrize("rows,n", [(1, 40), (1, 300), (1, 4000), (4, 300), (4, 4000), (100, 300), (100, 4000)])
+@pytest.mark.parametrize("hd,qt", [(64, "fp16"), (128, "bf16"), (256, "bf16")])
+def test_a_scale_that_fp32_rounds_to_nothing(rows, n, hd, qt):
+    """scale times kscale is 1e-50: every visible position counts the same, hidden ones nothing."""
+    layer = Layer(rows + n, [n], [rows], 4, 2, hd, qt=qt, cache="e4m3")
+    layer.kscale[:] = 1e-20
+    got = run(layer, rows == 1, torch.float32, scale=1e-30)
+    compare(got, *layer.want(torch.zeros(got.shape), scale=1e-30))
+
+
+@pytest.mark.parametrize("rows,n", [(1, 40), (1, 300), (1, 4000), (4, 300), (4, 4000), (100, 300), (100, 4000)])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+def test_a_scale_that_takes_scores_past_fp32(rows, n, hd, cache):
+    """Scores of 1e40 and more: the largest has all the weight, so a row is V at that position."""
+    layer = Layer(rows + n + hd, [n], [rows], 4, 2, hd, qt="bf16", cache=cache)
+    u = torch.randn(hd, generator=torch.Generator().manual_seed(3)).sign() * 1e6
+    layer.q[:] = u.to(layer.qt).repeat(layer.heads)
+    loud = n - rows - 17
+    page, slot = layer.where[0][loud]
+    if cache == "e4m3":                                                # of 1e6 hd 448 and 3e38
+        layer.kpool.view(torch.uint8)[page, :, slot] = (u.sign() * 448).to(E4M3).view(torch.uint8)
+        layer.kscale[:] = 1e10
+    else:
+        layer.kpool[page, :, slot] = u.to(layer.qt)
+    got = run(layer, rows == 1, torch.float32, scale=1e30).cpu().double()
+    want = layer.V[0][loud].repeat_interleave(2, 0).reshape(1, -1).expand(rows, -1)
+    assert bool(((got - want).abs() <= 2.0 ** -22 * want.abs()).all())  # the scale's product, a reciprocal of 1
