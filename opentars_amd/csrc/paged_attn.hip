@@ -487,8 +487,7 @@ __global__ __launch_bounds__(64 * kRowsWg / wave_rows(D), 2) void paged_prompt_k
     }
   }
   // In whole tiles V's infinities and NaN met the numerators, some of them rounded to 0: the outputs they reached are not finite.
-  const float mark = mark_of(o);
-  spoiled |= mark != mark;
+  spoiled |= not_all_finite(o);
   __syncthreads();
   if (threadIdx.x == 0) *reinterpret_cast<volatile int*>(lds[0]) = 0;
   __syncthreads();

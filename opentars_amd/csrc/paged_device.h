@@ -129,15 +129,17 @@ __device__ __forceinline__ int seq_of_row(const KvSeqs& s, int row) {
   return count_first(s.seqs, [&](int b) { return iclamp(s.starts[b + 1], 0, s.rows) <= row; });
 }
 
-// NaN if one of the accumulators is not finite, else 0.
+// Whether one of the accumulators is not finite (or their sum is not, of which nothing comes but a search): an infinity or
+// NaN stays one in a sum.
 template <class Acc, int N>
-__device__ __forceinline__ float mark_of(const Acc (&o)[N]) {
+__device__ __forceinline__ bool not_all_finite(const Acc (&o)[N]) {
   float z[4] = {0, 0, 0, 0};  // four chains
 #pragma unroll
   for (int t = 0; t < N; ++t)
 #pragma unroll
-    for (int e = 0; e < static_cast<int>(sizeof(Acc) / 4); ++e) z[e & 3] = __builtin_fmaf(o[t][e], 0.0f, z[e & 3]);
-  return z[0] + z[1] + (z[2] + z[3]);
+    for (int e = 0; e < static_cast<int>(sizeof(Acc) / 4); ++e) z[e & 3] += o[t][e];
+  const float sum = z[0] + z[1] + (z[2] + z[3]);
+  return !(sum - sum == 0);
 }
 
 // Four columns y of a row joined from n parts, the parts' own v(p): an infinity of a part whose weight fp32 rounds to 0 made

@@ -473,10 +473,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(PagedAttnArg
   // V's infinities and NaN in whole steps met the numerators, second halves of 0 or less among them: the outputs they reached
   // are not finite, and are put right at the end.
 #pragma unroll
-  for (int u = 0; u < CT; ++u) {
-    const float mark = mark_of(o[u]);
-    spoiled |= mark != mark;
-  }
+  for (int u = 0; u < CT; ++u) spoiled |= not_all_finite(o[u]);
 
   // The waves' parts in one: o[u][e][i] is column 16 u + col's (4 g + i) C + e % C of run e / C.
 #pragma unroll
