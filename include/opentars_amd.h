@@ -343,7 +343,8 @@ typedef struct tars_kv_pool {
  * dense) of new tokens at their positions; an E4M3 pool gets x / scale rounded to nearest even and
  * saturated (NaN kept). starts NULL: one row for each sequence (rows == seqs). Rows behind the last
  * sequence, at negative positions or on pages outside the pool are not stored. No two rows may have
- * one slot (a table that names a shared page where a sequence writes), and the pools overlap no input.
+ * one slot (a table that names a shared page where a sequence writes), and the pools overlap no input and
+ * not one another (they may interleave: the same strides, or extents that are apart).
  */
 int tars_kv_append(const tars_kv_pool* pool, const void* k, int64_t ldk, const void* v, int64_t ldv,
                    int32_t dtype, int32_t rows, const int32_t* table, int64_t ld_table,

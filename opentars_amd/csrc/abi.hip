@@ -163,6 +163,34 @@ bool strides_ok(int64_t row, const int64_t (&n)[3], const int64_t (&stride)[3], 
   return true;
 }
 
+// The strides of a pool's pages, heads and slots that lead anywhere (a count of one leads nowhere), the widest first, and the
+// bytes from the first row to the end of the last that are left at each.
+struct Levels {
+  int n = 0;
+  int64_t stride[3], count[3], extent[4];
+  Levels(int64_t row, int64_t pages, int64_t heads, int64_t slots, int64_t s0, int64_t s1, int64_t s2) {
+    const int64_t strides[3] = {s0, s1, s2}, counts[3] = {pages, heads, slots};
+    int at[3] = {0, 1, 2};
+    std::sort(at, at + 3, [&](int i, int j) { return strides[i] > strides[j]; });
+    for (int i : at)
+      if (counts[i] > 1) stride[n] = strides[i], count[n++] = counts[i];
+    extent[n] = row;
+    for (int i = n; i-- > 0;) extent[i] = extent[i + 1] + stride[i] * (count[i] - 1);
+  }
+};
+
+// Whether a byte belongs to a row of both, b's first row lying d bytes behind a's. Each stride holds what is within it, so of
+// one stride on both sides only the steps apart that bring the insides together are followed, three at most. Where the strides
+// differ and the extents meet the answer is yes.
+bool meet(const Levels& a, const Levels& b, int64_t d, int i = 0, int j = 0) {
+  if (d >= a.extent[i] || -d >= b.extent[j]) return false;
+  if (i == a.n || j == b.n || a.stride[i] != b.stride[j]) return true;
+  const int64_t s = a.stride[i];
+  for (int64_t k = std::max(-(d / s) - 2, 1 - a.count[i]); k <= std::min(-(d / s) + 2, b.count[j] - 1); ++k)
+    if (meet(a, b, d + k * s, i + 1, j + 1)) return true;
+  return false;
+}
+
 struct PagedCall {
   tars::KvPool pool;
   tars::KvSeqs seqs;
@@ -891,7 +919,11 @@ int tars_kv_append(const tars_kv_pool* pool, const void* k, int64_t ldk, const v
   const int64_t row = 2LL * pool->kv_heads * pool->hd;
   if (int rc = check_rows(k, ldk, rows_, row)) return rc;
   if (int rc = check_rows(v, ldv, rows_, row)) return rc;
-  if (pool->k == pool->v) return fail(TARS_E_OVERLAP, "the K and V pools are the same memory");
+  const int64_t kv_row = static_cast<int64_t>(pool->dtype == TARS_KV_E4M3 ? 1 : 2) * pool->hd;
+  if (meet(Levels(kv_row, pool->pages, pool->kv_heads, pool->page, pool->k_page, pool->k_head, pool->k_slot),
+           Levels(kv_row, pool->pages, pool->kv_heads, pool->page, pool->v_page, pool->v_head, pool->v_slot),
+           static_cast<char*>(pool->v) - static_cast<char*>(pool->k)))
+    return fail(TARS_E_OVERLAP, "the K and V pools share memory");
   const Mat kin = rows(k, ldk, rows_, row), vin = rows(v, ldv, rows_, row);
   for (const Mat* m : {&c.k, &c.v}) {
     bool hit = overlaps(*m, kin) || overlaps(*m, vin);
