@@ -147,6 +147,9 @@ float f32_of(uint32_t b) {
 constexpr int kMaxPagedRows = 1 << 22, kMaxPositions = 1 << 30, kMaxPagedHeads = 1024, kMaxPagedSeqs = 65535;
 constexpr int64_t kMaxSlotBytes = 1 << 26, kMaxSeqHeads = 1 << 22, kMaxRowHeads = 1 << 28;
 
+bool head_ok(int32_t hd) { return hd == 64 || hd == 128 || hd == 256; }
+bool page_ok(int32_t page) { return page >= 16 && (page & (page - 1)) == 0 && page <= kMaxPositions; }
+
 // Whether n_i items at stride_i (in any order of the three) hold `row` bytes each without sharing a byte; `end` gets
 // the extent.
 bool strides_ok(int64_t row, const int64_t (&n)[3], const int64_t (&stride)[3], int64_t* end) {
@@ -206,9 +209,8 @@ int check_paged(const tars_kv_pool* p, int32_t dtype, int32_t rows_, const int32
   if (dtype != TARS_KV_BF16 && dtype != TARS_KV_FP16) return fail(TARS_E_FIELD, "rows are BF16 or FP16");
   if (p->dtype != dtype && p->dtype != TARS_KV_E4M3) return fail(TARS_E_FIELD, "the pool holds the rows' type or E4M3");
   if (p->dtype != TARS_KV_E4M3 && (p->kscale || p->vscale)) return fail(TARS_E_FIELD, "scales belong to E4M3 pools");
-  if (p->hd != 64 && p->hd != 128 && p->hd != 256) return fail(TARS_E_FIELD, "hd must be 64, 128 or 256");
-  if (p->page < 16 || (p->page & (p->page - 1)) || p->page > kMaxPositions)
-    return fail(TARS_E_FIELD, "page must be a power of two, 16 or more");
+  if (!head_ok(p->hd)) return fail(TARS_E_FIELD, "hd must be 64, 128 or 256");
+  if (!page_ok(p->page)) return fail(TARS_E_FIELD, "page must be a power of two, 16 or more");
   if (p->kv_heads < 1 || p->kv_heads > kMaxPagedHeads) return fail(TARS_E_FIELD, "kv_heads must be 1..1024");
   if (p->pages < 1 || table_pages < 1 || seqs < 1 || rows_ < 1) return fail(TARS_E_ALIGN, "pages, table_pages, seqs, rows >= 1");
   if (!starts && rows_ != seqs) return fail(TARS_E_FIELD, "without starts every sequence has one row");
@@ -936,7 +938,7 @@ int tars_kv_append(const tars_kv_pool* pool, const void* k, int64_t ldk, const v
 
 int64_t tars_paged_workspace(int32_t heads, int32_t kv_heads, int32_t hd, int32_t rows_, int32_t seqs,
                              int32_t table_pages, int32_t page, int32_t decode) {
-  if (heads < 1 || kv_heads < 1 || heads % kv_heads || hd < 1 || rows_ < 1 || seqs < 1 || table_pages < 1 || page < 1 ||
+  if (heads < 1 || kv_heads < 1 || heads % kv_heads || !head_ok(hd) || !page_ok(page) || rows_ < 1 || seqs < 1 || table_pages < 1 ||
       heads > kMaxPagedHeads || rows_ > kMaxPagedRows || seqs > kMaxPagedSeqs ||
       static_cast<int64_t>(seqs) * heads > kMaxSeqHeads || static_cast<int64_t>(rows_) * heads > kMaxRowHeads ||
       static_cast<int64_t>(table_pages) * page > kMaxPositions)

@@ -123,3 +123,14 @@ def test_what_fits_is_passed_on(library):
     assert decode[0] == "tars_paged_decode" and decode[1][8] == OUT_FP32 and decode[1][10:12] == [2 ** 31 - 1] * 2
     assert prompt[0] == "tars_paged_attention" and prompt[1][8] == OUT_BF16 and prompt[1][10:12] == [7, 4]
     assert store[0] == "tars_kv_append" and store[1][6] == 2 and store[1][2] == 256
+
+
+@pytest.mark.parametrize("decode", [0, 1])
+def test_no_workspace_for_sizes_that_the_calls_refuse(decode):
+    size = _lib.lib().tars_paged_workspace
+    good = dict(heads=8, kv=2, hd=128, rows=3, seqs=3, width=4096, page=16)
+    assert size(*good.values(), decode) > 0
+    for bad in (dict(hd=32), dict(hd=96), dict(hd=512), dict(hd=1), dict(page=3), dict(page=1), dict(page=8), dict(page=48),
+                dict(page=-16), dict(kv=3), dict(kv=0), dict(heads=1026), dict(rows=0), dict(rows=2 ** 22 + 1), dict(seqs=65536),
+                dict(width=2 ** 27), dict(width=0), dict(heads=1024, rows=2 ** 19), dict(heads=1024, seqs=4097)):
+        assert size(*{**good, **bad}.values(), decode) == 0, bad
