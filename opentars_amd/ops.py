@@ -588,7 +588,7 @@ def _paged_meta(cache: PagedCache, table: torch.Tensor, lens: torch.Tensor, star
         raise ValueError("table, lens and starts must be int32")
     if table.get_device() != index or lens.get_device() != index or (starts is not None and starts.get_device() != index):
         raise ValueError("table, lens and starts must live on the cache's GPU")
-    if torch._C._cuda_getDevice() != index:
+    if torch.cuda.current_device() != index:
         raise ValueError("the cache's GPU must be the current device")
     if table.dim() != 2 or lens.dim() != 1:
         raise ValueError("table must be [seqs, table_pages] and lens [seqs]")
