@@ -474,7 +474,8 @@ __global__ __launch_bounds__(64 * kRowsWg / wave_rows(D), 2) void paged_prompt_k
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int e = 0; e < N; e += 4)
-          store4<T>(y, head_out * D + R * t + e * (64 / R) + 4 * part, a.out_f32, o[t][e] * k, o[t][e + 1] * k, o[t][e + 2] * k, o[t][e + 3] * k);
+          store4<T>(y, head_out * D + R * t + e * (64 / R) + 4 * part, a.out_f32, o[t][e] * k, o[t][e + 1] * k, o[t][e + 2] * k,
+                    o[t][e + 3] * k, !E4M3);
     } else {
       float* at = ws + (static_cast<int64_t>(tile.first + token_out) * a.heads + head_out) * (D + 4);
 #pragma unroll
@@ -558,7 +559,7 @@ __global__ __launch_bounds__(256) void paged_prompt_join_kernel(PagedAttnArgs a,
   join_unfinite(y, parts, [&](int p) { return *reinterpret_cast<const float4*>(ws + p * ld + d); });
   const float vs = a.pool.vscale ? a.pool.vscale[h] : 1.0f;
   const float k = sum == 0 ? 0.0f : vs * __builtin_amdgcn_rcpf(sum);
-  if (lane < L) store4<T>(a.y + row * a.ldy, head * D + d, a.out_f32, y.x * k, y.y * k, y.z * k, y.w * k);
+  if (lane < L) store4<T>(a.y + row * a.ldy, head * D + d, a.out_f32, y.x * k, y.y * k, y.z * k, y.w * k, !a.pool.vscale);
 }
 
 // Tiles start in the order of their length where more workgroups come than run at once, 512, and up to 64 sequences bring

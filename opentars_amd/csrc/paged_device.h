@@ -18,6 +18,7 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 // 16-bit element types: bits to fp32 (exact) and back (to nearest even).
 struct Bf16 {
   static constexpr uint32_t kExponent = 0x7F80;  // all ones: infinite or NaN
+  static constexpr float kLargest = 0;           // as good as fp32's
   static __device__ __forceinline__ float wide(uint32_t bits) { return __uint_as_float(bits << 16); }
   static __device__ __forceinline__ uint32_t pair(float lo, float hi) {
     const v2bf r = {static_cast<__bf16>(lo), static_cast<__bf16>(hi)};
@@ -40,6 +41,7 @@ struct Bf16 {
 };
 struct Fp16 {
   static constexpr uint32_t kExponent = 0x7C00;
+  static constexpr float kLargest = 65504.0f;
   static __device__ __forceinline__ float wide(uint32_t bits) {
     return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)));
   }
@@ -103,11 +105,21 @@ __device__ __forceinline__ uint32_t nan_e4m3(uint32_t x) {    // 0xFF in each by
   return (top << 1) - (top >> 7);
 }
 
-// Four neighbouring values of an output row, rounded once: fp32 or T.
+// Four neighbouring values of an output row, rounded once: fp32 or T. mean: they are means of T's values, without a scale, by
+// numerators rounded to T, whose rounding may take binary16's largest value to infinity: half a step is enough. (bf16's
+// largest is fp32's but for the rounding; numerators in two parts are off by 2^-22.)
 template <class T>
-__device__ __forceinline__ void store4(char* row, int at, int f32, float a, float b, float c, float d) {
+__device__ __forceinline__ float within(float x, bool mean) {
+  if (!mean || T::kLargest == 0) return x;
+  x = x > T::kLargest && x < INFINITY ? T::kLargest : x;
+  return x < -T::kLargest && x > -INFINITY ? -T::kLargest : x;
+}
+template <class T>
+__device__ __forceinline__ void store4(char* row, int at, int f32, float a, float b, float c, float d, bool mean = false) {
   if (f32) *reinterpret_cast<float4*>(row + 4 * at) = make_float4(a, b, c, d);
-  else *reinterpret_cast<uint2*>(row + 2 * at) = make_uint2(T::pair(a, b), T::pair(c, d));
+  else
+    *reinterpret_cast<uint2*>(row + 2 * at) =
+        make_uint2(T::pair(within<T>(a, mean), within<T>(b, mean)), T::pair(within<T>(c, mean), within<T>(d, mean)));
 }
 
 // The number of sequences, of `seqs`, that ended(b) holds for, which holds for the first ones: 64 of every 4096, 64 and 1

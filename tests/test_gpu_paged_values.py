@@ -181,3 +181,19 @@ def test_a_scale_that_takes_scores_past_fp32(rows, n, hd, cache):
     got = run(layer, rows == 1, torch.float32, scale=1e30).cpu().double()
     want = layer.V[0][loud].repeat_interleave(2, 0).reshape(1, -1).expand(rows, -1)
     assert bool(((got - want).abs() <= 2.0 ** -22 * want.abs()).all())  # the scale's product, a reciprocal of 1
+
+
+@pytest.mark.parametrize("rows,n", [(1, 300), (1, 4000), (4, 700), (100, 300), (100, 4000)])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_a_mean_of_binary16_values_is_in_their_range(rows, n, hd):
+    """Columns of V that hold binary16's largest value at every position: so does every row, however its numerators are
+    rounded (a part in 2^12 more is an infinity)."""
+    layer = Layer(rows + n + hd, [n], [rows], 4, 2, hd, qt="fp16")
+    layer.q *= 8                                                       # one position or two have most of the weight
+    for page, slot in layer.where[0]:
+        layer.vpool[page, 0, slot, ::2], layer.vpool[page, 1, slot, 1::2] = 65504.0, -65504.0
+    got = run(layer, rows == 1, torch.float16).cpu()
+    got = got.view(rows, 2, 2, hd)
+    assert bool(torch.isfinite(got.float()).all())
+    for part, value in ((got[:, 0, :, ::2], 65504.0), (got[:, 1, :, 1::2], -65504.0)):
+        assert bool(((part.double() / value - 1).abs() <= 2.0 ** -11 + 2.0 ** -11).all())     # numerators, the result
