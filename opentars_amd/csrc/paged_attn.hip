@@ -504,12 +504,8 @@ __global__ __launch_bounds__(64 * kRowsWg / wave_rows(D), 2) void paged_prompt_k
     return parts > 1 ? ws + (static_cast<int64_t>(tile.first + t) * a.heads + h * a.group + x - t * a.group) * (D + 4) : nullptr;
   };
   const auto sound = [&](int x) { return parts > 1 || sums[x - tile.r0] < INFINITY; };
-#pragma unroll 1
-  for (int turn = 0; turn < 2; ++turn)
-#pragma unroll 1
-    for (int i = t0; i < t1; ++i)
-      add_unfinite<T, E4M3, D>(a, turn == 0, tile.b, h, tile.len, steps.at(i) * kTile, (steps.at(i) + 1) * kTile, p0, tile.first,
-                               tile.r0, min(M, total - tile.r0), part_row, sound);
+  set_unfinite<T, E4M3, D, kTile>(
+      a, tile.b, h, tile.len, [&](int i) { return steps.at(i); }, t0, t1, p0, tile.first, tile.r0, min(M, total - tile.r0), part_row, sound);
 }
 
 // Joins the parts of rows whose tiles were split: a workgroup per row and 4 heads, D / 4 lanes of a wave for a head's

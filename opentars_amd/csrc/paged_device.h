@@ -169,49 +169,67 @@ __device__ __forceinline__ void join_unfinite(float4& y, int n, F v) {
   y = make_float4(z.x == 0 ? y.x : z.x, z.y == 0 ? y.y : z.y, z.z == 0 ? y.z : z.z, z.w == 0 ? y.w : z.w);
 }
 
-// V's infinities and NaN at the positions [k0, k1), k0 a multiple of 16, of sequence b, in the outputs of the columns [c0, c0 + cols)
-// of K / V head h that see them: clear, then add. What such a value made of an output in the products does not matter (nothing
-// where it was left out, an infinity or NaN otherwise): the output is the sum of those it sees. sound(x): column x has a
-// finite sum of numerators (an output of one that has not stays NaN), or is a row of a part. Column x is query head h *
-// group + x % group of row first + x / group, at position p0 + x / group; part(x): its row of a part in the workspace, or
-// null where its output is final. A thread per column of V, 16 positions of a page at a time; all of the workgroup's
-// outputs are written, and the barrier behind that passed.
-template <class T, bool E4M3, int D, class F, class G>
-__device__ void add_unfinite(const PagedAttnArgs& a, bool clear, int b, int h, int len, int k0, int k1, int p0, int first, int c0,
-                             int cols, F part, G sound) {
+// A set of up to 128 columns.
+struct Columns {
+  uint64_t lo = 0, hi = 0;
+  static __device__ __forceinline__ uint64_t below(int n) { return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1; }
+  __device__ __forceinline__ void add(Range r) {
+    lo |= below(r.hi) & ~below(r.lo);
+    hi |= below(r.hi - 64) & ~below(r.lo - 64);
+  }
+  __device__ __forceinline__ bool has(int x) const { return (x < 64 ? lo >> x : hi >> (x - 64)) & 1; }
+};
+
+// Sets the outputs that V's infinities and NaN reach to the sum of those they see, at the positions of the steps `at(i)` of STEP
+// positions, i in [t0, t1), of sequence b. What such a value made of an output in the products (nothing where it was left
+// out, an infinity or NaN otherwise) does not count. The columns are [c0, c0 + cols), 128 at most, of K / V head h; column x
+// is query head h * group + x % group of row first + x / group, at position p0 + x / group. sound(x): the column's sum of
+// numerators is finite (an output of one whose is not stays NaN), or it is a row of a part; part(x): its row of a part in
+// the workspace, or null where its output is final. A thread per column of V, 16 positions of a page at a time; all of the
+// workgroup's outputs are written, and the barrier behind that passed.
+template <class T, bool E4M3, int D, int STEP, class At, class F, class G>
+__device__ void set_unfinite(const PagedAttnArgs& a, int b, int h, int len, At at, int t0, int t1, int p0, int first, int c0, int cols,
+                             F part, G sound) {
+  static_assert(STEP % 16 == 0, "16 positions of one page at a time");
   for (int d = threadIdx.x; d < D; d += blockDim.x) {
+    Columns nan, plus, minus, all;
+    all.add({0, cols});
 #pragma unroll 1
-    for (int j0 = k0; j0 < min(k1, len); j0 += 16) {
+    for (int i = t0 * (STEP / 16); i < t1 * (STEP / 16) && (nan.lo != all.lo || nan.hi != all.hi); ++i) {
+      const int j0 = at(i / (STEP / 16)) * STEP + i % (STEP / 16) * 16;
+      if (j0 >= len) break;
       const int page = a.seqs.table[b * a.seqs.ld_table + (j0 >> a.pool.page_shift)];
       if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pool.pages)) continue;
-      const char* at = a.pool.v + h * a.pool.v_head + page * a.pool.v_page + (j0 & ((1 << a.pool.page_shift) - 1)) * a.pool.v_slot;
-      const auto value = [&](int i) {
-        const char* row = at + i * a.pool.v_slot;
+      const char* block = a.pool.v + h * a.pool.v_head + page * a.pool.v_page + (j0 & ((1 << a.pool.page_shift) - 1)) * a.pool.v_slot;
+      const auto value = [&](int k) {
+        const char* row = block + k * a.pool.v_slot;
         return E4M3 ? T::template from_e4m3<false>(reinterpret_cast<const uint8_t*>(row)[d]) & 0xFFFFu
                     : static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[d]);
       };
       uint32_t bad = 0;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) bad |= static_cast<uint32_t>(not_finite<T>(value(i)) != 0) << i;
+      for (int k = 0; k < 16; ++k) bad |= static_cast<uint32_t>(not_finite<T>(value(k)) != 0) << k;
 #pragma unroll 1
       for (; bad; bad &= bad - 1) {
-        const int i = __builtin_ctz(bad), j = j0 + i;
-        const float v = T::wide(value(i));
-#pragma unroll 1
-        for (int x = c0; x < c0 + cols; ++x) {
-          const int t = x / a.group, head = h * a.group + x - t * a.group;
-          if (j >= len || !sees(p0 + t, j, a.window, a.sinks) || !sound(x)) continue;
-          if (float* to = part(x)) {
-            to[d] = clear ? 0.0f : to[d] + v;
-          } else if (a.out_f32) {
-            float* y = reinterpret_cast<float*>(a.y + (first + t) * a.ldy) + head * D + d;
-            *y = clear ? 0.0f : *y + v;
-          } else {
-            uint16_t* y = reinterpret_cast<uint16_t*>(a.y + (first + t) * a.ldy) + head * D + d;
-            *y = clear ? 0 : static_cast<uint16_t>(T::pair(T::wide(*y) + v, 0.0f));
-          }
-        }
+        const int k = __builtin_ctz(bad), j = j0 + k;
+        if (j >= len) break;
+        const float v = T::wide(value(k));
+        const Range seen = seen_by(j, p0, a.group, c0, cols, a.window, a.sinks);
+        if (v != v) nan.add(seen);
+        else if (v > 0) plus.add(seen);
+        else minus.add(seen);
       }
+    }
+    if ((nan.lo | nan.hi | plus.lo | plus.hi | minus.lo | minus.hi) == 0) continue;
+#pragma unroll 1
+    for (int x = 0; x < cols; ++x) {
+      const bool up = plus.has(x), down = minus.has(x), no = nan.has(x) || (up && down);
+      if (!(up || down || no) || !sound(c0 + x)) continue;
+      const float v = no ? NAN : up ? INFINITY : -INFINITY;
+      const int t = (c0 + x) / a.group, head = h * a.group + c0 + x - t * a.group;
+      if (float* to = part(c0 + x)) to[d] = v;
+      else if (a.out_f32) reinterpret_cast<float*>(a.y + (first + t) * a.ldy)[head * D + d] = v;
+      else reinterpret_cast<uint16_t*>(a.y + (first + t) * a.ldy)[head * D + d] = static_cast<uint16_t>(T::pair(v, 0.0f));
     }
   }
 }

@@ -53,6 +53,18 @@ TARS_HD bool sees(int p, int j, int window, int sinks) {
   return j <= p && (window == 0 || j > p - window || j < sinks);
 }
 
+// Of the columns [c0, c0 + cols), `group` of them to a row, rows at positions p0, p0 + 1, ...: the ones that see position j >= 0
+// are c0 + lo .. c0 + hi - 1 (lo >= hi: none).
+struct Range {
+  int lo, hi;
+};
+TARS_HD Range seen_by(int j, int p0, int group, int c0, int cols, int window, int sinks) {
+  const int rows = ceil_div(c0 + cols, group);  // no row behind them counts
+  const int64_t after = window == 0 || j < sinks ? rows : int64_t{j} - p0 + window;
+  const int first = iclamp(j - p0, 0, rows), end = after < 0 ? 0 : after > rows ? rows : static_cast<int>(after);
+  return {iclamp(first * group - c0, 0, cols), iclamp(end * group - c0, 0, cols)};
+}
+
 // The steps of `step` positions that hold every position seen by a row at a position in [plo, phi] of a sequence of
 // length len: [0, a) and [b0, b1), a <= b0 <= b1. A step of the first part may hold positions of the window, and
 // steps of either may hold positions that a row does not see.

@@ -558,12 +558,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_rows_kernel(PagedAttnArg
     for (int w = 0; w < kWaves; ++w) sum += ls[w][x - c0];
     return part.parts > 1 || sum < INFINITY;
   };
-#pragma unroll 1
-  for (int turn = 0; turn < 2; ++turn)
-#pragma unroll 1
-    for (int i = t0; i < t1; ++i)
-      add_unfinite<T, E4M3, D>(a, turn == 0, part.b, h, len, steps.at(i) * kStep, (steps.at(i) + 1) * kStep, p0, part.work.first, c0,
-                               cols, [&](int x) { return part.parts > 1 ? ws + (x - c0) * (D + 4) : nullptr; }, sound);
+  set_unfinite<T, E4M3, D, kStep>(
+      a, part.b, h, len, [&](int i) { return steps.at(i); }, t0, t1, p0, part.work.first, c0, cols,
+      [&](int x) { return part.parts > 1 ? ws + (x - c0) * (D + 4) : nullptr; }, sound);
 }
 
 // Joins the parts of a row, of `all`: a workgroup per row and head, D / 4 lanes for a part's row.

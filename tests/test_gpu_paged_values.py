@@ -197,3 +197,23 @@ def test_a_mean_of_binary16_values_is_in_their_range(rows, n, hd):
     assert bool(torch.isfinite(got.float()).all())
     for part, value in ((got[:, 0, :, ::2], 65504.0), (got[:, 1, :, 1::2], -65504.0)):
         assert bool(((part.double() / value - 1).abs() <= 2.0 ** -11 + 2.0 ** -11).all())     # numerators, the result
+
+
+@pytest.mark.parametrize("value", [INF, NAN])
+@pytest.mark.parametrize("window", [0, 700])
+def test_a_cache_of_nothing_but_infinities_or_nan(value, window):
+    """What a model that has diverged leaves in V: prompts, few rows and single tokens over it are right in ordinary time."""
+    kv, hd, page, n = 2, 128, 16, 20000
+    pages = -(-n // page)
+    k = torch.randn(pages, kv, page, hd, device="cuda", dtype=torch.bfloat16)
+    v = torch.full_like(k, value)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").view(1, -1)
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    for rows in (1, 5, 1500):
+        q = torch.randn(rows, 4 * kv * hd, device="cuda", dtype=torch.bfloat16)
+        starts = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+        y = ops.paged_attention(ops.PagedCache(k, v), q, table, lens, starts, window=window)
+        assert bool(y.isnan().all() if value != value else (y == value).all())
+        if rows == 1:
+            y = ops.paged_decode(ops.PagedCache(k, v), q, table, lens, window=window)
+            assert bool(y.isnan().all() if value != value else (y == value).all())
