@@ -318,6 +318,8 @@ int tars_attention_noalloc(const float* const* q, int64_t ldq, const float* cons
  * Device arrays are not checked on the host; whatever they hold, nothing outside the call's buffers is
  * read or written: lens is clamped to [0, table_pages * page], starts to [0, rows], a page number
  * outside the pool means that its positions hold nothing.
+ * Scores q k and sums of numerators (up to 64 each) times V are fp32: where one passes 3.4e38, the row is not
+ * finite.
  * Limits (TARS_E_FIELD / TARS_E_RANGE past them): 1024 heads, 65535 sequences, 2^22 rows, seqs * heads
  * 2^22, rows * heads 2^28, slots 2^26 bytes apart. */
 #define TARS_KV_BF16  0
@@ -368,7 +370,7 @@ int64_t tars_paged_workspace(int32_t heads, int32_t kv_heads, int32_t hd, int32_
  *   q [rows, heads * hd] at ldq, BF16 or FP16; query head h reads K / V head h / (heads / kv_heads).
  *   y [rows, heads * hd] at ldy, out = FP32 or q's type (BF16 / FP16). fp32 scores, maxima and sums;
  *   the softmax's numerators are rounded to q's type for the product with V (for few rows, or few over
- *   a short cache, to the sum of two values of it).
+ *   a short table, to the sum of two values of it).
  *   0 < scale <= 1e30; work: tars_paged_workspace bytes, 16-byte aligned, for this call until it is done.
  */
 int tars_paged_attention(const tars_kv_pool* pool, const void* q, int64_t ldq, int32_t dtype,

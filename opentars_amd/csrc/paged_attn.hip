@@ -22,8 +22,8 @@
 // A workgroup has 128 rows, a wave 32 (16 for heads of 256); the last rows of a sequence, which see most, start first.
 // With few rows their tiles are split over workgroups and joined by a second launch.
 //
-// What bounds it: the matrix units within the power limit. 8192 rows of 32 heads of 128, causal: 530 us, 1.04 PF/s (1.25
-// with zeros for data; the library's bf16 product of 8192 x 8192 x 8192 runs at 1.23 to 1.35); 2000 rows behind 14000 of
+// What bounds it: the matrix units within the power limit. 8192 rows of 32 heads of 128, causal: 530 to 560 us from card to
+// card, 0.98 to 1.04 PF/s (1.25 with zeros for data; the library's bf16 product of 8192 x 8192 x 8192 runs at 1.23 to 1.35); 2000 rows behind 14000 of
 // 16 heads 268 us, 0.92 PF/s; heads of 256, 16 of them, 619 us, 0.89 PF/s, the reads of K and V from LDS beside the
 // products, and 748 us over an e4m3 pool, whose widening adds to them. Few workgroups are bound by their number: two
 // chunks of 2000 to 3001 rows, heads of 256 with a window of 1024 in e4m3, 316 on 256 CUs, 126 us; 400 rows of 16 heads
@@ -567,11 +567,12 @@ struct Plan {
   bool sorted;
 };
 // Few workgroups are split until there are up to 512, two on every CU, in parts of kLeast tiles or more: 256 rows of 16
-// heads behind 30000 85 us (up to 256: 100, 1024: 108), 40 behind 3000 20.3 us (8 tiles: 23.1); two parts are not worth
-// the second launch (480 rows, 16 heads of 64: 14.0 us in one, 18.5 in two), three are (80 rows behind 600: 15.9, 18.1 in
-// one). Of heads of 256, whose
-// workgroups have twice the waves, a CU holds one: 128 rows of 16 heads behind 8000 41 us (up to 512: 58), 256 behind
-// 30000 175 us (193).
+// heads behind 30000 85 us (up to 256: 100, 1024: 108), 40 behind 3000 20.3 us (8 tiles: 23.1). Tables of up to 8 tiles are
+// not split (480 rows of 16 heads of 64: 14.2 us in one, 18.7 in two). Past them the second launch pays the sooner the fewer
+// workgroups there are: 16 of them (80 rows of 16 heads of 128) in 9 tiles 19.1 us and 21.5 in one part, in 24 20.9 and 38.4;
+// 64 (480 rows) in 9 25.1 and 21.8, in 15 26.9 and 27.2; 120 (480 rows of 32 heads) in 11 33.8 and 23.9, in 24 as long: there
+// the rule costs more than it gives. Of heads of 256, whose workgroups have twice the waves, a CU holds one: 128 rows of 16
+// heads behind 8000 41 us (up to 512: 58), 256 behind 30000 175 us (193).
 constexpr int resident(int hd) { return hd == 256 ? 256 : 512; }
 constexpr int kLeast = 4;
 Plan plan(int heads, int kv_heads, int hd, int rows, int seqs, int cap) {
@@ -601,10 +602,13 @@ hipError_t go(const PagedAttnArgs& a, hipStream_t s) {
 }  // namespace
 
 // Sequences of 32 columns or fewer on average go to the kernel for few rows: 16 caches of 3k to 16k with 20 columns 134 us
-// and 148 here, with 32 143 and 150, with 64 233 and 157. So do short caches of five tiles or more with rows for a quarter of
-// their positions at most, where this kernel's tiles follow one another in few workgroups and that one has one for each 32
-// (16) columns: 77 rows behind 300, 16 heads of 64, 10.5 us (13.4), of 128 13.4 us (17.8), 8 of 256 14.6 us (19.0). With
-// rows for all positions, or fewer tiles, it is the other way round (400 rows: 14.9 and 12.6 here, 20: 8.3 and 7.6).
+// and 148 here, with 32 143 and 150, with 64 233 and 157. So do rows that fill a quarter at most of a table for 257 to 512
+// positions, where this kernel's tiles follow one another in few workgroups and that one has one for each 32 (16) columns: 20 to
+// 77 rows behind 300 to 470, in four layouts of heads, 10.6 to 17.8 us there and 11.7 to 20.4 here, each of them faster there
+// (77 behind 300, 16 heads of 64: 10.8 and 14.1; of 128: 13.6 and 17.7; 8 of 256: 15.2 and 19.0). The edges are not where the
+// two kernels meet: 77 rows behind 200 in a table for 304 positions, more than a quarter of it, come here and take 13.2, 10.6
+// there. 200 rows behind 300 (19.8 and 20.9 there), 77 behind 700 (15.7 and 16.9) and rows with no past (400: 12.6 and 14.9)
+// are faster here.
 constexpr int kShort = 256, kShortCap = 512, kShortWgs = 512;
 static bool few_rows(int group, int kv_heads, int hd, int rows, int seqs, int cap) {
   const int64_t columns = static_cast<int64_t>(rows) * group;

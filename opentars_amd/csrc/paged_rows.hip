@@ -32,7 +32,7 @@
 // 64 query heads 162 us, 5.4 TB/s, the widening of K and V beside the loads; 16 of 3k to 16k with five rows each (32
 // columns, two workgroups on a CU instead of three) 134 us, 4.8 TB/s. Short work is bound by the chain launch -> lengths
 // -> page numbers -> K and V -> second launch: one cache of 2k 10.8 us, of 300 9.1 us; 100 windows of 512, one K / V
-// head of 256, 19.7 us.
+// head of 256, 20.2 us.
 #include <algorithm>
 
 #include "paged_device.h"
@@ -49,9 +49,9 @@ constexpr int kWaves = 4;
 // dealt to two workgroups on a CU: 100 windows of 512 13.9 us (16.4 with one, which is better for one long cache: 8k 15.0
 // and 13.1). A share has a step for each wave at least: one cache of 4k 10.9 us (12.8 with half of that).
 constexpr int kSlots = 512, kFew = 512, kShort = 512;
-// Caches that may have up to kAlone steps are not split, which spares the second launch: one of 120 positions 7.3 us (8.8),
-// of 300 9.1 us (9.8), of 480 10.4 us (10.2; the host's work is 3 us less), 32 of up to 480 13.1 us (16.3); of 600, whose
-// 19 steps are split, 10.3 us (11.4).
+// Caches that may have up to kAlone steps, by the table's width or the window, are not split, which spares the second launch:
+// one of 120 positions 7.3 us (8.7 in a table for 8192), of 300 9.1 us (9.8), of 480 10.4 us (10.2; the host's work is 3 us
+// less), 32 of up to 480 14.8 us (18.0); of 600, whose 19 steps are split, 10.3 us (11.4).
 constexpr int kAlone = 16;
 
 struct Deal {
