@@ -14,7 +14,7 @@
  * golden model's "every check before any write" rule (tars_mini/golden.py:450-472).
  *
  * Results are bit-exact against the golden model's arithmetic (tars_mini/golden.py,
- * tars_mini/numerics.py; the paged cache is outside that contract): exact int32 dot products, then
+ * tars_mini/numerics.py; the paged cache and the operators around it are outside that contract): exact int32 dot products, then
  * the fp32 epilogue one rounded step at a time (round-to-nearest-even, subnormals flushed on the way
  * in and out, canonical NaN, no FMA).
  * Results never depend on launch geometry.
@@ -388,6 +388,106 @@ int tars_paged_decode(const tars_kv_pool* pool, const void* q, int64_t ldq, int3
                       int32_t window, int32_t sinks, const int32_t* table, int64_t ld_table,
                       int32_t table_pages, const int32_t* lens, void* work, int64_t work_bytes,
                       void* stream);
+
+/* ---------------------------------------------------------------- a serving step around the cache
+ * Three operators next to the paged cache, outside the golden contract as it is: sums are fp32 and each
+ * result is rounded once; a repeated call gives the same bits. */
+
+/*
+ * The norm of queries and keys for each head and their rotation by position, in one pass: for a head's
+ * hd elements x, u = x gamma / sqrt(mean(x^2) + eps) (u = x where its gamma is NULL; the sum of squares
+ * is fp32), then with h = rot / 2 and row p of tab, [cos(0 .. h - 1), sin(0 .. h - 1)] (the layout of
+ * tars_rope): y[i] = u[i] cos_i - u[i + h] sin_i and y[i + h] = u[i + h] cos_i + u[i] sin_i for i < h;
+ * elements behind rot are u.
+ *   q [rows, heads * hd] at ldq, k [rows, kv_heads * hd] at ldk (bytes, 0 = dense), yq and yk their
+ *   outputs, dtype BF16 or FP16 (TARS_KV_*), hd 64, 128 or 256; pointers and row strides multiples of 16.
+ *   An output may be its input (same address and stride); any other overlap is refused.
+ *   qgamma, kgamma fp32 [hd] or NULL; tab fp32 [positions, rot], dense; rot a multiple of 16, up to hd.
+ *   lens, starts, seqs: the rows' sequences, as tars_kv_append's; row i of a sequence's n is at position
+ *   lens[b] - n + i. A row without a sequence, at a negative position or at one that tab does not have
+ *   leaves its outputs as they were.
+ */
+int tars_qk_norm_rope(const void* q, int64_t ldq, const void* k, int64_t ldk, int32_t dtype, int32_t heads,
+                      int32_t kv_heads, int32_t hd, int32_t rows, const float* qgamma, const float* kgamma,
+                      float eps, const float* tab, int32_t positions, int32_t rot, const int32_t* lens,
+                      const int32_t* starts, int32_t seqs, void* yq, int64_t ldyq, void* yk, int64_t ldyk,
+                      void* stream);
+
+/*
+ * tars_qk_norm_rope with the keys going to their pages instead of yk, and the values beside them as they
+ * are: tars_kv_append of keys that were never written in between (an E4M3 pool gets the fp32 key over its
+ * scale, rounded once). The pool's kv_heads and hd are k's and v's; the rules on rows and pages are
+ * tars_kv_append's, and of rows at positions that tab does not have neither key nor value is stored.
+ */
+int tars_kv_append_rope(const tars_kv_pool* pool, const void* q, int64_t ldq, const void* k, int64_t ldk,
+                        const void* v, int64_t ldv, int32_t dtype, int32_t heads, int32_t rows,
+                        const float* qgamma, const float* kgamma, float eps, const float* tab,
+                        int32_t positions, int32_t rot, const int32_t* table, int64_t ld_table,
+                        int32_t table_pages, const int32_t* lens, const int32_t* starts, int32_t seqs,
+                        void* yq, int64_t ldyq, void* stream);
+
+/* A matrix of `rows` x `k` in microscaled 4-bit floating point (OCP MXFP4). values: two e2m1 codes to a
+ * byte, the even k in the low half, rows of k / 2 bytes at ld_values; scales: the exponent byte b of each
+ * 32 consecutive k, for 2^(b - 127) (255: the block is NaN), at ld_scales. A row's scales take up whole
+ * 16-byte pieces of memory, 16 * ceil(k / 512) bytes, whatever is in those behind k / 32. Device
+ * pointers; addresses and strides are multiples of 16, a stride 0 = dense (of whole pieces). k is a
+ * multiple of 32, at most 2^20; strides at most 2^22. */
+typedef struct tars_mx4 {
+  void* values;
+  void* scales;
+  int64_t ld_values, ld_scales;
+  int32_t rows, k;
+} tars_mx4;
+
+/*
+ * Quantises x [dst->rows, dst->k] (FP32, BF16 or FP16: TARS_OUT_*) at ldx bytes into dst. A block's b is
+ * the exponent field of its largest magnitude as fp32, less 2, at least 0; a code is x / 2^(b - 127)
+ * rounded to nearest even at 0, 0.5, 1, 1.5, 2, 3, 4, 6, past 6 to 6, with x's sign. A block that holds an
+ * infinity or NaN gets b = 255 and codes of 0. The bytes behind a row's scales get 0.
+ * x and ldx are multiples of 16 bytes.
+ */
+int tars_quant_mx4(const void* x, int64_t ldx, int32_t dtype, const tars_mx4* dst, void* stream);
+
+/*
+ * y[m][n] = sum over k of x[m][k] w[n][k] + bias[n], for x [M, K] and w [N, K] in microscaled 4 bits.
+ *   bias fp32 [N] or NULL; y [M, N] at ldy bytes (0 = dense; a multiple of the element size, as y's
+ *   address), out FP32, BF16 or FP16. Products of codes are exact, their sums fp32; past the output's
+ *   largest value is infinity. Scales whose sum of exponents passes fp32's ends do so in the product too:
+ *   sums below 2^-126 may come out 0. Without a sum that is NaN, the result is the same bits for any M
+ *   that runs the same way (few rows, many rows). At most 2^22 rows of x and 2^24 of w.
+ */
+int tars_gemm_mx4(const tars_mx4* x, const tars_mx4* w, const float* bias, void* y, int64_t ldy,
+                  int32_t out, void* work, int64_t work_bytes, void* stream);
+
+/* The same with x [M, w->k] of FP32, BF16 or FP16 (TARS_OUT_*) rows at ldx bytes (address and stride
+ * multiples of 16), quantised as tars_quant_mx4 does: the same results as the two calls. */
+int tars_quant_gemm_mx4(const void* x, int64_t ldx, int32_t dtype, int32_t M, const tars_mx4* w,
+                        const float* bias, void* y, int64_t ldy, int32_t out, void* work,
+                        int64_t work_bytes, void* stream);
+
+/* Bytes of device scratch, 16-byte aligned, that tars_gemm_mx4 (quantises = 0) or tars_quant_gemm_mx4 (1)
+ * needs until it is done; 0 where none is (or for sizes the calls refuse). Host only. */
+int64_t tars_mx4_workspace(int32_t M, int32_t N, int32_t K, int32_t quantises);
+
+/*
+ * Log probabilities of given tokens under the rows' softmax, its entropy, and the top alternatives.
+ *   x [rows, vocab] logits (FP32, BF16 or FP16: TARS_OUT_*) at ld bytes (0 = dense; a multiple of the
+ *   element size); tokens [rows, given] int32, or int64 with wide_tokens, at ld_tokens bytes (0 = dense),
+ *   NULL with given 0. Outputs, dense: logprobs fp32 [rows, given], entropy fp32 [rows] (in nats), and
+ *   with top > 0 (at most 64 and vocab) top_logprobs fp32 and top_ids int32 [rows, top], the largest
+ *   logit first, equal ones by their places.
+ * A logit of -infinity is a token that cannot come: log probability -infinity, nothing in the entropy. A
+ * row of nothing else has log probabilities of -infinity and entropy 0. A token outside the vocabulary
+ * has -infinity. A NaN or +infinity makes the row's results NaN (-infinity for tokens outside), its
+ * alternatives ordered with NaN above all.
+ * work: tars_logprobs_workspace bytes, 16-byte aligned, until the call is done. At most 2^22 rows and
+ * 2^24 tokens in the vocabulary, 2^16 given.
+ */
+int tars_token_logprobs(const void* x, int64_t ld, int32_t dtype, int32_t rows, int32_t vocab,
+                        const void* tokens, int64_t ld_tokens, int32_t wide_tokens, int32_t given,
+                        float* logprobs, float* entropy, int32_t top, float* top_logprobs, int32_t* top_ids,
+                        void* work, int64_t work_bytes, void* stream);
+int64_t tars_logprobs_workspace(int32_t rows, int32_t vocab, int32_t dtype, int32_t top);
 
 /* Library version string ("opentars_amd <semver> gfx950"). Host only, never fails. */
 const char* tars_version(void);

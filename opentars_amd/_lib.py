@@ -37,6 +37,12 @@ class KvPool(ctypes.Structure):
                 ("pages", c_int32), ("page", c_int32), ("kv_heads", c_int32), ("hd", c_int32), ("dtype", c_int32)]
 
 
+class Mx4(ctypes.Structure):
+    """tars_mx4: a matrix in microscaled 4-bit floating point."""
+    _fields_ = [("values", c_void_p), ("scales", c_void_p), ("ld_values", c_int64), ("ld_scales", c_int64),
+                ("rows", c_int32), ("k", c_int32)]
+
+
 # Every exported entry point: name -> (restype, argtypes)
 SIGNATURES = {
     "tars_quant_rows": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int32, c_int32, c_void_p]),
@@ -90,6 +96,21 @@ SIGNATURES = {
     "tars_paged_decode": (c_int, [POINTER(KvPool), c_void_p, c_int64, c_int32, c_int32, c_int32, c_void_p, c_int64,
                                   c_int32, c_float, c_int32, c_int32, c_void_p, c_int64, c_int32, c_void_p, c_void_p,
                                   c_int64, c_void_p]),
+    "tars_qk_norm_rope": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int32, c_int32, c_int32, c_int32, c_int32,
+                                  c_void_p, c_void_p, c_float, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_int32,
+                                  c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
+    "tars_kv_append_rope": (c_int, [POINTER(KvPool), c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int32,
+                                    c_int32, c_int32, c_void_p, c_void_p, c_float, c_void_p, c_int32, c_int32, c_void_p,
+                                    c_int64, c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_int64, c_void_p]),
+    "tars_quant_mx4": (c_int, [c_void_p, c_int64, c_int32, POINTER(Mx4), c_void_p]),
+    "tars_gemm_mx4": (c_int, [POINTER(Mx4), POINTER(Mx4), c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_int64,
+                              c_void_p]),
+    "tars_quant_gemm_mx4": (c_int, [c_void_p, c_int64, c_int32, c_int32, POINTER(Mx4), c_void_p, c_void_p, c_int64,
+                                    c_int32, c_void_p, c_int64, c_void_p]),
+    "tars_mx4_workspace": (c_int64, [c_int32] * 4),
+    "tars_token_logprobs": (c_int, [c_void_p, c_int64, c_int32, c_int32, c_int32, c_void_p, c_int64, c_int32, c_int32,
+                                    c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "tars_logprobs_workspace": (c_int64, [c_int32] * 4),
 }
 
 _lib: ctypes.CDLL | None = None

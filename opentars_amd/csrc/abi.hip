@@ -248,6 +248,15 @@ int check_paged(const tars_kv_pool* p, int32_t dtype, int32_t rows_, const int32
   return TARS_OK;
 }
 
+int check_pools_apart(const tars_kv_pool* pool) {
+  const int64_t kv_row = static_cast<int64_t>(pool->dtype == TARS_KV_E4M3 ? 1 : 2) * pool->hd;
+  if (meet(Levels(kv_row, pool->pages, pool->kv_heads, pool->page, pool->k_page, pool->k_head, pool->k_slot),
+           Levels(kv_row, pool->pages, pool->kv_heads, pool->page, pool->v_page, pool->v_head, pool->v_slot),
+           static_cast<char*>(pool->v) - static_cast<char*>(pool->k)))
+    return fail(TARS_E_OVERLAP, "the K and V pools share memory");
+  return TARS_OK;
+}
+
 int check_rows(const void* p, int64_t& ld, int64_t n, int64_t row_bytes) {
   if (ld == 0) ld = row_bytes;
   if (ld < row_bytes || ld % 16) return fail(TARS_E_ALIGN, "strides must be multiples of 16 holding a row");
@@ -718,6 +727,115 @@ int attention_args(const float* const* q, int64_t ldq, const float* const* k, in
   return TARS_OK;
 }
 
+
+// ---- a serving step around the cache
+
+constexpr int kMaxMxK = 1 << 20, kMaxMxX = 1 << 22, kMaxMxW = 1 << 24, kMaxVocab = 1 << 24, kMaxGiven = 1 << 16, kMaxTop = 64;
+constexpr int64_t kMaxMxStride = 1 << 22;
+
+bool float_type(int32_t t) { return t == TARS_OUT_FP32 || t == TARS_OUT_BF16 || t == TARS_OUT_FP16; }
+int64_t mx_scale_row(int32_t k) { return (k + 511LL) / 512 * 16; }
+
+// A list of address intervals that an output must not meet.
+struct Others {
+  Mat at[16];
+  int n = 0;
+  void add(const void* p, int64_t bytes) {
+    if (p && bytes > 0) at[n++] = one(p, bytes);
+  }
+  void add(const Mat& m) { at[n++] = m; }
+  bool hit(const Mat& m) const {
+    for (int i = 0; i < n; ++i)
+      if (overlaps(m, at[i])) return true;
+    return false;
+  }
+};
+
+// q and the arguments that both of its forms share; c.seqs and, into a cache, c.pool are set.
+int check_rope(const void* q, int64_t& ldq, int32_t heads, int32_t kv_heads, int32_t hd, int32_t rows_, const float* qgamma,
+               const float* kgamma, float eps, const float* tab, int32_t positions, int32_t rot, void* yq, int64_t& ldyq) {
+  if (heads < 1 || heads > kMaxPagedHeads || kv_heads < 1 || kv_heads > kMaxPagedHeads) return fail(TARS_E_FIELD, "heads must be 1..1024");
+  if (!head_ok(hd)) return fail(TARS_E_FIELD, "hd must be 64, 128 or 256");
+  if (!(eps >= 0) || eps > 3e38f) return fail(TARS_E_FIELD, "eps must not be negative, and finite");
+  if (rot < 16 || rot > hd || rot % 16) return fail(TARS_E_ALIGN, "rot must be a multiple of 16, up to hd");
+  if (positions < 1) return fail(TARS_E_ALIGN, "positions >= 1");
+  if (!aligned(tab, 16) || !aligned(qgamma, 16) || !aligned(kgamma, 16)) return fail(TARS_E_ALIGN, "pointers must be 16-byte aligned");
+  if (positions > kMaxPositions) return fail(TARS_E_RANGE, "at most 2^30 positions");
+  if (static_cast<int64_t>(rows_) * heads > kMaxRowHeads) return fail(TARS_E_RANGE, "rows * heads must be at most 2^28");
+  if (!extent_ok(tab, 4LL * rot, positions, 4LL * rot)) return fail(TARS_E_RANGE, "extent overflows");
+  if (int rc = check_rows(q, ldq, rows_, 2LL * heads * hd)) return rc;
+  return check_rows(yq, ldyq, rows_, 2LL * heads * hd);
+}
+
+struct Mx4Rows {
+  tars::Mx4Matrix m;
+  Mat values, scales;
+};
+int check_mx4(const tars_mx4* m, int32_t most, Mx4Rows& c) {
+  if (!m || !m->values || !m->scales) return fail(TARS_E_ARG, "NULL pointer");
+  if (m->rows < 1 || m->k < 32 || m->k % 32) return fail(TARS_E_ALIGN, "rows >= 1, k a multiple of 32");
+  const int64_t vrow = m->k / 2, srow = mx_scale_row(m->k);
+  const int64_t ldv = m->ld_values ? m->ld_values : vrow, lds = m->ld_scales ? m->ld_scales : srow;
+  if (ldv < vrow || ldv % 16 || lds < srow || lds % 16) return fail(TARS_E_ALIGN, "strides must be multiples of 16 holding a row");
+  if (!aligned(m->values, 16) || !aligned(m->scales, 16)) return fail(TARS_E_ALIGN, "pointers must be 16-byte aligned");
+  if (m->rows > most || m->k > kMaxMxK || ldv > kMaxMxStride || lds > kMaxMxStride)
+    return fail(TARS_E_RANGE, "too many rows, k over 2^20 or strides over 2^22");
+  if (!extent_ok(m->values, ldv, m->rows, vrow) || !extent_ok(m->scales, lds, m->rows, srow)) return fail(TARS_E_RANGE, "extent overflows");
+  c.m = {static_cast<const char*>(m->values), static_cast<const uint8_t*>(m->scales), ldv, lds};
+  c.values = rows(m->values, ldv, m->rows, vrow);
+  c.scales = rows(m->scales, lds, m->rows, srow);
+  return TARS_OK;
+}
+
+// The product's weights, bias, output and workspace; the caller has set a.M, a.K and what x is.
+int check_mx4_product(const tars_mx4* w, const float* bias, void* y, int64_t ldy, int32_t out, void* work, int64_t work_bytes,
+                      int64_t need, const Others& x, tars::Mx4GemmArgs& a) {
+  if (!y) return fail(TARS_E_ARG, "NULL pointer");
+  if (!float_type(out)) return fail(TARS_E_FIELD, "out must be FP32, BF16 or FP16");
+  Mx4Rows c;
+  if (int rc = check_mx4(w, kMaxMxW, c)) return rc;
+  if (w->k != a.K) return fail(TARS_E_FIELD, "x and w disagree on k");
+  a.w = c.m;
+  a.N = w->rows;
+  a.bias = bias;
+  a.out = out;
+  a.y = static_cast<char*>(y);
+  const int64_t e = esize(out), row = e * a.N;
+  a.ldy = ldy ? ldy : row;
+  if (a.ldy < row || a.ldy % e || !aligned(y, e) || !aligned(bias, 4)) return fail(TARS_E_ALIGN, "y: whole elements, a stride that holds a row");
+  if (!extent_ok(y, a.ldy, a.M, row)) return fail(TARS_E_RANGE, "extent overflows");
+  a.wide_store = a.N % 4 == 0 && a.ldy % (4 * e) == 0 && aligned(y, 4 * e);
+  if (need > 0 && !work) return fail(TARS_E_ARG, "the call needs a workspace (tars_mx4_workspace)");
+  if (need > 0 && !aligned(work, 16)) return fail(TARS_E_ALIGN, "pointers must be 16-byte aligned");
+  if (work_bytes < need) return fail(TARS_E_RANGE, "the workspace is smaller than tars_mx4_workspace says");
+  Others in = x;
+  in.add(c.values);
+  in.add(c.scales);
+  in.add(bias, 4LL * a.N);
+  const Mat ym = rows(y, a.ldy, a.M, row);
+  if (in.hit(ym)) return fail(TARS_E_OVERLAP, "the output overlaps an input");
+  if (need > 0) {
+    in.add(ym);
+    if (in.hit(one(work, need))) return fail(TARS_E_OVERLAP, "the workspace overlaps an input or the output");
+  }
+  return TARS_OK;
+}
+
+// The workspace: x's codes and scales where a launch of its own makes them, then the product's.
+int64_t mx4_need(int32_t M, int32_t N, int32_t K, bool quantises) {
+  return (quantises && !tars::mx4_quantises(M) ? M * (K / 2 + mx_scale_row(K)) : 0) + tars::mx4_parts_bytes(M, N, K);
+}
+bool mx4_sizes_ok(int32_t M, int32_t N, int32_t K) {
+  return M >= 1 && N >= 1 && K >= 32 && K % 32 == 0 && M <= kMaxMxX && N <= kMaxMxW && K <= kMaxMxK;
+}
+bool logprobs_sizes_ok(int32_t rows_, int32_t vocab, int32_t dtype, int32_t top) {
+  return rows_ >= 1 && vocab >= 1 && float_type(dtype) && top >= 0 && top <= kMaxTop && top <= vocab && rows_ <= kMaxPagedRows && vocab <= kMaxVocab;
+}
+int64_t logprobs_need(int32_t rows_, int32_t vocab, int32_t dtype, int32_t top) {
+  const int parts = tars::logprobs_parts(rows_, vocab, dtype);
+  return parts > 1 ? static_cast<int64_t>(rows_) * parts * tars::logprobs_part_bytes(top) : 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -921,11 +1039,7 @@ int tars_kv_append(const tars_kv_pool* pool, const void* k, int64_t ldk, const v
   const int64_t row = 2LL * pool->kv_heads * pool->hd;
   if (int rc = check_rows(k, ldk, rows_, row)) return rc;
   if (int rc = check_rows(v, ldv, rows_, row)) return rc;
-  const int64_t kv_row = static_cast<int64_t>(pool->dtype == TARS_KV_E4M3 ? 1 : 2) * pool->hd;
-  if (meet(Levels(kv_row, pool->pages, pool->kv_heads, pool->page, pool->k_page, pool->k_head, pool->k_slot),
-           Levels(kv_row, pool->pages, pool->kv_heads, pool->page, pool->v_page, pool->v_head, pool->v_slot),
-           static_cast<char*>(pool->v) - static_cast<char*>(pool->k)))
-    return fail(TARS_E_OVERLAP, "the K and V pools share memory");
+  if (int rc = check_pools_apart(pool)) return rc;
   const Mat kin = rows(k, ldk, rows_, row), vin = rows(v, ldv, rows_, row);
   for (const Mat* m : {&c.k, &c.v}) {
     bool hit = overlaps(*m, kin) || overlaps(*m, vin);
@@ -964,6 +1078,203 @@ int tars_paged_decode(const tars_kv_pool* pool, const void* q, int64_t ldq, int3
                       int64_t work_bytes, void* stream) {
   return paged_attention(pool, q, ldq, dtype, heads, seqs, y, ldy, out, scale, window, sinks, table, ld_table, table_pages,
                          lens, nullptr, seqs, work, work_bytes, true, stream);
+}
+
+int tars_qk_norm_rope(const void* q, int64_t ldq, const void* k, int64_t ldk, int32_t dtype, int32_t heads, int32_t kv_heads,
+                      int32_t hd, int32_t rows_, const float* qgamma, const float* kgamma, float eps, const float* tab,
+                      int32_t positions, int32_t rot, const int32_t* lens, const int32_t* starts, int32_t seqs, void* yq,
+                      int64_t ldyq, void* yk, int64_t ldyk, void* stream) {
+  g_last_error.clear();
+  if (!q || !k || !yq || !yk || !tab || !lens) return fail(TARS_E_ARG, "NULL pointer");
+  if (dtype != TARS_KV_BF16 && dtype != TARS_KV_FP16) return fail(TARS_E_FIELD, "rows are BF16 or FP16");
+  if (seqs < 1 || rows_ < 1) return fail(TARS_E_ALIGN, "seqs, rows >= 1");
+  if (!starts && rows_ != seqs) return fail(TARS_E_FIELD, "without starts every sequence has one row");
+  if (!aligned(lens, 4) || !aligned(starts, 4)) return fail(TARS_E_ALIGN, "4-byte data must be 4-byte aligned");
+  if (rows_ > kMaxPagedRows || seqs > kMaxPagedSeqs) return fail(TARS_E_RANGE, "at most 2^22 rows and 65535 sequences");
+  if (int rc = check_rope(q, ldq, heads, kv_heads, hd, rows_, qgamma, kgamma, eps, tab, positions, rot, yq, ldyq)) return rc;
+  const int64_t krow = 2LL * kv_heads * hd, qrow = 2LL * heads * hd;
+  if (int rc = check_rows(k, ldk, rows_, krow)) return rc;
+  if (int rc = check_rows(yk, ldyk, rows_, krow)) return rc;
+  Others in;
+  in.add(tab, 4LL * rot * positions);
+  in.add(qgamma, qgamma ? 4LL * hd : 0);
+  in.add(kgamma, kgamma ? 4LL * hd : 0);
+  in.add(lens, 4LL * seqs);
+  in.add(starts, 4 * (seqs + 1LL));
+  const Mat qm = rows(q, ldq, rows_, qrow), km = rows(k, ldk, rows_, krow), yqm = rows(yq, ldyq, rows_, qrow), ykm = rows(yk, ldyk, rows_, krow);
+  const bool q_place = q == yq && ldq == ldyq, k_place = k == yk && ldk == ldyk;
+  if (in.hit(yqm) || in.hit(ykm) || (!q_place && overlaps(qm, yqm)) || (!k_place && overlaps(km, ykm)) || overlaps(qm, ykm) ||
+      overlaps(km, yqm))
+    return fail(TARS_E_OVERLAP, "an output overlaps an input that is not its own");
+  if (overlaps(yqm, ykm)) return fail(TARS_E_OVERLAP, "the outputs overlap");
+  tars::QkRopeArgs a{};
+  a.seqs = {nullptr, 0, lens, starts, seqs, rows_, kMaxPositions};
+  a.q = static_cast<const char*>(q);
+  a.k = static_cast<const char*>(k);
+  a.yq = static_cast<char*>(yq);
+  a.yk = static_cast<char*>(yk);
+  a.ldq = ldq, a.ldk = ldk, a.ldyq = ldyq, a.ldyk = ldyk;
+  a.qgamma = qgamma, a.kgamma = kgamma, a.tab = tab, a.eps = eps;
+  a.positions = positions, a.rot = rot, a.dtype = dtype, a.heads = heads, a.kv_heads = kv_heads, a.hd = hd;
+  return launched(tars::launch_qk_rope(a, static_cast<hipStream_t>(stream)));
+}
+
+int tars_kv_append_rope(const tars_kv_pool* pool, const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                        int32_t dtype, int32_t heads, int32_t rows_, const float* qgamma, const float* kgamma, float eps,
+                        const float* tab, int32_t positions, int32_t rot, const int32_t* table, int64_t ld_table,
+                        int32_t table_pages, const int32_t* lens, const int32_t* starts, int32_t seqs, void* yq, int64_t ldyq,
+                        void* stream) {
+  g_last_error.clear();
+  if (!q || !k || !v || !yq || !tab) return fail(TARS_E_ARG, "NULL pointer");
+  PagedCall c;
+  if (int rc = check_paged(pool, dtype, rows_, table, ld_table, table_pages, lens, starts, seqs, c)) return rc;
+  if (int rc = check_rope(q, ldq, heads, pool->kv_heads, pool->hd, rows_, qgamma, kgamma, eps, tab, positions, rot, yq, ldyq)) return rc;
+  const int64_t krow = 2LL * pool->kv_heads * pool->hd, qrow = 2LL * heads * pool->hd;
+  if (int rc = check_rows(k, ldk, rows_, krow)) return rc;
+  if (int rc = check_rows(v, ldv, rows_, krow)) return rc;
+  if (int rc = check_pools_apart(pool)) return rc;
+  Others in;
+  in.add(tab, 4LL * rot * positions);
+  in.add(qgamma, qgamma ? 4LL * pool->hd : 0);
+  in.add(kgamma, kgamma ? 4LL * pool->hd : 0);
+  for (int i = 0; i < c.nmeta; ++i) in.add(c.meta[i]);
+  in.add(rows(k, ldk, rows_, krow));
+  in.add(rows(v, ldv, rows_, krow));
+  const Mat qm = rows(q, ldq, rows_, qrow), yqm = rows(yq, ldyq, rows_, qrow);
+  if (in.hit(yqm) || (!(q == yq && ldq == ldyq) && overlaps(qm, yqm)))
+    return fail(TARS_E_OVERLAP, "the output overlaps an input that is not its own");
+  for (const Mat* m : {&c.k, &c.v})
+    if (in.hit(*m) || overlaps(*m, qm) || overlaps(*m, yqm)) return fail(TARS_E_OVERLAP, "the pool overlaps an input or the output");
+  tars::QkRopeArgs a{};
+  a.pool = c.pool;
+  a.seqs = c.seqs;
+  a.q = static_cast<const char*>(q);
+  a.k = static_cast<const char*>(k);
+  a.v = static_cast<const char*>(v);
+  a.yq = static_cast<char*>(yq);
+  a.ldq = ldq, a.ldk = ldk, a.ldv = ldv, a.ldyq = ldyq;
+  a.qgamma = qgamma, a.kgamma = kgamma, a.tab = tab, a.eps = eps;
+  a.positions = positions, a.rot = rot, a.dtype = dtype, a.heads = heads, a.kv_heads = pool->kv_heads, a.hd = pool->hd;
+  return launched(tars::launch_qk_rope(a, static_cast<hipStream_t>(stream)));
+}
+
+int tars_quant_mx4(const void* x, int64_t ldx, int32_t dtype, const tars_mx4* dst, void* stream) {
+  g_last_error.clear();
+  if (!x) return fail(TARS_E_ARG, "NULL pointer");
+  if (!float_type(dtype)) return fail(TARS_E_FIELD, "x must be FP32, BF16 or FP16");
+  Mx4Rows c;
+  if (int rc = check_mx4(dst, kMaxMxW, c)) return rc;
+  const int64_t row = static_cast<int64_t>(esize(dtype)) * dst->k;
+  if (int rc = check_rows(x, ldx, dst->rows, row)) return rc;
+  const Mat xm = rows(x, ldx, dst->rows, row);
+  if (overlaps(xm, c.values) || overlaps(xm, c.scales)) return fail(TARS_E_OVERLAP, "an output overlaps the input");
+  if (overlaps(c.values, c.scales)) return fail(TARS_E_OVERLAP, "the outputs overlap");
+  const tars::Mx4QuantArgs a{static_cast<const char*>(x), ldx, static_cast<char*>(dst->values), static_cast<uint8_t*>(dst->scales),
+                             c.m.ld_values, c.m.ld_scales, dst->rows, dst->k, static_cast<int>(mx_scale_row(dst->k)), dtype};
+  return launched(tars::launch_mx4_quant(a, static_cast<hipStream_t>(stream)));
+}
+
+int64_t tars_mx4_workspace(int32_t M, int32_t N, int32_t K, int32_t quantises) {
+  if (!mx4_sizes_ok(M, N, K)) return 0;
+  return mx4_need(M, N, K, quantises != 0);
+}
+
+int tars_gemm_mx4(const tars_mx4* x, const tars_mx4* w, const float* bias, void* y, int64_t ldy, int32_t out, void* work,
+                  int64_t work_bytes, void* stream) {
+  g_last_error.clear();
+  Mx4Rows c;
+  if (int rc = check_mx4(x, kMaxMxX, c)) return rc;
+  tars::Mx4GemmArgs a{};
+  a.x = c.m;
+  a.dtype = -1;
+  a.M = x->rows;
+  a.K = x->k;
+  Others in;
+  in.add(c.values);
+  in.add(c.scales);
+  const int64_t need = w && mx4_sizes_ok(a.M, w->rows, a.K) ? mx4_need(a.M, w->rows, a.K, false) : 0;
+  if (int rc = check_mx4_product(w, bias, y, ldy, out, work, work_bytes, need, in, a)) return rc;
+  a.work = static_cast<char*>(work);
+  return launched(tars::launch_mx4_gemm(a, static_cast<hipStream_t>(stream)));
+}
+
+int tars_quant_gemm_mx4(const void* x, int64_t ldx, int32_t dtype, int32_t M, const tars_mx4* w, const float* bias, void* y,
+                        int64_t ldy, int32_t out, void* work, int64_t work_bytes, void* stream) {
+  g_last_error.clear();
+  if (!x || !w) return fail(TARS_E_ARG, "NULL pointer");
+  if (!float_type(dtype)) return fail(TARS_E_FIELD, "x must be FP32, BF16 or FP16");
+  if (M < 1 || w->k < 32 || w->k % 32) return fail(TARS_E_ALIGN, "M >= 1, k a multiple of 32");
+  if (M > kMaxMxX || w->k > kMaxMxK) return fail(TARS_E_RANGE, "at most 2^22 rows of x, k up to 2^20");
+  const int64_t row = static_cast<int64_t>(esize(dtype)) * w->k;
+  if (int rc = check_rows(x, ldx, M, row)) return rc;
+  tars::Mx4GemmArgs a{};
+  a.rows = static_cast<const char*>(x);
+  a.ld_rows = ldx;
+  a.dtype = dtype;
+  a.M = M;
+  a.K = w->k;
+  Others in;
+  in.add(rows(x, ldx, M, row));
+  const int64_t need = mx4_sizes_ok(M, w->rows, w->k) ? mx4_need(M, w->rows, w->k, true) : 0;
+  if (int rc = check_mx4_product(w, bias, y, ldy, out, work, work_bytes, need, in, a)) return rc;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  a.work = static_cast<char*>(work);
+  if (!tars::mx4_quantises(M)) {  // into the workspace's first bytes
+    const int64_t values = static_cast<int64_t>(M) * (w->k / 2), pad = mx_scale_row(w->k);
+    a.x = {a.work, reinterpret_cast<const uint8_t*>(a.work + values), w->k / 2, pad};
+    const tars::Mx4QuantArgs qa{a.rows, ldx, a.work, reinterpret_cast<uint8_t*>(a.work + values), w->k / 2, pad, M, w->k,
+                                static_cast<int>(pad), dtype};
+    if (int rc = launched(tars::launch_mx4_quant(qa, s))) return rc;
+    a.dtype = -1;
+    a.work += values + M * pad;
+  }
+  return launched(tars::launch_mx4_gemm(a, s));
+}
+
+int64_t tars_logprobs_workspace(int32_t rows_, int32_t vocab, int32_t dtype, int32_t top) {
+  return logprobs_sizes_ok(rows_, vocab, dtype, top) ? logprobs_need(rows_, vocab, dtype, top) : 0;
+}
+
+int tars_token_logprobs(const void* x, int64_t ld, int32_t dtype, int32_t rows_, int32_t vocab, const void* tokens,
+                        int64_t ld_tokens, int32_t wide_tokens, int32_t given, float* logprobs, float* entropy, int32_t top,
+                        float* top_logprobs, int32_t* top_ids, void* work, int64_t work_bytes, void* stream) {
+  g_last_error.clear();
+  if (!x || !entropy || (given > 0 && (!tokens || !logprobs)) || (top > 0 && (!top_logprobs || !top_ids)))
+    return fail(TARS_E_ARG, "NULL pointer");
+  if (!float_type(dtype)) return fail(TARS_E_FIELD, "logits must be FP32, BF16 or FP16");
+  if (wide_tokens != 0 && wide_tokens != 1) return fail(TARS_E_FIELD, "wide_tokens is 0 or 1");
+  if (given < 0 || given > kMaxGiven) return fail(TARS_E_FIELD, "given must be 0..65536");
+  if (top < 0 || top > kMaxTop || top > vocab) return fail(TARS_E_FIELD, "top must be 0..64 and within the vocabulary");
+  if (rows_ < 1 || vocab < 1) return fail(TARS_E_ALIGN, "rows, vocab >= 1");
+  if (rows_ > kMaxPagedRows || vocab > kMaxVocab) return fail(TARS_E_RANGE, "at most 2^22 rows and 2^24 tokens in the vocabulary");
+  const int64_t e = esize(dtype), row = e * vocab, te = wide_tokens ? 8 : 4, trow = te * given;
+  if (ld == 0) ld = row;
+  if (ld_tokens == 0) ld_tokens = trow;
+  if (ld < row || ld % e || (given > 0 && (ld_tokens < trow || ld_tokens % te))) return fail(TARS_E_ALIGN, "strides: whole elements holding a row");
+  if (!aligned(x, e) || !aligned(tokens, te) || !aligned(logprobs, 4) || !aligned(entropy, 4) || !aligned(top_logprobs, 4) ||
+      !aligned(top_ids, 4))
+    return fail(TARS_E_ALIGN, "pointers must be aligned to their elements");
+  if (!extent_ok(x, ld, rows_, row) || !extent_ok(tokens, ld_tokens, rows_, trow)) return fail(TARS_E_RANGE, "extent overflows");
+  const int64_t need = logprobs_need(rows_, vocab, dtype, top);
+  if (need > 0 && !work) return fail(TARS_E_ARG, "the call needs a workspace (tars_logprobs_workspace)");
+  if (need > 0 && !aligned(work, 16)) return fail(TARS_E_ALIGN, "pointers must be 16-byte aligned");
+  if (work_bytes < need) return fail(TARS_E_RANGE, "the workspace is smaller than tars_logprobs_workspace says");
+  Others seen;  // the inputs, then each output too: none may meet another
+  seen.add(rows(x, ld, rows_, row));
+  if (given > 0) seen.add(rows(tokens, ld_tokens, rows_, trow));
+  const int64_t n = rows_;
+  const struct {
+    const void* p;
+    int64_t bytes;
+  } outs[] = {{entropy, 4 * n}, {logprobs, 4 * n * given}, {top_logprobs, 4 * n * top}, {top_ids, 4 * n * top}, {work, need}};
+  for (const auto& o : outs) {
+    if (!o.bytes) continue;
+    if (seen.hit(one(o.p, o.bytes))) return fail(TARS_E_OVERLAP, "an output or the workspace overlaps an input or another output");
+    seen.add(o.p, o.bytes);
+  }
+  const tars::LogprobArgs a{static_cast<const char*>(x), ld, rows_, vocab, dtype, tokens, ld_tokens, wide_tokens, given, top, logprobs,
+                            entropy, top_logprobs, top_ids, tars::logprobs_parts(rows_, vocab, dtype), need > 0 ? work : nullptr};
+  return launched(tars::launch_logprobs(a, static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

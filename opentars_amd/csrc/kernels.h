@@ -442,6 +442,76 @@ hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t s);
 // Few rows for each sequence (paged_rows.hip), one where seqs.starts is null.
 hipError_t launch_paged_rows(const PagedAttnArgs& a, hipStream_t s);
 
+// The norm of queries and keys for each head and their rotation (qk_rope.hip); into a cache where v is not null. Strides in bytes.
+struct QkRopeArgs {
+  KvPool pool;            // with v
+  KvSeqs seqs;            // its table with v
+  const char* q;          // [rows, heads * hd]
+  const char* k;          // [rows, kv_heads * hd]
+  const char* v;          // the same, or null
+  int64_t ldq, ldk, ldv;
+  char* yq;
+  char* yk;               // without v
+  int64_t ldyq, ldyk;
+  const float* qgamma;    // fp32 [hd], or null: no norm
+  const float* kgamma;
+  const float* tab;       // fp32 [positions, rot]
+  float eps;
+  int positions, rot, dtype, heads, kv_heads, hd;
+};
+hipError_t launch_qk_rope(const QkRopeArgs& a, hipStream_t s);
+
+// Microscaled 4-bit floating point (mx4.hip). Element types are the output codes: 0 fp32, 1 bf16, 3 binary16.
+struct Mx4QuantArgs {
+  const char* x;          // [M, K] at ldx bytes
+  int64_t ldx;
+  char* values;           // [M, K / 2] at ld_values
+  uint8_t* scales;        // [M, pad_blocks] at ld_scales, zeros behind a row's K / 32
+  int64_t ld_values, ld_scales;
+  int M, K, pad_blocks, dtype;
+};
+hipError_t launch_mx4_quant(const Mx4QuantArgs& a, hipStream_t s);
+struct Mx4Matrix {
+  const char* values;
+  const uint8_t* scales;
+  int64_t ld_values, ld_scales;
+};
+struct Mx4GemmArgs {
+  Mx4Matrix w;            // [N, K]
+  Mx4Matrix x;            // [M, K], with dtype -1
+  const char* rows;       // [M, K] of dtype at ld_rows bytes, quantised by the kernel: mx4_quantises(M)
+  int64_t ld_rows;
+  const float* bias;      // fp32 [N], or null
+  char* y;                // [M, N] at ldy bytes, of type out
+  int64_t ldy;
+  int M, N, K, dtype, out;
+  int wide_store;         // four neighbouring outputs are aligned and within N
+  char* work;             // mx4_parts_bytes()
+};
+bool mx4_quantises(int M);
+// Scratch of a product that is split over K between workgroups.
+int64_t mx4_parts_bytes(int M, int N, int K);
+hipError_t launch_mx4_gemm(const Mx4GemmArgs& a, hipStream_t s);
+
+// Log probabilities (logprobs.hip).
+struct LogprobArgs {
+  const char* x;          // [rows, vocab] of dtype (as above) at ld bytes
+  int64_t ld;
+  int rows, vocab, dtype;
+  const void* tokens;     // [rows, given], int32 or int64 (wide_tokens), at ld_tokens bytes
+  int64_t ld_tokens;
+  int wide_tokens, given, top;
+  float* logprobs;        // [rows, given]
+  float* entropy;         // [rows]
+  float* top_values;      // [rows, top]
+  int32_t* top_ids;
+  int parts;              // of a row, logprobs_parts(); more than one: work holds rows * parts * logprobs_part_bytes(top)
+  void* work;
+};
+__host__ __device__ __forceinline__ int64_t logprobs_part_bytes(int top) { return 16 + (top + 1) / 2 * 16; }
+int logprobs_parts(int rows, int vocab, int dtype);
+hipError_t launch_logprobs(const LogprobArgs& a, hipStream_t s);
+
 hipError_t launch_attention(const AttnArgs& a, hipStream_t s);
 // Prompt rows (attn_rows.hip): 16 query rows of a head per workgroup; the arguments of launch_attention
 // (no scratch, no norm + RoPE prologue).

@@ -24,6 +24,15 @@ and, outside the golden model and its bit-exactness, a serving cache in pages:
   paged_attention(cache, q, ..., starts) prompts' rows over the cache: causal, sliding window, first tokens
   paged_decode(cache, q, table, lens)    one row per sequence over the cache
 
+and what a serving step does before, between and after them:
+
+  Mx4(values, scales)                    a matrix in microscaled 4-bit floating point
+  quant_mx4(x)                           rows of a tensor as such a matrix
+  gemm_mx4(x, w, bias)                   x w^T + bias for such a w, x a tensor or in 4 bits too
+  qk_norm_rope(q, k, hd, tab, lens)      the norm of queries and keys for each head, and their rotation by position
+  kv_append_rope(cache, q, k, v, ...)    the same, the keys and the values going to their pages
+  token_logprobs(logits, tokens, top)    log probabilities of tokens, entropy, top alternatives
+
 Inputs are torch tensors on the GPU (results stay there, stream-ordered on the current stream),
 or numpy arrays (copied in; results come back as numpy after a synchronize, which is what
 golden-style callers expect). 2-D operands may be row-strided views whose rows are contiguous.
@@ -33,7 +42,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
-from typing import Sequence
+from typing import NamedTuple, Sequence
 
 import numpy as np
 import torch
@@ -688,6 +697,319 @@ def paged_decode(cache: PagedCache, q: torch.Tensor, table: torch.Tensor, lens: 
     return _paged(cache, q, table, lens, None, scale, window, sinks, out, y)
 
 
+# ---------------------------------------------------------------- a serving step around the cache
+_FLOATS = {torch.float32: OUT_FP32, torch.bfloat16: OUT_BF16, torch.float16: OUT_FP16}
+_OUT_FLOATS = {OUT_FP32: torch.float32, OUT_BF16: torch.bfloat16, OUT_FP16: torch.float16}
+
+
+def _on_current(index: int, *ts: torch.Tensor | None) -> None:
+    """Every tensor lives on the GPU `index`, and that is the current device, whose stream the call is on."""
+    for t in ts:
+        if t is not None and t.get_device() != index:
+            raise ValueError("the call's tensors must live on one GPU")
+    if torch.cuda.current_device() != index:
+        raise ValueError("the tensors' GPU must be the current device")
+
+
+def _own_rows(t: torch.Tensor, what: str) -> int:
+    """The row stride in bytes of a 2-D tensor whose rows are contiguous and rows of their own; 0, dense, for one row."""
+    if t.dim() != 2:
+        raise ValueError(f"{what} must be 2-D")
+    rows, cols = t.shape
+    return _row_stride(t, rows, cols, t.element_size())
+
+
+class Mx4:
+    """A matrix [rows, cols] in microscaled 4-bit floating point (OCP MXFP4), on the GPU: values uint8 [rows, cols / 2], two
+    e2m1 codes to a byte, the even column in the low half; scales uint8 [rows, cols / 32], the exponent byte b of each 32
+    columns, 2^(b - 127), 255 for NaN. cols is a multiple of 32. Made once for weights; quant_mx4 makes it of a tensor.
+    The products read whole 16-byte pieces of aligned rows: tensors that do not lie so are copied to where they do, and
+    later changes to them are not seen; .values and .scales are what the products read."""
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor):
+        if not (values.is_cuda and scales.is_cuda) or values.device != scales.device:
+            raise ValueError("values and scales must live on one GPU")
+        if values.dtype != torch.uint8 or scales.dtype != torch.uint8 or values.dim() != 2 or scales.dim() != 2:
+            raise ValueError("values and scales must be uint8 matrices")
+        rows, half = values.shape
+        if half % 16 or half == 0 or tuple(scales.shape) != (rows, half // 16):
+            raise ValueError("values must be [rows, cols / 2] and scales [rows, cols / 32], cols a multiple of 32")
+        if rows and (values.stride(1) != 1 or values.data_ptr() % 16 or (rows > 1 and (values.stride(0) < half or values.stride(0) % 16))):
+            values = values.contiguous()
+            values = values.clone() if values.data_ptr() % 16 else values
+        pad = -(-half // 256) * 16
+        if rows and not _whole_pieces(scales, rows, pad):
+            room = torch.zeros((rows, pad), dtype=torch.uint8, device=scales.device)
+            room[:, :half // 16] = scales
+            scales = room[:, :half // 16]
+        self._set(values, scales, rows, 2 * half)
+
+    def _set(self, values: torch.Tensor, scales: torch.Tensor, rows: int, cols: int) -> None:
+        _fit_int32(rows, cols)
+        self.values, self.scales, self.rows, self.cols = values, scales, rows, cols
+        self.device, self.index = values.device, values.get_device()
+        self._mx = _lib.Mx4(values.data_ptr(), scales.data_ptr(), values.stride(0) if rows > 1 else 0,
+                            scales.stride(0) if rows > 1 else 0, rows, cols)
+        self._ref = ctypes.byref(self._mx)
+
+
+def _whole_pieces(scales: torch.Tensor, rows: int, pad: int) -> bool:
+    """Whether each row of scales starts a 16-byte piece and its last piece belongs to the tensor's memory."""
+    if scales.data_ptr() % 16 or (scales.shape[1] > 1 and scales.stride(1) != 1):
+        return False
+    ld = scales.stride(0)
+    if rows > 1 and (ld < pad or ld % 16):
+        return False
+    return scales.storage_offset() + (rows - 1) * ld + pad <= scales.untyped_storage().nbytes()
+
+
+def _mx4_rows(x: torch.Tensor, what: str = "x"):
+    """Element code, shape and row stride (bytes) of rows that are quantised."""
+    code = _FLOATS.get(x.dtype)
+    if code is None:
+        raise ValueError(f"{what} must be fp32, bf16 or fp16")
+    if not x.is_cuda:
+        raise ValueError(f"{what} must live on the GPU")
+    return code, *x.shape, _own_rows(x, what)
+
+
+def quant_mx4(x: torch.Tensor) -> Mx4:
+    """x [rows, cols], fp32, bf16 or fp16, cols a multiple of 32, in microscaled 4 bits: each 32 columns' scale has the exponent
+    of their largest magnitude, less 2; x over it is rounded to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6, even codes on a tie
+    and 6 past it. A block that holds an infinity or NaN is NaN."""
+    code, rows, cols, ld = _mx4_rows(x)
+    if cols % 32 or cols == 0:
+        raise ValueError("x must be [rows, cols], cols a multiple of 32")
+    _on_current(x.get_device())
+    values = torch.empty((rows, cols // 2), dtype=torch.uint8, device=x.device)
+    pad = -(-cols // 512) * 16
+    scales = torch.empty((rows, pad), dtype=torch.uint8, device=x.device)
+    m = Mx4.__new__(Mx4)
+    m._set(values, scales[:, :cols // 32], rows, cols)
+    m._mx.ld_scales = pad
+    if rows:
+        _check(_lib.lib().tars_quant_mx4(x.data_ptr(), ld, code, m._ref, _stream()))
+    return m
+
+
+@functools.lru_cache(maxsize=1024)
+def _mx4_workspace(*sizes: int) -> int:
+    return _lib.lib().tars_mx4_workspace(*sizes)
+
+
+def gemm_mx4(x: torch.Tensor | Mx4, w: Mx4, bias: torch.Tensor | None = None, out: int | None = None,
+             y: torch.Tensor | None = None) -> torch.Tensor:
+    """y = x w^T + bias for a weight matrix w [N, K] in microscaled 4 bits. x [M, K]: a tensor (fp32, bf16 or fp16), which the
+    call quantises as quant_mx4 does, or an Mx4. bias fp32 [N]. Sums are fp32 and rounded once, to out (OUT_FP32, OUT_BF16,
+    OUT_FP16; a given y's type, else x's own, else OUT_BF16). y [M, N], rows contiguous."""
+    mx = isinstance(x, Mx4)
+    if mx:
+        code, M, K, ld = None, x.rows, x.cols, 0
+        index = x.index
+    else:
+        code, M, K, ld = _mx4_rows(x)
+        index = x.get_device()
+    if K != w.cols:
+        raise ValueError("x must be [M, K] for a w of [N, K]")
+    N = w.rows
+    if bias is not None:
+        if bias.dtype != torch.float32:
+            raise ValueError("bias must be fp32")
+        _vec(bias, N, "bias")
+    if y is None:
+        if out is None:
+            out = OUT_BF16 if mx else code
+        elif out not in _OUT_FLOATS:
+            raise ValueError("out must be OUT_FP32, OUT_BF16 or OUT_FP16")
+        _on_current(index, w.values, bias)
+        y = torch.empty((M, N), dtype=_OUT_FLOATS[out], device=w.device)
+        ldy = 0
+    else:
+        own = _FLOATS.get(y.dtype)
+        if own is None or (out is not None and out != own) or y.shape != (M, N):
+            raise ValueError("y must be [M, N], of the type that out names")
+        _on_current(index, w.values, bias, y)
+        out, ldy = own, _own_rows(y, "y")
+    if M == 0 or N == 0:
+        return y
+    _fit_int32(M)
+    lib = _lib.lib()
+    need = _mx4_workspace(M, N, K, not mx)
+    work = torch.empty(need, dtype=torch.uint8, device=w.device) if need else None
+    if mx:
+        _check(lib.tars_gemm_mx4(x._ref, w._ref, _ptr(bias), y.data_ptr(), ldy, out, _ptr(work), need, _stream()))
+    else:
+        _check(lib.tars_quant_gemm_mx4(x.data_ptr(), ld, code, M, w._ref, _ptr(bias), y.data_ptr(), ldy, out, _ptr(work), need,
+                                       _stream()))
+    return y
+
+
+def _rope_rows(index: int, t: torch.Tensor, what: str, hd: int):
+    """The element code, rows, heads and row stride (bytes) of packed rows of heads."""
+    code = _KV_DTYPES.get(t.dtype)
+    if code is None or code == 2:
+        raise ValueError(f"{what} must be bf16 or fp16")
+    if t.get_device() != index:
+        raise ValueError(f"{what} must live on the call's GPU")
+    if t.dim() != 2:
+        raise ValueError("expected a 2-D tensor with contiguous rows")
+    rows, cols = t.shape
+    heads = cols // hd
+    if heads * hd != cols or heads < 1:
+        raise ValueError(f"{what} must be [rows, heads * hd]")
+    return code, rows, heads, _row_stride(t, rows, cols, 2)
+
+
+def _rope_out(y: torch.Tensor | None, x: torch.Tensor, what: str):
+    """A rope output like x (zeros: rows without a position keep what it holds) and its row stride."""
+    if y is None:
+        return torch.zeros(x.shape, dtype=x.dtype, device=x.device), 0
+    if y.shape != x.shape or y.get_device() != x.get_device() or _KV_DTYPES.get(y.dtype) != _KV_DTYPES[x.dtype]:
+        raise ValueError(f"{what} must have its input's shape, type and place")
+    return y, _row_stride(y, *y.shape, 2)
+
+
+def _rope_consts(index: int, hd: int, tab: torch.Tensor, qgamma: torch.Tensor | None, kgamma: torch.Tensor | None):
+    if tab.dtype != torch.float32 or tab.dim() != 2 or not tab.is_contiguous() or tab.get_device() != index:
+        raise ValueError("tab must be a dense fp32 [positions, rot] table on the call's GPU")
+    for t, what in ((qgamma, "qgamma"), (kgamma, "kgamma")):
+        if t is not None:
+            if t.dtype != torch.float32 or t.get_device() != index:
+                raise ValueError(f"{what} must be fp32 on the call's GPU")
+            _vec(t, hd, what)
+    positions, rot = tab.shape
+    _fit_int32(positions, rot)
+    return tab.data_ptr(), positions, rot
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, hd: int, tab: torch.Tensor, lens: torch.Tensor,
+                 starts: torch.Tensor | None = None, qgamma: torch.Tensor | None = None, kgamma: torch.Tensor | None = None,
+                 eps: float = 1e-6, yq: torch.Tensor | None = None, yk: torch.Tensor | None = None):
+    """The RMS norm of each head of q [rows, heads * hd] and k [rows, kv_heads * hd] (bf16 or fp16, columns of one projection's
+    output, say) times qgamma / kgamma (fp32 [hd]; without one, no norm), and their rotation by position, in one pass:
+    fp32 all the way, rounded once. tab fp32 [positions, rot], row p = [cos, sin] of position p as rope_rows takes it (rot a
+    multiple of 16, up to hd: the first rot elements turn, i with i + rot / 2). lens, starts: the rows' sequences, as
+    kv_append's; row i of a sequence's n is at position lens - n + i. Returns (yq, yk), like q and k; a given yq or yk may be
+    q or k itself. Rows behind the last sequence, at negative positions or at ones that tab does not have stay as they were
+    in a given output (0 without one)."""
+    index = q.get_device()
+    if hd < 1:
+        raise ValueError("hd must be 64, 128 or 256")
+    code, rows, heads, ldq = _rope_rows(index, q, "q", hd)
+    kcode, krows, kv_heads, ldk = _rope_rows(index, k, "k", hd)
+    if kcode != code or krows != rows:
+        raise ValueError("q and k must have one type and the same rows")
+    if lens.dtype != torch.int32 or lens.dim() != 1 or (starts is not None and starts.dtype != torch.int32):
+        raise ValueError("lens and starts must be int32 vectors")
+    seqs = lens.shape[0]
+    _vec(lens, seqs, "lens")
+    if starts is not None:
+        _vec(starts, seqs + 1, "starts")
+    elif rows != seqs:
+        raise ValueError("q must have a row for each sequence")
+    _on_current(index, lens, starts)
+    tp, positions, rot = _rope_consts(index, hd, tab, qgamma, kgamma)
+    _fit_int32(rows, heads, kv_heads, hd, seqs)
+    yq, ldyq = _rope_out(yq, q, "yq")
+    yk, ldyk = _rope_out(yk, k, "yk")
+    if rows == 0 or seqs == 0:
+        return yq, yk
+    _check(_lib.lib().tars_qk_norm_rope(q.data_ptr(), ldq, k.data_ptr(), ldk, code, heads, kv_heads, hd, rows, _ptr(qgamma),
+                                        _ptr(kgamma), eps, tp, positions, rot, lens.data_ptr(), _ptr(starts), seqs,
+                                        yq.data_ptr(), ldyq, yk.data_ptr(), ldyk, _stream()))
+    return yq, yk
+
+
+def kv_append_rope(cache: PagedCache, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+                   tab: torch.Tensor, starts: torch.Tensor | None = None, qgamma: torch.Tensor | None = None,
+                   kgamma: torch.Tensor | None = None, eps: float = 1e-6, yq: torch.Tensor | None = None) -> torch.Tensor:
+    """qk_norm_rope and kv_append in one pass: the keys, normed and rotated, and the values as they are go to the pages of their
+    sequences (an e4m3 pool gets the fp32 key over its scale, rounded once), and the queries come back, ready for
+    paged_attention or paged_decode. Arguments as theirs; a position that tab does not have is not stored either."""
+    index, hd = cache.index, cache.hd
+    code, rows, heads, ldq = _rope_rows(index, q, "q", hd)
+    kcode, krows, kheads, ldk = _rope_rows(index, k, "k", hd)
+    vcode, vrows, vheads, ldv = _rope_rows(index, v, "v", hd)
+    if kcode != code or vcode != code or krows != rows or vrows != rows:
+        raise ValueError("q, k and v must have one type and the same rows")
+    if kheads != cache.kv_heads or vheads != cache.kv_heads:
+        raise ValueError("k and v must be [rows, kv_heads * hd]")
+    meta = _paged_meta(cache, table, lens, starts)
+    if starts is None and rows != meta[5]:
+        raise ValueError("q must have a row for each sequence")
+    tp, positions, rot = _rope_consts(index, hd, tab, qgamma, kgamma)
+    _fit_int32(rows, heads, meta[2], meta[5])
+    yq, ldyq = _rope_out(yq, q, "yq")
+    if rows == 0 or meta[5] == 0:
+        return yq
+    _check(_lib.lib().tars_kv_append_rope(cache._ref, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, code, heads, rows,
+                                          _ptr(qgamma), _ptr(kgamma), eps, tp, positions, rot, *meta, yq.data_ptr(), ldyq,
+                                          _stream()))
+    return yq
+
+
+class TokenLogprobs(NamedTuple):
+    """token_logprobs' results: fp32 like tokens (None without), fp32 [rows], fp32 and int32 [rows, top] (None with top 0)."""
+    logprobs: torch.Tensor | None
+    entropy: torch.Tensor
+    top_logprobs: torch.Tensor | None
+    top_ids: torch.Tensor | None
+
+
+@functools.lru_cache(maxsize=1024)
+def _logprobs_workspace(*sizes: int) -> int:
+    return _lib.lib().tars_logprobs_workspace(*sizes)
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top: int = 0) -> TokenLogprobs:
+    """Log probabilities of `tokens` (int32 or int64, [rows] or [rows, n]) under the softmax of each row of logits
+    [rows, vocab] (fp32, bf16 or fp16; rows contiguous), its entropy in nats, and the `top` (up to 64) most likely tokens, the
+    lower of two equal ones first, all in one pass over the logits. A logit of -infinity is a token that cannot come; a row
+    of nothing else gives -infinity for every token and entropy 0. Tokens outside the vocabulary (-1 for padding) get
+    -infinity. A row with a NaN or +infinity gives NaN."""
+    code = _FLOATS.get(logits.dtype)
+    if code is None:
+        raise ValueError("logits must be fp32, bf16 or fp16")
+    if not logits.is_cuda:
+        raise ValueError("logits must live on the GPU")
+    ld = _own_rows(logits, "logits")
+    rows, vocab = logits.shape
+    given = wide = ldt = 0
+    lp = tv = ti = None
+    device = logits.device
+    _on_current(logits.get_device(), tokens)
+    if tokens is not None:
+        if tokens.dtype not in (torch.int32, torch.int64) or tokens.dim() not in (1, 2) or tokens.shape[0] != rows:
+            raise ValueError("tokens must be int32 or int64, [rows] or [rows, n]")
+        wide = int(tokens.dtype == torch.int64)
+        if tokens.dim() == 1:
+            given = 1
+            ldt = tokens.stride(0) * tokens.element_size()
+            if rows > 1 and ldt <= 0:
+                raise ValueError("tokens must have elements of their own")
+            ldt = ldt if rows > 1 else 0
+        else:
+            given = tokens.shape[1]
+            ldt = _own_rows(tokens, "tokens") if given else 0
+        lp = torch.empty(tokens.shape, dtype=torch.float32, device=device)
+    _fit_int32(rows, vocab, given, top)
+    if not 0 <= top <= min(64, vocab):
+        raise ValueError("top must be 0..64 and within the vocabulary")
+    entropy = torch.empty(rows, dtype=torch.float32, device=device)
+    if top:
+        tv = torch.empty((rows, top), dtype=torch.float32, device=device)
+        ti = torch.empty((rows, top), dtype=torch.int32, device=device)
+    result = TokenLogprobs(lp, entropy, tv, ti)
+    if rows == 0:
+        return result
+    need = _logprobs_workspace(rows, vocab, code, top)
+    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _check(_lib.lib().tars_token_logprobs(logits.data_ptr(), ld, code, rows, vocab, tokens.data_ptr() if given else None, ldt, wide,
+                                          given, lp.data_ptr() if given else None, entropy.data_ptr(), top, _ptr(tv), _ptr(ti),
+                                          _ptr(work), need, _stream()))
+    return result
+
+
 def set_w8a8_path(path: str) -> str:
     """'auto' | 'gemv' | 'mfma': which W8A8 kernel family runs for M >= 2 (and M = 1). Returns the
     previous setting."""
@@ -698,7 +1020,8 @@ def set_w8a8_path(path: str) -> str:
 
 __all__ = ["TarsError", "ContractError", "quant_rows", "gemm_rowcol", "quant_gemm_rowcol", "gemm_rowcol_ksplit",
            "align_w4_groups", "gemm_w4", "embed_rows", "attention",
-           "PagedCache", "kv_append", "paged_attention", "paged_decode", "set_w8a8_path", "ESIZE", "softmax_rows", "softmax_rows_causal",
+           "PagedCache", "kv_append", "paged_attention", "paged_decode", "Mx4", "quant_mx4", "gemm_mx4", "qk_norm_rope",
+           "kv_append_rope", "TokenLogprobs", "token_logprobs", "set_w8a8_path", "ESIZE", "softmax_rows", "softmax_rows_causal",
            "layernorm_rows", "rmsnorm_rows", "l2norm_rows", "relu", "elt", "rope_rows", "fdot_nt", "fdot_nn",
            "ROW_SOFTMAX", "ROW_LAYERNORM", "ROW_RMSNORM", "ROW_L2NORM", "ELT_MUL", "ELT_ADD", "ELT_MULADD",
            "ELT_SUB", "BM_DENSE", "BM_ROW", "BM_COL", "BM_SCALAR"]
