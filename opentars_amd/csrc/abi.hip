@@ -804,6 +804,7 @@ int check_mx4_product(const tars_mx4* w, const float* bias, void* y, int64_t ldy
   a.ldy = ldy ? ldy : row;
   if (a.ldy < row || a.ldy % e || !aligned(y, e) || !aligned(bias, 4)) return fail(TARS_E_ALIGN, "y: whole elements, a stride that holds a row");
   if (!extent_ok(y, a.ldy, a.M, row)) return fail(TARS_E_RANGE, "extent overflows");
+  a.wide_rows = a.ldy % 16 == 0 && a.ldy <= 1 << 23 && aligned(y, 16) && aligned(bias, 16);
   a.wide_store = a.N % 4 == 0 && a.ldy % (4 * e) == 0 && aligned(y, 4 * e);
   if (need > 0 && !work) return fail(TARS_E_ARG, "the call needs a workspace (tars_mx4_workspace)");
   if (need > 0 && !aligned(work, 16)) return fail(TARS_E_ALIGN, "pointers must be 16-byte aligned");

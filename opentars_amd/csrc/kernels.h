@@ -486,6 +486,7 @@ struct Mx4GemmArgs {
   int64_t ldy;
   int M, N, K, dtype, out;
   int wide_store;         // four neighbouring outputs are aligned and within N
+  int wide_rows;          // y's rows, 2^23 bytes apart at most, and bias lie on 16 bytes
   char* work;             // mx4_parts_bytes()
 };
 bool mx4_quantises(int M);
