@@ -5,10 +5,14 @@
 // S' = f S, T' = f (T + (m - m') S); lanes, waves and parts of a row are joined by the same rule, in order. A logit of
 // -infinity adds nothing; NaN and +infinity make S NaN, and with it every result of the row.
 //
-// The top alternatives are kept for each wave as a sorted list of 64-bit keys, one to a lane: the logit's bits in an order that
-// whole numbers keep (NaN last), above the place counted down, so that equal logits are in order of their places and no two keys
-// are equal. A logit below the list's last is passed by with one comparison; the first group of loads is filtered by the top-th
-// largest of the lanes' maxima.
+// The top alternatives are found by 64-bit keys: the logit's bits in an order that whole numbers keep (NaN last), above the place
+// counted down, so that equal logits are in order of their places and no two keys are equal. The pass over the logits only notes,
+// to 16 bits, the largest of each group of a lane's loads. The top-th largest of the lanes' maxima is a bound that at least `top`
+// logits reach, and little more than that do: the few groups that reach it are fetched again, and the logits above the bound go to
+// their wave's list in LDS. A list that fills up is cut to its largest `top`, the last of which is the wave's new bound. A key's
+// place among the largest is the number of larger ones, counted over all lists at the end.
+//
+// A workgroup takes a row, or a part of one where there are few; a second launch joins the parts.
 #include <algorithm>
 
 #include "kernels.h"
@@ -18,6 +22,7 @@ namespace tars {
 namespace {
 
 constexpr int kWaves = 4, kLoads = 4, kLanes = 64;
+constexpr int kGroups = 32;  // of a lane's loads, whose maxima are noted
 constexpr float kLog2e = 1.44269504f, kFar = -1e4f;  // e^kFar is 0 in fp32
 
 struct Sums {
@@ -55,34 +60,68 @@ __device__ __forceinline__ Key lane_key(Key k, int lane) {
          static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(k), lane));
 }
 
-// A wave's largest keys, lane i the i-th; 0 where there is none.
-struct List {
-  Key mine = 0, last = 0;  // last: the top-th, or a bound below which nothing counts
-  __device__ __forceinline__ void take(Key k, bool in, int top) {
-    const int lane = threadIdx.x & 63;
-    uint64_t todo = __ballot(in && k > last);
-    while (todo) {
-      const Key c = lane_key(k, __builtin_ctzll(todo));
-      const int at = __popcll(__ballot(mine > c));
-      const Key up = static_cast<Key>(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(mine >> 32), 0x138, 0xF, 0xF, false))) << 32 |
-                     static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(mine), 0x138, 0xF, 0xF, false));  // the lane before's
-      mine = lane < at ? mine : lane == at ? c : up;
-      const Key end = lane_key(mine, top - 1);
-      last = end > last ? end : last;
-      todo &= todo - 1;
-      todo &= __ballot(k > last);
-    }
-  }
+constexpr int kAtOnce = 4;                     // keys of a lane that are offered together
+constexpr int kRoom = (1 + kAtOnce) * kLanes;  // of a wave's list: 64 and what may be offered
+constexpr int kAhead = 8;                      // keys that a count fetches at once: lists end in as many zeros
+struct Shared {
+  Key keys[kWaves][kRoom + kAhead];
+  Key all[kWaves * kLanes + kAhead];
+  Key top[kLanes];
+  uint16_t group[kGroups][kWaves * kLanes];
+  uint32_t most[kWaves][kLanes];
+  Key bound;
+  int equal;
+  int n[kWaves];
+  float sums[kWaves][3];
 };
 
-// The n-th largest of the lanes' values.
-__device__ __forceinline__ uint32_t nth_of(uint32_t x, int n) {
-  uint32_t v = 0;
+// A wave's list of keys above its bound.
+struct List {
+  Key* keys;  // kRoom of them in LDS
+  Key last = 0;
+  int n = 0, top;
+  // At most kAtOnce times between two calls of cut().
+  __device__ __forceinline__ void take(Key k, bool in) {
+    const int lane = threadIdx.x & 63;
+    const uint64_t who = __ballot(in && k > last);
+    const int at = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(who >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(who), 0));
+    if (who >> lane & 1) keys[n + at] = k;
+    n += __popcll(who);
+  }
+  // Where the list has more than 64, keeps the largest `top`.
+  __device__ __forceinline__ void cut() {
+    if (n <= kLanes) return;
+    const int lane = threadIdx.x & 63;
+    Key a[kRoom / kLanes];
+    int place[kRoom / kLanes];
+    if (lane < kAhead) keys[n + lane] = 0;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < kRoom / kLanes; ++i) {
+      a[i] = lane + kLanes * i < n ? keys[lane + kLanes * i] : 0;
+      place[i] = 0;
+    }
 #pragma unroll 1
-  for (uint32_t bit = 0x80000000u; bit; bit >>= 1)
-    if (__popcll(__ballot(x >= (v | bit))) >= n) v |= bit;
-  return v;
-}
+    for (int k = 0; k < n; k += kAhead) {
+      Key c[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) c[i] = keys[k + i];
+#pragma unroll
+      for (int i = 0; i < kRoom / kLanes; ++i)
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) place[i] += c[j] > a[i];
+    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < kRoom / kLanes; ++i)
+      if (a[i] && place[i] < top) keys[place[i]] = a[i];
+    __builtin_amdgcn_wave_barrier();
+    n = min(n, top);
+    const Key end = keys[top - 1];
+    last = static_cast<Key>(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(end >> 32)))) << 32 |
+           static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(end)));
+  }
+};
 
 struct XF32 {
   static constexpr int kEach = 4;  // logits in 16 bytes
@@ -114,39 +153,93 @@ __device__ __forceinline__ Sums over_wave(Sums a) {
   return a;
 }
 
-struct Shared {
-  Key keys[kWaves][kLanes];
-  Key top[kLanes];
-  Sums sums[kWaves];
-};
-
-// The waves' lists as one in sh.top: a key's place is its own list's and the number of larger ones in each other. The waves' sums joined.
-__device__ __forceinline__ Sums over_workgroup(Shared& sh, Sums a, Key mine, int top) {
+// The workgroup's bound, for every wave: the top-th largest of the lanes' maxima, to 16 bits of their `ordered` values (0: a lane
+// without one); where more lanes than that are equal by those bits, by their whole keys (place() is where a lane has its maximum
+// first).
+template <class F>
+__device__ __forceinline__ Key bound_of(Shared& sh, uint32_t most, int top, F place) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  a = over_wave(a);
-  if (lane == 0) sh.sums[wave] = a;
-  if (top) {
-    sh.keys[wave][lane] = mine;
-    if (wave == 0) sh.top[lane] = 0;
+  const bool mine = wave == static_cast<int>((blockIdx.x + blockIdx.y) & (kWaves - 1));  // one wave's work, another's in each workgroup
+  sh.most[wave][lane] = most >> 16;
+  __syncthreads();
+  if (mine) {
+    uint32_t x[kWaves], v = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) x[w] = sh.most[w][lane];
+    int reach = 0;
+#pragma unroll
+    for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
+      int count = 0;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) count += __popcll(__ballot(x[w] >= (v | bit)));
+      if (count >= top) v |= bit, reach = count;
+    }
+    if (lane == 0) {
+      sh.bound = static_cast<Key>(v) << 48;
+      sh.equal = v != 0 && reach > top + 24;
+    }
   }
   __syncthreads();
-  if (top && lane < top) {
-    int place = lane;
+  Key b = sh.bound;
+  if (sh.equal) {
+    sh.keys[wave][lane] = most ? static_cast<Key>(most) << 32 | static_cast<uint32_t>(~place()) : 0;
+    __syncthreads();
+    Key k[kWaves];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) {
-      const Key* other = sh.keys[(wave + w) % kWaves];
-      int n = 0;  // the first ones are larger
+    for (int w = 0; w < kWaves; ++w) k[w] = sh.keys[w][lane];
+#pragma unroll 1
+    for (Key bit = Key{1} << 47; bit; bit >>= 1) {
+      int count = 0;
 #pragma unroll
-      for (int step = 32; step; step /= 2)
-        if (other[n + step - 1] > mine) n += step;
-      if (n == 63 && other[63] > mine) n = 64;
-      place += n;
+      for (int w = 0; w < kWaves; ++w) count += __popcll(__ballot(k[w] >= (b | bit)));
+      if (count >= top) b |= bit;
     }
-    if (mine && place < top) sh.top[place] = mine;
+    __syncthreads();  // before the lists take the keys' room
   }
-  Sums all = sh.sums[0];
+  return b ? b - 1 : 0;
+}
+
+// The waves' lists as one in sh.top, the largest key first, 0 behind the last; their sums joined.
+__device__ __forceinline__ Sums over_workgroup(Shared& sh, Sums a, List& list) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (list.top) list.cut();
+  a = over_wave(a);
+  if (lane == 0) {
+    sh.sums[wave][0] = a.m;
+    sh.sums[wave][1] = a.s;
+    sh.sums[wave][2] = a.t;
+    sh.n[wave] = list.n;
+  }
+  if (wave == 0) sh.top[lane] = 0;
+  __syncthreads();
+  if (list.top) {
+    int first = 0, n = 0;
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) all.join(sh.sums[w]);
+    for (int w = 0; w < kWaves; ++w) {
+      first += w < wave ? sh.n[w] : 0;
+      n += sh.n[w];
+    }
+    if (lane < list.n) sh.all[first + lane] = list.keys[lane];
+    if (wave == 0 && lane < kAhead) sh.all[n + lane] = 0;
+    __syncthreads();
+    const int t = threadIdx.x;
+    if (64 * wave < n) {
+      const Key mine = t < n ? sh.all[t] : 0;
+      int place = 0;
+#pragma unroll 1
+      for (int k = 0; k < n; k += kAhead) {
+        Key c[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) c[i] = sh.all[k + i];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) place += c[i] > mine;
+      }
+      if (mine && place < list.top) sh.top[place] = mine;
+    }
+  }
+  Sums all{sh.sums[0][0], sh.sums[0][1], sh.sums[0][2]};
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) all.join({sh.sums[w][0], sh.sums[w][1], sh.sums[w][2]});
   __syncthreads();
   return all;
 }
@@ -179,7 +272,7 @@ __device__ __forceinline__ char* part_at(const LogprobArgs& a, int row, int part
 }
 
 template <class X, bool TOP>
-__global__ __launch_bounds__(64 * kWaves) void logprobs_kernel(LogprobArgs a) {
+__global__ __launch_bounds__(64 * kWaves, 4) void logprobs_kernel(LogprobArgs a) {
   __shared__ Shared sh;
   constexpr int kEach = X::kEach, kSize = 16 / kEach;
   const int row = blockIdx.y + blockIdx.z * 65535, part = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -192,64 +285,123 @@ __global__ __launch_bounds__(64 * kWaves) void logprobs_kernel(LogprobArgs a) {
   const int share = ceil_div(ceil_div(pieces, a.parts * kWaves), 64) * 64;
   const int p0 = min(pieces, (part * kWaves + wave) * share), p1 = min(pieces, p0 + share);
   Sums sums = Sums::none();
-  List list;
-  if (part == 0 && wave == 0 && head + tail > 0) {
-    const bool in = lane < head + tail;
-    const int at = lane < head ? lane : a.vocab - tail + lane - head;
-    const float v = in ? X::one(x + static_cast<int64_t>(at) * kSize) : -INFINITY;
-    if (in) {
-      sums.move(fmaxf(sums.m, v));
-      sums.add(v);
-    }
-    if constexpr (TOP) list.take(key_of(v, at), in, a.top);
+  List list{sh.keys[wave]};
+  list.top = TOP ? a.top : 0;
+  // the logits around the pieces
+  const bool edge = part == 0 && wave == 0 && lane < head + tail;
+  const int edge_at = lane < head ? lane : a.vocab - tail + lane - head;
+  const float edge_v = edge ? X::one(x + static_cast<int64_t>(edge_at) * kSize) : -INFINITY;
+  if (edge) {
+    sums.move(fmaxf(sums.m, edge_v));
+    sums.add(edge_v);
   }
-  bool first = true;
+  const auto load = [&](int p, uint4 (&w)[kLoads]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) w[i] = *reinterpret_cast<const uint4*>(body + 16ll * min(p + 64 * i + lane, p1 - 1));
+  };
+  const auto unpack = [&](int p, const uint4 (&w)[kLoads], float (&v)[kLoads][kEach]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const uint32_t word[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) v[i][e] = X::at(word, e);
+    }
+    if (p + 64 * kLoads > p1)
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) v[i][e] = p + 64 * i + lane < p1 ? v[i][e] : -INFINITY;
+  };
+  const int steps = ceil_div(share, 64 * kLoads), stride = ceil_div(steps, kGroups);  // steps of a wave, and of a group
+  float most = -INFINITY, in_group = -INFINITY;
+  uint4 w[kLoads];
+  if (p0 < p1) load(p0, w);
+  int left = stride, group = 0;
   for (int p = p0; p < p1; p += 64 * kLoads) {
-    uint32_t w[kLoads][4];
+    float v[kLoads][kEach], here = -INFINITY;
+    unpack(p, w, v);
+    if (p + 64 * kLoads < p1) load(p + 64 * kLoads, w);
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int q = p + 64 * i + lane;
-      const uint4 v = *reinterpret_cast<const uint4*>(body + 16ll * min(q, p1 - 1));
-      w[i][0] = v.x;
-      w[i][1] = v.y;
-      w[i][2] = v.z;
-      w[i][3] = v.w;
-    }
-    float v[kLoads][kEach], most = -INFINITY;
+    for (int i = 0; i < kLoads; ++i)
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const bool in = p + 64 * i + lane < p1;
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        v[i][e] = in ? X::at(w[i], e) : -INFINITY;
-        most = fmaxf(most, v[i][e]);
-      }
-    }
-    sums.move(fmaxf(sums.m, most));
+      for (int e = 0; e < kEach; ++e) here = fmaxf(here, v[i][e]);
+    sums.move(fmaxf(sums.m, here));
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
 #pragma unroll
       for (int e = 0; e < kEach; ++e) sums.add(v[i][e]);
     if constexpr (TOP) {
-      if (first) {  // at least `top` logits reach the top-th largest maximum, where that many lanes have one
-        const uint32_t bound = nth_of(p + lane < p1 ? ordered(most) : 0, a.top);
-        if (bound) {
-          const Key below = (static_cast<Key>(bound) << 32) - 1;
-          list.last = below > list.last ? below : list.last;
-        }
-        first = false;
-      }
-      const float least = value_of(static_cast<uint32_t>(list.last >> 32));
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int q = p + 64 * i + lane;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e)
-          if (__ballot(list.last == 0 || !(v[i][e] < least))) list.take(key_of(v[i][e], head + q * kEach + e), q < p1, a.top);
+      in_group = fmaxf(in_group, here);
+      if (--left == 0 || p + 64 * kLoads >= p1) {
+        // a maximum passes NaN by; the sum does not
+        sh.group[group][threadIdx.x] = static_cast<uint16_t>(sums.s != sums.s ? 0xFFFF : ordered(in_group) >> 16);
+        most = fmaxf(most, in_group);
+        in_group = -INFINITY;
+        left = stride;
+        ++group;
       }
     }
   }
-  const Sums all = over_workgroup(sh, sums, list.mine, TOP ? a.top : 0);
+  if constexpr (TOP) {
+    const auto at_of = [&](int p, int i, int e) { return head + (p + 64 * i + lane) * kEach + e; };
+    const bool any = p0 + lane < p1;
+    list.last = bound_of(sh, any ? ordered(most) : 0, a.top, [&]() {  // where the lane has its maximum first
+      int at = a.vocab - 1;
+#pragma unroll 1
+      for (int p = p0; __ballot(any && at == a.vocab - 1) && p < p1; p += 64 * kLoads) {
+        load(p, w);
+        float v[kLoads][kEach];
+        unpack(p, w, v);
+#pragma unroll
+        for (int i = kLoads; i-- > 0;)
+#pragma unroll
+          for (int e = kEach; e-- > 0;) at = v[i][e] == most && p + 64 * i + lane < p1 ? min(at, at_of(p, i, e)) : at;
+      }
+      return at;
+    });
+    list.take(key_of(edge_v, edge_at), edge);
+    uint32_t groups = 0;
+    for (int k = 0; k < group; ++k) groups |= static_cast<uint32_t>(sh.group[k][threadIdx.x] >= static_cast<uint32_t>((list.last + 1) >> 48)) << k;
+#pragma unroll 1
+    for (uint32_t all = any ? groups : 0; __ballot(all != 0); all &= all - 1) {
+      const int k = all ? __builtin_ctz(all) : 0;
+#pragma unroll 1
+      for (int j = 0; j < stride; ++j) {  // each lane its own group
+        const int p = p0 + (k * stride + j) * 64 * kLoads;
+        load(p, w);
+        float v[kLoads][kEach];
+        unpack(p, w, v);
+        // a bit for each logit whose key may be the bound's next or above: of those equal to its logit only the places up to its own
+        const Key next = list.last + 1;
+        const float least = value_of(static_cast<uint32_t>(next >> 32));  // NaN at either end: all may be
+        const int upto = static_cast<int>(min(~static_cast<uint32_t>(next), 0x7FFFFFFEu)) + 1;
+        uint32_t may = 0;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          uint32_t up = 0, eq = 0;
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) {
+            up |= static_cast<uint32_t>(!(v[i][e] <= least)) << e;
+            eq |= static_cast<uint32_t>(v[i][e] == least) << e;
+          }
+          const bool in = all != 0 && p + 64 * i + lane < p1;
+          may |= in ? (up | (eq & ((1u << iclamp(upto - at_of(p, i, 0), 0, kEach)) - 1))) << (i * kEach) : 0;
+        }
+#pragma unroll 1
+        while (__ballot(may != 0)) {
+          list.cut();
+#pragma unroll
+          for (int u = 0; u < kAtOnce; ++u) {
+            const int b = may ? __builtin_ctz(may) : 0, at = at_of(min(p + 64 * (b / kEach), p1 - 1 - lane), 0, 0) + b % kEach;
+            const float again = X::one(x + static_cast<int64_t>(may ? at : 0) * kSize);
+            list.take(key_of(again, at), may != 0);
+            may &= may - 1;
+          }
+        }
+      }
+    }
+  }
+  const Sums all = over_workgroup(sh, sums, list);
   if (a.parts == 1) {
     answer<X>(a, sh, all, row);
     return;
@@ -268,15 +420,20 @@ __global__ __launch_bounds__(64 * kWaves) void logprobs_join_kernel(LogprobArgs 
     const float4 v = *reinterpret_cast<const float4*>(part_at(a, row, p));
     sums.join({v.x, v.y, v.z});
   }
-  List list;
-  if (a.top)
-    for (int i = 64 * wave; i < a.parts * a.top; i += 64 * kWaves) {
-      const int at = i + lane, k = at / a.parts;  // the parts' largest first
-      const bool in = at < a.parts * a.top;
+  List list{sh.keys[wave]};
+  list.top = a.top;
+  if (a.top) {
+    const int n = a.parts * a.top;
+    for (int base = 0; base < n; base += 64 * kWaves) {
+      const int at = base + threadIdx.x, k = at / a.parts;  // the parts' largest first
+      const bool in = at < n;
       const Key key = in ? reinterpret_cast<const Key*>(part_at(a, row, at - k * a.parts) + 16)[k] : 0;
-      list.take(key, in, a.top);
+      if (base == 0) list.last = bound_of(sh, static_cast<uint32_t>(key >> 32), a.top, [&]() { return static_cast<int>(~static_cast<uint32_t>(key)); });
+      list.cut();
+      list.take(key, in);
     }
-  const Sums all = over_workgroup(sh, sums, list.mine, a.top);
+  }
+  const Sums all = over_workgroup(sh, sums, list);
   answer<X>(a, sh, all, row);
 }
 
@@ -291,11 +448,13 @@ hipError_t go(const LogprobArgs& a, hipStream_t s) {
 
 }  // namespace
 
-// Parts of a row: enough workgroups for the card where there are few rows, 16 KiB of logits each at least.
+// Parts of a row: groups of loads to each wave so many that there are three workgroups to a CU, or a quarter of one where that
+// leaves CUs idle.
 int logprobs_parts(int rows, int vocab, int dtype) {
-  const int64_t bytes = static_cast<int64_t>(vocab) * (dtype == 0 ? 4 : 2);
-  const int64_t most = std::max<int64_t>(1, bytes >> 14), want = std::max(1, 1024 / rows);
-  return static_cast<int>(std::min(most, want));
+  const int pieces = std::max(1, vocab / (dtype == 0 ? 4 : 8)), groups = ceil_div(pieces, 64 * kLoads * kWaves);
+  const int64_t all = static_cast<int64_t>(rows) * groups;
+  if (all <= 64) return ceil_div(pieces, 64 * kWaves);
+  return ceil_div(groups, static_cast<int>(std::min<int64_t>((all + 767) / 768, groups)));
 }
 
 hipError_t launch_logprobs(const LogprobArgs& a, hipStream_t s) {

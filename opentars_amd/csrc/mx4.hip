@@ -298,9 +298,9 @@ constexpr int kGroup = 8;  // tiles of x that take turns over a tile of w
 template <int FM, int FN, int WN, bool TAIL>
 __global__ __launch_bounds__(128 * WN, 4 / WN + (WN == 4)) void mx4_tile_kernel(Mx4GemmArgs a, int mt, int nt) {
   constexpr int kWaves = 2 * WN, BM = 32 * FM, BN = 16 * FN * WN, L = (BM + BN) / 16 / kWaves, XL = BM / 16 / kWaves;
-  constexpr int SL = (BM + BN) / 64 / kWaves;
-  static_assert(BM % (16 * kWaves) == 0 && BN % (16 * kWaves) == 0 && (BM + BN) % (64 * kWaves) == 0 && BM % 64 == 0 && FN % 4 == 0, "whole loads");
-  constexpr int kStage = (BM + BN) * 64, kScales = (BM + BN) * 16;
+  constexpr int SL = (BM + BN + 64 * kWaves - 1) / (64 * kWaves);
+  static_assert(BM % (16 * kWaves) == 0 && BN % (16 * kWaves) == 0 && BM % 64 == 0 && FN % 4 == 0, "whole loads");
+  constexpr int kStage = (BM + BN) * 64, kScales = SL * kWaves * 1024;
   constexpr int kTwice = 1, kOnce = FM - kTwice, kSlots = FM * FN;
   __shared__ __align__(1024) char lds[3 * kStage + 2 * kScales];  // the ring, scales as they come, scales transposed
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(128 * WN, 4 / WN + (WN == 4)) void mx4_tile_kernel(
   }
 #pragma unroll
   for (int u = 0; u < SL; ++u) {
-    const int row = 64 * (wave + kWaves * u) + lane, mine = row < BM ? row : w_scale_row(row - BM);
+    const int row = min(64 * (wave + kWaves * u) + lane, BM + BN - 1), mine = row < BM ? row : w_scale_row(row - BM);
     soff[u] = row < BM ? min(mine, a.M - 1 - m0) * static_cast<uint32_t>(a.x.ld_scales) : min(mine, a.N - 1 - n0) * static_cast<uint32_t>(a.w.ld_scales);
   }
   const uint32_t ring = lds_addr(lds);
