@@ -824,7 +824,7 @@ int check_mx4_product(const tars_mx4* w, const float* bias, void* y, int64_t ldy
 
 // The workspace: x's codes and scales where a launch of its own makes them, then the product's.
 int64_t mx4_need(int32_t M, int32_t N, int32_t K, bool quantises) {
-  return (quantises && !tars::mx4_quantises(M) ? M * (K / 2 + mx_scale_row(K)) : 0) + tars::mx4_parts_bytes(M, N, K);
+  return (quantises && !tars::mx4_quantises(M, N, K) ? M * (K / 2 + mx_scale_row(K)) : 0) + tars::mx4_parts_bytes(M, N, K);
 }
 bool mx4_sizes_ok(int32_t M, int32_t N, int32_t K) {
   return M >= 1 && N >= 1 && K >= 32 && K % 32 == 0 && M <= kMaxMxX && N <= kMaxMxW && K <= kMaxMxK;
@@ -1220,7 +1220,7 @@ int tars_quant_gemm_mx4(const void* x, int64_t ldx, int32_t dtype, int32_t M, co
   if (int rc = check_mx4_product(w, bias, y, ldy, out, work, work_bytes, need, in, a)) return rc;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   a.work = static_cast<char*>(work);
-  if (!tars::mx4_quantises(M)) {  // into the workspace's first bytes
+  if (!tars::mx4_quantises(M, a.N, w->k)) {  // into the workspace's first bytes
     const int64_t values = static_cast<int64_t>(M) * (w->k / 2), pad = mx_scale_row(w->k);
     a.x = {a.work, reinterpret_cast<const uint8_t*>(a.work + values), w->k / 2, pad};
     const tars::Mx4QuantArgs qa{a.rows, ldx, a.work, reinterpret_cast<uint8_t*>(a.work + values), w->k / 2, pad, M, w->k,

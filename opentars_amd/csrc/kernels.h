@@ -479,7 +479,7 @@ struct Mx4Matrix {
 struct Mx4GemmArgs {
   Mx4Matrix w;            // [N, K]
   Mx4Matrix x;            // [M, K], with dtype -1
-  const char* rows;       // [M, K] of dtype at ld_rows bytes, quantised by the kernel: mx4_quantises(M)
+  const char* rows;       // [M, K] of dtype at ld_rows bytes, quantised by the kernel: mx4_quantises()
   int64_t ld_rows;
   const float* bias;      // fp32 [N], or null
   char* y;                // [M, N] at ldy bytes, of type out
@@ -489,7 +489,8 @@ struct Mx4GemmArgs {
   int wide_rows;          // y's rows, 2^23 bytes apart at most, and bias lie on 16 bytes
   char* work;             // mx4_parts_bytes()
 };
-bool mx4_quantises(int M);
+// Whether the product quantises its rows itself.
+bool mx4_quantises(int M, int N, int K);
 // Scratch of a product that is split over K between workgroups.
 int64_t mx4_parts_bytes(int M, int N, int K);
 hipError_t launch_mx4_gemm(const Mx4GemmArgs& a, hipStream_t s);

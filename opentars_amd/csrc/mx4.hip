@@ -117,9 +117,8 @@ __global__ __launch_bounds__(256) void mx4_quant_kernel(Mx4QuantArgs a) {
   if (at % 4 == 0) a.scales[row * a.ld_scales + block] = static_cast<uint8_t>(byte);
 }
 
-// ---- the second operand of a product: a matrix in 4 bits, or one that is quantised in the registers
+// ---- a block of x as a product's operand: in 4 bits, or quantised here
 struct Codes {};
-
 struct Operand {
   uint4 v;
   int s;
@@ -175,106 +174,162 @@ __device__ __forceinline__ void store_outputs(const Mx4GemmArgs& a, int m, int n
   }
 }
 
-// ---- few rows: a wave takes NT tiles of 16 weight rows and MT of 16 rows, over its share of K, straight from memory; the KW
-// waves that share the tiles add theirs in LDS, in order.
-constexpr int kFewWaves = 8;
+// The swap of the four 16-byte blocks of a row's 64 bytes in LDS, such that the reads of a fragment's 16 rows, row r by lane r, meet
+// every bank once: the hardware takes 16 lanes of a 16-byte read together, lanes 0-3, 12-15 and 20-27 of each 32, and the rest.
+__device__ __forceinline__ int swap_of(int r) { return -(r >> 2) & 3; }
 
-template <class X, int MT, int NT>
-__global__ __launch_bounds__(64 * kFewWaves) void mx4_few_kernel(Mx4GemmArgs a, int kw) {
-  __shared__ v4f part[kFewWaves][MT * NT][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-  const int share = wave % kw, group = blockIdx.x * (kFewWaves / kw) + wave / kw;
-  const int n0 = group * 16 * NT, m0 = blockIdx.y * 16 * MT;
-  const int blocks = a.K / 32, steps = ceil_div(blocks, 4);
-  v4f c[MT][NT];
+// ---- few rows: the workgroup keeps all of x in LDS, in 4 bits, its waves read w's rows once
+//
+// A wave takes tiles of 16 rows of w over its share of K; the kw waves that share a tile add theirs in LDS, in order. w comes by
+// direct loads into the wave's own two slots of four steps of 128 k: lanes that are neighbours then read neighbouring bytes of a
+// row (an operand's lanes are rows apart: read straight into it, 83 MB took 25 us, the loads' addresses what bounded it). One slot is
+// loaded while the other is multiplied, the first one while x is quantised.
+constexpr int kFewWaves = 8, kFewSteps = 4, kFewSlot = kFewSteps * 1024 + 256;
+
+template <class X, int MT>
+__global__ __launch_bounds__(64 * kFewWaves) void mx4_few_kernel(Mx4GemmArgs a, int kw, int per) {
+  extern __shared__ __align__(1024) char few_lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+  const int share = wave % kw, tiles = ceil_div(a.N, 16), blocks = a.K / 32, steps = ceil_div(blocks, 4);
+  const int first = min(steps, share * per), end = min(steps, first + per), loads = min(per, kFewSteps);
+  char* const slots = few_lds + 2 * kFewSlot * wave;
+  char* const xv = few_lds + 2 * kFewSlot * kFewWaves;                  // block b of row m: 16 bytes at b M + m
+  uint8_t* const xs = reinterpret_cast<uint8_t*>(xv) + 16 * blocks * a.M;
+  v4f* const part = reinterpret_cast<v4f*>(xv + (17 * blocks * a.M + 15) / 16 * 16);
+  const int stride = gridDim.x * (kFewWaves / kw);
+  int tile = blockIdx.x * (kFewWaves / kw) + wave / kw;
+
+  const int load_row = lane >> 2, load_chunk = (lane & 3) ^ swap_of(load_row);
+  const auto issue = [&](int tile, int s0, int slot) __attribute__((always_inline)) {
+    const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_addr(slots) + kFewSlot * slot);
+    const char* v = a.w.values + min(16 * tile + load_row, a.N - 1) * a.w.ld_values;
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) c[i][j] = v4f{0, 0, 0, 0};
-  if (n0 < a.N) {
-    const char* wv[NT];
-    const uint8_t* ws[NT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int64_t n = min(n0 + 16 * j + r, a.N - 1);
-      wv[j] = a.w.values + n * a.w.ld_values;
-      ws[j] = a.w.scales + n * a.w.ld_scales;
-    }
-    const int per = ceil_div(steps, kw), s1 = min(steps, (share + 1) * per);
-    for (int s = share * per; s < s1; ++s) {
-      const int block = 4 * s + g;
-      const bool in = block < blocks;
-      const int at = in ? block : 0;
-      Operand w[NT], x[MT];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        w[j].v = *reinterpret_cast<const uint4*>(wv[j] + 16 * at);
-        w[j].s = in ? ws[j][at] : 0;
+    for (int u = 0; u < kFewSteps; ++u)
+      if (u < loads) {
+        const int block = 4 * (s0 + u) + load_chunk;
+        ring_load16(v + 16 * (block < blocks ? block : 0), dst + 1024 * u);
       }
+    if (lane < 16) ring_load16(a.w.scales + min(16 * tile + lane, a.N - 1) * a.w.ld_scales + (s0 & ~3) * 4, dst + 1024 * kFewSteps);
+  };
+  const auto wait_loads = [&](bool behind) __attribute__((always_inline)) {  // for a slot, with another's loads behind it
+    if (!behind) wait_vmcnt<0>();
+    else if (loads == 1) wait_vmcnt<2>();
+    else if (loads == 2) wait_vmcnt<3>();
+    else wait_vmcnt<5>();
+    asm volatile("" ::: "memory");
+  };
+  const auto barrier = [&]() __attribute__((always_inline)) {
+    asm volatile("" ::: "memory");
+    wait_lgkm0();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  if (tile < tiles && first < end) issue(tile, first, 0);
+  for (int i = threadIdx.x; i < blocks * a.M; i += 64 * kFewWaves) {
+    const int m = i / blocks, b = i - m * blocks;
+    const Operand o = load_x<X>(a, m, b);
+    *reinterpret_cast<uint4*>(xv + 16 * (b * a.M + m)) = o.v;
+    xs[b * a.M + m] = static_cast<uint8_t>(o.s);
+  }
+  barrier();
+  int row[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) row[i] = min(16 * i + r, a.M - 1);
+  const int value_at = 64 * r + 16 * (g ^ swap_of(r)), scale_at = 1024 * kFewSteps + 16 * r + g;
+  int slot = 0;
+  for (int base = blockIdx.x * (kFewWaves / kw); base < tiles; base += stride, tile += stride) {  // the same for every wave
+    v4f c[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) c[i] = v4f{0, 0, 0, 0};
+    if (tile < tiles)
+      for (int s0 = first; s0 < end; s0 += kFewSteps) {
+        const bool last = s0 + kFewSteps >= end, more = !last || tile + stride < tiles;
+        wait_lgkm0();  // the other slot has been read
+        if (more) issue(last ? tile + stride : tile, last ? first : s0 + kFewSteps, slot ^ 1);
+        wait_loads(more);
+        const char* from = slots + kFewSlot * slot;
+#pragma unroll
+        for (int u = 0; u < kFewSteps; ++u)
+          if (u < loads) {
+            const int block = 4 * (s0 + u) + g;
+            // behind K or the wave's share: any block, with scales whose products are below fp32's smallest number
+            const bool in = s0 + u < end && block < blocks;
+            const int at = (in ? block : 0) * a.M;
+            const uint4 v = *reinterpret_cast<const uint4*>(from + value_at + 1024 * u);
+            const int w = from[scale_at + 4 * ((s0 + u) & 3)] & 255, ws = in ? w : 0;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              const uint4 x = *reinterpret_cast<const uint4*>(xv + 16 * (at + row[i]));
+              const int s = in ? xs[at + row[i]] : 0;
+              c[i] = mfma_fp4(v, ws, x, s, c[i]);
+            }
+          }
+        slot ^= 1;
+      }
+    if (kw > 1) {
+      if (share)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) part[(wave * MT + i) * 64 + lane] = c[i];
+      barrier();
+      if (!share)
+        for (int k = 1; k < kw; ++k)
+#pragma unroll
+          for (int i = 0; i < MT; ++i) c[i] += part[((wave + k) * MT + i) * 64 + lane];
+      if (base + stride < tiles) barrier();
+    }
+    if (share == 0 && tile < tiles)
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        const int m = m0 + 16 * i + r;
-        x[i] = {make_uint4(0, 0, 0, 0), 0};
-        if (in && m < a.M) x[i] = load_x<X>(a, m, at);
+        const int m = 16 * i + r, n = 16 * tile + 4 * g;
+        if (m < a.M && n < a.N) store_outputs(a, m, n, c[i]);
       }
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) c[i][j] = mfma_fp4(w[j].v, w[j].s, x[i].v, x[i].s, c[i][j]);
-    }
   }
-  if (kw > 1) {
-    if (share)
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) part[wave][i * NT + j][lane] = c[i][j];
-    __syncthreads();
-    if (share) return;
-    for (int k = 1; k < kw; ++k)
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) c[i][j] += part[wave + k][i * NT + j][lane];
-  }
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int m = m0 + 16 * i + r, n = n0 + 16 * j + 4 * g;
-      if (m < a.M && n < a.N) store_outputs(a, m, n, c[i][j]);
-    }
 }
+
+// Whether x fits a workgroup's LDS beside the slots.
+constexpr int kLds = 160 << 10;
+int64_t few_lds_bytes(int M, int K, int kw) {
+  return 2 * kFewSlot * kFewWaves + (17ll * (K / 32) * M + 15) / 16 * 16 + (kw > 1 ? kFewWaves * 1024 * ceil_div(M, 16) : 0);
+}
+int few_split(int M, int N, int K) {
+  const int tiles = ceil_div(N, 16), steps = ceil_div(K, 128);
+  int kw = 1;
+  while (kw < kFewWaves && tiles * kw < (M <= 16 ? 2048 : 1024) && 2 * kw <= steps) kw *= 2;
+  return kw;
+}
+bool few_fits(int M, int N, int K) { return M <= 64 && few_lds_bytes(M, K, few_split(M, N, K)) <= kLds; }
 
 template <class X>
 hipError_t few(const Mx4GemmArgs& a, hipStream_t s) {
-  const int tiles = ceil_div(a.N, 16), steps = ceil_div(a.K, 128);
-  int kw = 1;
-  while (kw < kFewWaves && tiles * kw < 2048 && 2 * kw <= steps) kw *= 2;
-  const dim3 block(64 * kFewWaves);
-  const int groups = ceil_div(tiles, kFewWaves / kw);
-  if (a.M <= 16) hipLaunchKernelGGL((mx4_few_kernel<X, 1, 1>), dim3(groups, 1), block, 0, s, a, kw);
-  else if (a.M <= 32) hipLaunchKernelGGL((mx4_few_kernel<X, 2, 1>), dim3(groups, 1), block, 0, s, a, kw);
-  else hipLaunchKernelGGL((mx4_few_kernel<X, 4, 1>), dim3(groups, ceil_div(a.M, 64)), block, 0, s, a, kw);
+  const int kw = few_split(a.M, a.N, a.K), groups = ceil_div(ceil_div(a.N, 16), kFewWaves / kw), share = ceil_div(ceil_div(a.K, 128), kw);
+  const int per = share <= 2 ? share : ceil_div(share, kFewSteps) * kFewSteps;  // no slot's steps in two 16-byte pieces of scales
+  const int lds = static_cast<int>(few_lds_bytes(a.M, a.K, kw));
+  const dim3 grid(std::min(groups, 256 * (kLds / lds))), block(64 * kFewWaves);
+  if (a.M <= 16) hipLaunchKernelGGL((mx4_few_kernel<X, 1>), grid, block, lds, s, a, kw, per);
+  else if (a.M <= 32) hipLaunchKernelGGL((mx4_few_kernel<X, 2>), grid, block, lds, s, a, kw, per);
+  else if (a.M <= 48) hipLaunchKernelGGL((mx4_few_kernel<X, 3>), grid, block, lds, s, a, kw, per);
+  else hipLaunchKernelGGL((mx4_few_kernel<X, 4>), grid, block, lds, s, a, kw, per);
   return hipGetLastError();
 }
 
 // ---- many rows: a workgroup of 2 x WN waves takes 32 FM rows of x and 16 FN WN of w, a wave 16 FM and 16 FN
 //
-// Stages of 128 k pass through a ring of three in LDS, by direct loads: a row's 64 bytes at a time, its four 16-byte blocks
-// permuted so that a fragment's reads meet every bank once (the hardware takes 16 lanes of a 16-byte read together: lanes 0-3,
-// 12-15 and 20-27 of each 32, and the rest). A stage's fragments are read, and a later stage loaded, between the products of the
-// one before, an instruction or two behind each product, which is as many as a product hides; so nothing waits for LDS behind a
-// barrier. x's fragments but the last kTwice are read over the ones that were just multiplied; those and w's have two places,
-// so that the last read of a stage is well before its barrier.
+// Pairs of stages of 128 k pass through a ring of D pairs in LDS, by direct loads: a row's 128 bytes at a time, a cache line, its
+// eight 16-byte blocks swapped so that a fragment's reads meet every bank once. (Stages of 64 bytes a row came twice from L2.) A
+// stage's fragments are read, and a later pair loaded, between the products of the one before, an instruction or two behind each
+// product, which is as many as a product hides; so nothing waits for LDS behind a barrier, of which there is one to a pair. x's
+// fragments but the last kTwice are read over the ones that were just multiplied; those and w's have two places, so that the last
+// read of a stage is well before its barrier.
 //
-// Scales come for four stages at a time: a row's 16 bytes, transposed as 4 x 4 on their way, so that a lane's dword holds the
-// four stages' scales of its block, of which the product's operand selects the byte.
+// Scales come for two pairs at a time: a row's 16 bytes, transposed as 4 x 4 on their way, so that a lane's dword holds the four
+// stages' scales of its block, of which the product's operand selects the byte.
 //
 // Fragment j of w holds rows 64 (j / 4) + 16 (r / 4) + 4 (j % 4) + r % 4: the outputs of a lane's four neighbouring fragments
 // are then 16 neighbours of a row.
-__device__ __forceinline__ int x_swap(int row) { return -(row >> 2) & 3; }
-__device__ __forceinline__ int w_swap(int row) { return -(row >> 4) & 3; }
+//
+// The swap of a row's blocks: row r of a fragment, by lane r (and as swap_of, for rows of 128 bytes).
+__device__ __forceinline__ int x_swap(int row) { return row >> 1 & 7; }
+__device__ __forceinline__ int w_swap(int row) { return (row >> 3 & 6) | (row >> 1 & 1); }
 // The row of w whose scales lie in place `at`: a fragment's 16 rows in neighbouring ones.
 __device__ __forceinline__ int w_scale_row(int at) { return (at & ~63) | (at >> 2 & 3) << 4 | (at >> 4 & 3) << 2 | (at & 3); }
 
@@ -295,21 +350,21 @@ __device__ __forceinline__ v4f mfma_fp4_scale(uint4 a, int sa, uint4 b, int sb, 
 
 constexpr int kGroup = 8;  // tiles of x that take turns over a tile of w
 
-template <int FM, int FN, int WN, bool TAIL>
-__global__ __launch_bounds__(128 * WN, 4 / WN + (WN == 4)) void mx4_tile_kernel(Mx4GemmArgs a, int mt, int nt) {
-  constexpr int kWaves = 2 * WN, BM = 32 * FM, BN = 16 * FN * WN, L = (BM + BN) / 16 / kWaves, XL = BM / 16 / kWaves;
+template <int FM, int FN, int WN, int D, bool TAIL>
+__global__ __launch_bounds__(128 * WN, 2) void mx4_tile_kernel(Mx4GemmArgs a, int mt, int nt) {
+  constexpr int kWaves = 2 * WN, BM = 32 * FM, BN = 16 * FN * WN, L = (BM + BN) / 8 / kWaves, XL = BM / 8 / kWaves;
   constexpr int SL = (BM + BN + 64 * kWaves - 1) / (64 * kWaves);
-  static_assert(BM % (16 * kWaves) == 0 && BN % (16 * kWaves) == 0 && BM % 64 == 0 && FN % 4 == 0, "whole loads");
-  constexpr int kStage = (BM + BN) * 64, kScales = SL * kWaves * 1024;
+  static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0 && BM % 64 == 0 && FN % 4 == 0 && D >= 2 && D <= 4, "whole loads; scales as far ahead as the ring");
+  constexpr int kPair = (BM + BN) * 128, kScales = SL * kWaves * 1024;
   constexpr int kTwice = 1, kOnce = FM - kTwice, kSlots = FM * FN;
-  __shared__ __align__(1024) char lds[3 * kStage + 2 * kScales];  // the ring, scales as they come, scales transposed
+  __shared__ __align__(1024) char lds[D * kPair + 3 * kScales];  // the ring, scales transposed, scales as they come
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
   const int wm = wave & 1, wn = wave >> 1;
   // consecutive tiles of an XCD: kGroup tiles of x by all of w's
   const int id = xcd_block(blockIdx.x, gridDim.x), per = kGroup * nt, first = id / per * kGroup, deep = min(kGroup, mt - first);
   const int m0 = (first + id % per % deep) * BM, n0 = id % per / deep * BN;
   // stages by fours; what is behind K counts for nothing
-  const int blocks = a.K / 32, pieces = ceil_div(blocks, 16), stages = 4 * pieces;
+  const int blocks = a.K / 32, pieces = ceil_div(blocks, 16), pairs = 2 * pieces;
 
   const char* const xb = a.x.values + m0 * a.x.ld_values;
   const char* const wb = a.w.values + n0 * a.w.ld_values;
@@ -318,9 +373,9 @@ __global__ __launch_bounds__(128 * WN, 4 / WN + (WN == 4)) void mx4_tile_kernel(
   uint32_t off[L], soff[SL];
   int chunk[L];
 #pragma unroll
-  for (int u = 0; u < L; ++u) {  // 16 rows to a load, x's first
-    const int row = 16 * (wave + kWaves * u) + lane / 4, mine = u < XL ? row : row - BM;
-    chunk[u] = (lane & 3) ^ (u < XL ? x_swap(mine) : w_swap(mine));
+  for (int u = 0; u < L; ++u) {  // 8 rows to a load, x's first
+    const int row = 8 * (wave + kWaves * u) + lane / 8, mine = u < XL ? row : row - BM;
+    chunk[u] = (lane & 7) ^ (u < XL ? x_swap(mine) : w_swap(mine));
     off[u] = u < XL ? min(mine, a.M - 1 - m0) * static_cast<uint32_t>(a.x.ld_values) : min(mine, a.N - 1 - n0) * static_cast<uint32_t>(a.w.ld_values);
     if (!TAIL) off[u] += 16 * chunk[u];
   }
@@ -330,28 +385,29 @@ __global__ __launch_bounds__(128 * WN, 4 / WN + (WN == 4)) void mx4_tile_kernel(
     soff[u] = row < BM ? min(mine, a.M - 1 - m0) * static_cast<uint32_t>(a.x.ld_scales) : min(mine, a.N - 1 - n0) * static_cast<uint32_t>(a.w.ld_scales);
   }
   const uint32_t ring = lds_addr(lds);
-  // load u of stage st
-  auto issue_one = [&](int st, uint32_t dst, int u) __attribute__((always_inline)) {
+  // load u of a pair of stages
+  auto issue_one = [&](int pair, uint32_t dst, int u) __attribute__((always_inline)) {
     const char* base = u < XL ? xb : wb;
     if constexpr (TAIL) {  // behind K: the row's first block, whose scales are taken for 0
-      const int block = 4 * st + chunk[u];
+      const int block = 8 * pair + chunk[u];
       ring_load16(base, off[u] + (block < blocks ? 16 * block : 0), dst + 1024 * kWaves * u);
     } else {
-      ring_load16(base + 64 * st, off[u], dst + 1024 * kWaves * u);
+      ring_load16(base + 128 * pair, off[u], dst + 1024 * kWaves * u);
     }
   };
-  auto stage_at = [&](int slot) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(ring + kStage * slot + 1024 * wave); };
+  auto pair_at = [&](int slot) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(ring + kPair * slot + 1024 * wave); };
   auto issue_scales = [&](int piece) __attribute__((always_inline)) {
-    const uint32_t dst = __builtin_amdgcn_readfirstlane(ring + 3 * kStage + 1024 * wave);
+    const int from = min(piece, pieces - 1);
+    const uint32_t dst = __builtin_amdgcn_readfirstlane(ring + D * kPair + kScales * (1 + (piece & 1)) + 1024 * wave);
 #pragma unroll
-    for (int u = 0; u < SL; ++u) ring_load16((64 * (wave + kWaves * u) < BM ? xsb : wsb) + 16 * piece, soff[u], dst + 1024 * kWaves * u);
+    for (int u = 0; u < SL; ++u) ring_load16((64 * (wave + kWaves * u) < BM ? xsb : wsb) + 16 * from, soff[u], dst + 1024 * kWaves * u);
   };
   // a thread's own loads of scales
-  char* const raw = lds + 3 * kStage + 16 * threadIdx.x;
+  char* const done = lds + D * kPair + 16 * threadIdx.x;
   auto transpose_scales = [&](int piece) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < SL; ++u) {
-      uint4 v = *reinterpret_cast<const uint4*>(raw + 1024 * kWaves * u);
+      uint4 v = *reinterpret_cast<const uint4*>(done + kScales * (1 + (piece & 1)) + 1024 * kWaves * u);
       if constexpr (TAIL) {
         uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -361,23 +417,24 @@ __global__ __launch_bounds__(128 * WN, 4 / WN + (WN == 4)) void mx4_tile_kernel(
         }
         v = make_uint4(w[0], w[1], w[2], w[3]);
       }
-      *reinterpret_cast<uint4*>(raw + kScales + 1024 * kWaves * u) = transposed(v);
+      *reinterpret_cast<uint4*>(done + 1024 * kWaves * u) = transposed(v);
     }
   };
   // the wave's fragments in a stage and their scales
-  const char* const x_at = lds + 64 * (wm * (BM / 2) + r) + 16 * (g ^ x_swap(r));
-  const char* const w_at = lds + 64 * (BM + wn * (16 * FN) + 16 * (r / 4) + r % 4) + 16 * (g ^ w_swap(16 * (r / 4)));
-  const char* const xs_at = lds + 3 * kStage + kScales + 16 * (wm * (BM / 2) + r) + 4 * g;
-  const char* const ws_at = lds + 3 * kStage + kScales + 16 * (BM + wn * (16 * FN) + r) + 4 * g;
+  // (of the pair's first stage; the second's are 64 bytes up or down)
+  const uint32_t x_at = 128 * (wm * (BM / 2) + r) + 16 * (g ^ x_swap(r));
+  const uint32_t w_at = 128 * (BM + wn * (16 * FN) + 16 * (r / 4) + r % 4) + 16 * (g ^ w_swap(16 * (r / 4) + r % 4));
+  const char* const xs_at = lds + D * kPair + 16 * (wm * (BM / 2) + r) + 4 * g;
+  const char* const ws_at = lds + D * kPair + 16 * (BM + wn * (16 * FN) + r) + 4 * g;
   struct Fragments {
     uint4 w[FN], x[kTwice];
   };
   uint4 x[kOnce];
   int xs[FM], ws[FN];
-  auto read_w = [&](int at, int j) __attribute__((always_inline)) {
-    return *reinterpret_cast<const uint4*>(w_at + at + 64 * (64 * (j / 4) + 4 * (j % 4)));
+  auto read_w = [&](uint32_t at, int j) __attribute__((always_inline)) {
+    return *reinterpret_cast<const uint4*>(lds + at + 128 * (64 * (j / 4) + 4 * (j % 4)));
   };
-  auto read_x = [&](int at, int i) __attribute__((always_inline)) { return *reinterpret_cast<const uint4*>(x_at + at + 1024 * i); };
+  auto read_x = [&](uint32_t at, int i) __attribute__((always_inline)) { return *reinterpret_cast<const uint4*>(lds + at + 2048 * i); };
   auto read_xs = [&](int i) __attribute__((always_inline)) { return *reinterpret_cast<const int*>(xs_at + 256 * i); };
   auto read_ws = [&](int j) __attribute__((always_inline)) { return *reinterpret_cast<const int*>(ws_at + 256 * j); };
   v4f c[FM][FN];
@@ -403,50 +460,53 @@ __global__ __launch_bounds__(128 * WN, 4 / WN + (WN == 4)) void mx4_tile_kernel(
 
   issue_scales(0);
 #pragma unroll
-  for (int st = 0; st < 3; ++st)
+  for (int d = 0; d < D; ++d) {
 #pragma unroll
-    for (int u = 0; u < L; ++u) issue_one(st, stage_at(st), u);
-  wait_vmcnt<L>();
+    for (int u = 0; u < L; ++u) issue_one(min(d, pairs - 1), pair_at(d), u);
+    if (d == 0) issue_scales(1);
+  }
+  wait_vmcnt<(D - 1) * L>();
   asm volatile("" ::: "memory");
   transpose_scales(0);
   wait_lgkm0();
   barrier();
   Fragments f0, f1;
 #pragma unroll
-  for (int j = 0; j < FN; ++j) f0.w[j] = read_w(0, j);
+  for (int j = 0; j < FN; ++j) f0.w[j] = read_w(w_at, j);
 #pragma unroll
-  for (int i = 0; i < FM; ++i) (i < kOnce ? x[i] : f0.x[i - kOnce]) = read_x(0, i);
+  for (int i = 0; i < FM; ++i) (i < kOnce ? x[i] : f0.x[i - kOnce]) = read_x(x_at, i);
 #pragma unroll
   for (int i = 0; i < FM; ++i) xs[i] = read_xs(i);
 #pragma unroll
   for (int j = 0; j < FN; ++j) ws[j] = read_ws(j);
   wait_lgkm0();
   barrier();
-  int slot = 0;  // of stage st
+  int slot = 0;  // of stage st's pair
   // Multiplies stage st's fragments, st % 4 = S, and reads the next one's (behind the last stage: of whatever is there, not used).
   auto step = [&](auto s_, int st, Fragments& now, Fragments& next) __attribute__((always_inline)) {
     constexpr int S = decltype(s_)::value;
-    const int after = slot + 1 == 3 ? 0 : slot + 1, at = kStage * after;
-    // the loads of the stage after the next two, or of the last again: their number does not change
-    const int ahead = min(st + 3, stages - 1);
-    const uint32_t dst = stage_at(slot);
-    if constexpr (S == 0) issue_scales(min((st >> 2) + 1, pieces - 1));
+    constexpr bool second = S & 1;  // the pair's fragments are all read: the pair that is a ring ahead, or the last again, takes its slot
+    const int after = !second ? slot : slot + 1 == D ? 0 : slot + 1;
+    const uint32_t xa = kPair * after + (second ? x_at : x_at ^ 64), wa = kPair * after + (second ? w_at : w_at ^ 64);
+    const int ahead = min((st >> 1) + D, pairs - 1);
+    const uint32_t dst = pair_at(slot);
+    if constexpr (S == 1) issue_scales((st >> 2) + 2);
     issue_fence();
     each<kSlots>([&](auto t_) __attribute__((always_inline)) {
       constexpr int t = decltype(t_)::value, i = t / FN, j = t % FN;
       c[i][j] = mfma_fp4_scale<S>(now.w[j], ws[j], i < kOnce ? x[i < kOnce ? i : 0] : now.x[i < kOnce ? 0 : i - kOnce], xs[i], c[i][j]);
       each<L>([&](auto u) __attribute__((always_inline)) {
-        if constexpr (decltype(u)::value * kSlots / L == t) issue_one(ahead, dst, decltype(u)::value);
+        if constexpr (second && decltype(u)::value * kSlots / L == t) issue_one(ahead, dst, decltype(u)::value);
       });
-      if constexpr (t % FN == 0 && t > 0 && t / FN <= kOnce) x[t / FN - 1] = read_x(at, t / FN - 1);
+      if constexpr (t % FN == 0 && t > 0 && t / FN <= kOnce) x[t / FN - 1] = read_x(xa, t / FN - 1);
       each<FN + kTwice>([&](auto k_) __attribute__((always_inline)) {
         constexpr int k = decltype(k_)::value;
         if constexpr (k * (kOnce * FN) / (FN + kTwice) + 1 == t) {
-          if constexpr (k < FN) next.w[k] = read_w(at, k);
-          else next.x[k - FN] = read_x(at, FM - kTwice + k - FN);
+          if constexpr (k < FN) next.w[k] = read_w(wa, k);
+          else next.x[k - FN] = read_x(xa, FM - kTwice + k - FN);
         }
       });
-      if constexpr (S == 2 && t == 2) transpose_scales(min((st >> 2) + 1, pieces - 1));
+      if constexpr (S == 2 && t == 2) transpose_scales((st >> 2) + 1);
       if constexpr (S == 3) {  // the next four stages' scales, x's over its own
         if constexpr (t % FN == 1 && t > FN) xs[t / FN - 1] = read_xs(t / FN - 1);
       }
@@ -459,8 +519,10 @@ __global__ __launch_bounds__(128 * WN, 4 / WN + (WN == 4)) void mx4_tile_kernel(
     }
     hold(0);
     wait_lgkm0();
-    wait_vmcnt<L>();
-    barrier();
+    if constexpr (!second) {
+      wait_vmcnt<(D - 2) * L>();
+      barrier();
+    }
     slot = after;
   };
   hold(0);
@@ -470,33 +532,38 @@ __global__ __launch_bounds__(128 * WN, 4 / WN + (WN == 4)) void mx4_tile_kernel(
     step(Int<1>{}, st + 1, f1, f0);
     step(Int<2>{}, st + 2, f0, f1);
     step(Int<3>{}, st + 3, f1, f0);
-  } while ((st += 4) < stages);
+  } while ((st += 4) < 2 * pairs);
   wait_vmcnt<0>();  // the ring's last loads, before its room gets another use
   barrier();
 
-  // (the lane again, so that nothing of it is kept over the stages)
-  int thread = threadIdx.x;
-  asm volatile("" : "+v"(thread));
-  const int nw = n0 + wn * (16 * FN), mw = m0 + wm * (BM / 2), col = thread & 15, part = thread >> 4 & 3;
-  if (a.wide_rows && n0 + BN <= a.N) {  // 16 neighbours to a lane, 64 to a row, 32-bit offsets
+  // the lane again where it is wanted, so that nothing of it is kept over the stages
+  const auto thread_again = []() __attribute__((always_inline)) {
+    int t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
+  };
+  const int nw = n0 + wn * (16 * FN), mw = m0 + wm * (BM / 2);
+  if (a.wide_rows && a.N % 8 == 0) {  // 16 neighbours to a lane, 64 to a row, eight of them within N or none; 32-bit offsets
     const auto all = [&](auto out_, auto bias_) __attribute__((always_inline)) {
       constexpr int out = decltype(out_)::value, e = out == 0 ? 4 : 2;
       char* const tile = a.y + mw * a.ldy + static_cast<int64_t>(nw) * e;
       const float* const bias = a.bias + nw;
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
-        const int m = 16 * i + col;
+        const int thread = thread_again(), col = thread & 15, part = thread >> 4 & 3, m = 16 * i + col;
         const uint32_t at = m * static_cast<uint32_t>(a.ldy) + 16 * part * e;
 #pragma unroll
         for (int j = 0; j < FN; j += 2) {
           const int n = 64 * (j / 4) + 4 * (j % 4);
           v4f y = c[i][j], z = c[i][j + 1];
+          const bool in = nw + 16 * part + n < a.N;
           if constexpr (decltype(bias_)::value) {
-            const float4 b = *reinterpret_cast<const float4*>(bias + 16 * part + n), d = *reinterpret_cast<const float4*>(bias + 16 * part + n + 4);
+            const float* at_bias = bias + (in ? 16 * part + n : -nw);
+            const float4 b = *reinterpret_cast<const float4*>(at_bias), d = *reinterpret_cast<const float4*>(at_bias + 4);
             y += v4f{b.x, b.y, b.z, b.w};
             z += v4f{d.x, d.y, d.z, d.w};
           }
-          if (mw + m < a.M) {
+          if (in && mw + m < a.M) {
             if constexpr (out == 0) {
               *reinterpret_cast<v4f*>(tile + (at + 4 * n)) = y;
               *reinterpret_cast<v4f*>(tile + (at + 4 * n + 16)) = z;
@@ -519,18 +586,19 @@ __global__ __launch_bounds__(128 * WN, 4 / WN + (WN == 4)) void mx4_tile_kernel(
     return;
   }
   // the output's edge, or rows that are not aligned: 16 rows at a time through the wave's own part of the ring
-  constexpr int kCols = 16 * FN, kPitch = kCols + 4;
-  static_assert(kWaves * 16 * kPitch * 4 <= 3 * kStage, "a wave's 16 rows fit");
+  constexpr int kCols = 16 * FN, kPitch = kCols + 4, kAtOnce = FM > 4 ? 1 : 8;
+  static_assert(kWaves * 16 * kPitch * 4 <= D * kPair, "a wave's 16 rows fit");
   float* mine = reinterpret_cast<float*>(lds) + wave * 16 * kPitch;
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
+    const int thread = thread_again(), col = thread & 15, part = thread >> 4 & 3;
 #pragma unroll
     for (int j = 0; j < FN; ++j)
       *reinterpret_cast<v4f*>(mine + col * kPitch + 64 * (j / 4) + 16 * part + 4 * (j % 4)) = c[i][j];
     hold(i + 1);
     wait_lgkm0();
     issue_fence();
-#pragma unroll 1
+#pragma unroll kAtOnce
     for (int k = thread & 63; k < 16 * kCols; k += 64) {
       const int m = mw + 16 * i + k / kCols, n = nw + k % kCols;
       if (m < a.M && n < a.N) {
@@ -545,13 +613,32 @@ __global__ __launch_bounds__(128 * WN, 4 / WN + (WN == 4)) void mx4_tile_kernel(
   }
 }
 
-template <int FM, int FN, int WN>
+template <int FM, int FN, int WN, int D>
 hipError_t tiles(const Mx4GemmArgs& a, hipStream_t s) {
   const int mt = ceil_div(a.M, 32 * FM), nt = ceil_div(a.N, 16 * FN * WN);
   const dim3 grid(mt * nt), block(128 * WN);
-  if (a.K % 512) hipLaunchKernelGGL((mx4_tile_kernel<FM, FN, WN, true>), grid, block, 0, s, a, mt, nt);
-  else hipLaunchKernelGGL((mx4_tile_kernel<FM, FN, WN, false>), grid, block, 0, s, a, mt, nt);
+  if (a.K % 512) hipLaunchKernelGGL((mx4_tile_kernel<FM, FN, WN, D, true>), grid, block, 0, s, a, mt, nt);
+  else hipLaunchKernelGGL((mx4_tile_kernel<FM, FN, WN, D, false>), grid, block, 0, s, a, mt, nt);
   return hipGetLastError();
+}
+
+// Tiles of 256 x 256, 128 x 128 or 64 x 128, by what a stage of all of them takes, in ns: the rounds that fill the card, and the
+// last one, which may leave CUs to fewer workgroups. Measured at 8192 x 8192 x 8192 (265, 353 and 464 us) and, a workgroup to a CU or
+// less, at 128 x 4096 x 4096 (23.8, 12.9 and 10.8 us); 2011 x 12288 x 4096 takes 71, 76 and 93 us.
+int tile_choice(int M, int N) {
+  const struct {
+    int m, n, slots, full, one, none;  // workgroups at a time; ns of a stage with all of them, with one to a CU, with few
+  } kinds[] = {{256, 256, 256, 1030, 1030, 650}, {128, 128, 512, 690, 400, 310}, {64, 128, 512, 450, 300, 240}};
+  int64_t best = INT64_MAX;
+  int choice = 0;
+  for (int i = 0; i < 3; ++i) {
+    const auto& k = kinds[i];
+    const int64_t tiles = static_cast<int64_t>(ceil_div(M, k.m)) * ceil_div(N, k.n), left = tiles % k.slots;
+    const int64_t last = left > 256 ? k.full : k.none + (k.one - k.none) * left / 256;
+    const int64_t ns = tiles / k.slots * k.full + (left ? last : 0);
+    if (ns < best) best = ns, choice = i;
+  }
+  return choice;
 }
 
 }  // namespace
@@ -564,18 +651,19 @@ hipError_t launch_mx4_quant(const Mx4QuantArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
-// Rows up to which the product quantises its operand itself.
-constexpr int kFusedRows = 16;
-
-bool mx4_quantises(int M) { return M <= kFusedRows; }
+// Few enough numbers that every workgroup may quantise them for itself, which saves a launch.
+bool mx4_quantises(int M, int N, int K) { return few_fits(M, N, K) && static_cast<int64_t>(M) * K <= 1 << 17; }
 
 int64_t mx4_parts_bytes(int, int, int) { return 0; }
 
 hipError_t launch_mx4_gemm(const Mx4GemmArgs& a, hipStream_t s) {
-  if (a.dtype < 0 && a.M > 64)
-    return static_cast<int64_t>(ceil_div(a.M, 256)) * ceil_div(a.N, 256) >= 200 ? tiles<8, 4, 4>(a, s) : tiles<4, 4, 2>(a, s);
-  if (a.dtype < 0) return few<Codes>(a, s);
-  return a.dtype == 0 ? few<XFp32>(a, s) : a.dtype == 1 ? few<XBf16>(a, s) : few<XFp16>(a, s);
+  if (a.dtype >= 0) return a.dtype == 0 ? few<XFp32>(a, s) : a.dtype == 1 ? few<XBf16>(a, s) : few<XFp16>(a, s);
+  if (few_fits(a.M, a.N, a.K)) return few<Codes>(a, s);
+  switch (tile_choice(a.M, a.N)) {
+    case 0: return tiles<8, 4, 4, 2>(a, s);
+    case 1: return tiles<4, 4, 2, 2>(a, s);
+    default: return tiles<2, 4, 2, 2>(a, s);
+  }
 }
 
 }  // namespace tars
