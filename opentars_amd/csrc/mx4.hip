@@ -348,10 +348,13 @@ __device__ __forceinline__ v4f mfma_fp4_scale(uint4 a, int sa, uint4 b, int sb, 
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, kFp4, kFp4, S, sa, S, sb);
 }
 
+// Columns of a split's sums in the workspace.
+__host__ __device__ __forceinline__ int split_cols(int N) { return (N + 15) / 16 * 16; }
+
 constexpr int kGroup = 8;  // tiles of x that take turns over a tile of w
 
 template <int FM, int FN, int WN, int D, bool TAIL>
-__global__ __launch_bounds__(128 * WN, 2) void mx4_tile_kernel(Mx4GemmArgs a, int mt, int nt) {
+__global__ __launch_bounds__(128 * WN, 2) void mx4_tile_kernel(Mx4GemmArgs a, int mt, int nt, int splits) {
   constexpr int kWaves = 2 * WN, BM = 32 * FM, BN = 16 * FN * WN, L = (BM + BN) / 8 / kWaves, XL = BM / 8 / kWaves;
   constexpr int SL = (BM + BN + 64 * kWaves - 1) / (64 * kWaves);
   static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0 && BM % 64 == 0 && FN % 4 == 0 && D >= 2 && D <= 4, "whole loads; scales as far ahead as the ring");
@@ -361,15 +364,17 @@ __global__ __launch_bounds__(128 * WN, 2) void mx4_tile_kernel(Mx4GemmArgs a, in
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
   const int wm = wave & 1, wn = wave >> 1;
   // consecutive tiles of an XCD: kGroup tiles of x by all of w's
-  const int id = xcd_block(blockIdx.x, gridDim.x), per = kGroup * nt, first = id / per * kGroup, deep = min(kGroup, mt - first);
+  const int number = xcd_block(blockIdx.x, gridDim.x), split = number / (mt * nt), id = number - split * mt * nt;
+  const int per = kGroup * nt, first = id / per * kGroup, deep = min(kGroup, mt - first);
   const int m0 = (first + id % per % deep) * BM, n0 = id % per / deep * BN;
-  // stages by fours; what is behind K counts for nothing
-  const int blocks = a.K / 32, pieces = ceil_div(blocks, 16), pairs = 2 * pieces;
+  // stages by fours, the workgroup's share of them; what is behind K counts for nothing
+  const int all_blocks = a.K / 32, each_split = ceil_div(ceil_div(all_blocks, 16), splits), start = split * each_split;
+  const int blocks = min(all_blocks - 16 * start, 16 * each_split), pieces = ceil_div(blocks, 16), pairs = 2 * pieces;
 
-  const char* const xb = a.x.values + m0 * a.x.ld_values;
-  const char* const wb = a.w.values + n0 * a.w.ld_values;
-  const uint8_t* const xsb = a.x.scales + m0 * a.x.ld_scales;
-  const uint8_t* const wsb = a.w.scales + n0 * a.w.ld_scales;
+  const char* const xb = a.x.values + m0 * a.x.ld_values + 256 * start;
+  const char* const wb = a.w.values + n0 * a.w.ld_values + 256 * start;
+  const uint8_t* const xsb = a.x.scales + m0 * a.x.ld_scales + 16 * start;
+  const uint8_t* const wsb = a.w.scales + n0 * a.w.ld_scales + 16 * start;
   uint32_t off[L], soff[SL];
   int chunk[L];
 #pragma unroll
@@ -543,42 +548,48 @@ __global__ __launch_bounds__(128 * WN, 2) void mx4_tile_kernel(Mx4GemmArgs a, in
     return t;
   };
   const int nw = n0 + wn * (16 * FN), mw = m0 + wm * (BM / 2);
-  if (a.wide_rows && a.N % 8 == 0) {  // 16 neighbours to a lane, 64 to a row, eight of them within N or none; 32-bit offsets
-    const auto all = [&](auto out_, auto bias_) __attribute__((always_inline)) {
-      constexpr int out = decltype(out_)::value, e = out == 0 ? 4 : 2;
-      char* const tile = a.y + mw * a.ldy + static_cast<int64_t>(nw) * e;
-      const float* const bias = a.bias + nw;
+  // 16 neighbours to a lane, 64 to a row, eight of them within `cols` or none; 32-bit offsets
+  const auto store_rows = [&](auto out_, auto bias_, char* y, int64_t ldy, int cols) __attribute__((always_inline)) {
+    constexpr int out = decltype(out_)::value, e = out == 0 ? 4 : 2;
+    char* const tile = y + mw * ldy + static_cast<int64_t>(nw) * e;
+    const float* const bias = a.bias + nw;
 #pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        const int thread = thread_again(), col = thread & 15, part = thread >> 4 & 3, m = 16 * i + col;
-        const uint32_t at = m * static_cast<uint32_t>(a.ldy) + 16 * part * e;
+    for (int i = 0; i < FM; ++i) {
+      const int thread = thread_again(), col = thread & 15, part = thread >> 4 & 3, m = 16 * i + col;
+      const uint32_t at = m * static_cast<uint32_t>(ldy) + 16 * part * e;
 #pragma unroll
-        for (int j = 0; j < FN; j += 2) {
-          const int n = 64 * (j / 4) + 4 * (j % 4);
-          v4f y = c[i][j], z = c[i][j + 1];
-          const bool in = nw + 16 * part + n < a.N;
-          if constexpr (decltype(bias_)::value) {
-            const float* at_bias = bias + (in ? 16 * part + n : -nw);
-            const float4 b = *reinterpret_cast<const float4*>(at_bias), d = *reinterpret_cast<const float4*>(at_bias + 4);
-            y += v4f{b.x, b.y, b.z, b.w};
-            z += v4f{d.x, d.y, d.z, d.w};
-          }
-          if (in && mw + m < a.M) {
-            if constexpr (out == 0) {
-              *reinterpret_cast<v4f*>(tile + (at + 4 * n)) = y;
-              *reinterpret_cast<v4f*>(tile + (at + 4 * n + 16)) = z;
-            } else {
-              *reinterpret_cast<uint4*>(tile + (at + 2 * n)) = make_uint4(pair(out, y[0], y[1]), pair(out, y[2], y[3]), pair(out, z[0], z[1]), pair(out, z[2], z[3]));
-            }
+      for (int j = 0; j < FN; j += 2) {
+        const int n = 64 * (j / 4) + 4 * (j % 4);
+        v4f v = c[i][j], z = c[i][j + 1];
+        const bool in = nw + 16 * part + n < cols;
+        if constexpr (decltype(bias_)::value) {
+          const float* at_bias = bias + (in ? 16 * part + n : -nw);
+          const float4 b = *reinterpret_cast<const float4*>(at_bias), d = *reinterpret_cast<const float4*>(at_bias + 4);
+          v += v4f{b.x, b.y, b.z, b.w};
+          z += v4f{d.x, d.y, d.z, d.w};
+        }
+        if (in && mw + m < a.M) {
+          if constexpr (out == 0) {
+            *reinterpret_cast<v4f*>(tile + (at + 4 * n)) = v;
+            *reinterpret_cast<v4f*>(tile + (at + 4 * n + 16)) = z;
+          } else {
+            *reinterpret_cast<uint4*>(tile + (at + 2 * n)) = make_uint4(pair(out, v[0], v[1]), pair(out, v[2], v[3]), pair(out, z[0], z[1]), pair(out, z[2], z[3]));
           }
         }
-        hold(i + 1);
-        issue_fence();
       }
-    };
+      hold(i + 1);
+      issue_fence();
+    }
+  };
+  if (splits > 1) {
+    const int64_t ld = 4ll * split_cols(a.N);
+    store_rows(Int<0>{}, Int<0>{}, a.work + split * a.M * ld, ld, split_cols(a.N));
+    return;
+  }
+  if (a.wide_rows && a.N % 8 == 0) {
     const auto of = [&](auto out) __attribute__((always_inline)) {
-      if (a.bias) all(out, Int<1>{});
-      else all(out, Int<0>{});
+      if (a.bias) store_rows(out, Int<1>{}, a.y, a.ldy, a.N);
+      else store_rows(out, Int<0>{}, a.y, a.ldy, a.N);
     };
     if (a.out == 0) of(Int<0>{});
     else if (a.out == 1) of(Int<1>{});
@@ -613,30 +624,58 @@ __global__ __launch_bounds__(128 * WN, 2) void mx4_tile_kernel(Mx4GemmArgs a, in
   }
 }
 
+// The splits' sums in order: four neighbours to a thread.
+__global__ __launch_bounds__(256) void mx4_join_kernel(Mx4GemmArgs a, int splits) {
+  const int cols = split_cols(a.N), quads = cols / 4;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, all = static_cast<int64_t>(a.M) * quads;
+  if (i >= all) return;
+  const int m = static_cast<int>(i / quads), n = static_cast<int>(i - static_cast<int64_t>(m) * quads) * 4;
+  const v4f* from = reinterpret_cast<const v4f*>(a.work) + i;
+  v4f y = from[0];
+#pragma unroll 4
+  for (int k = 1; k < splits; ++k) y += from[k * all];
+  if (n < a.N) store_outputs(a, m, n, y);
+}
+
 template <int FM, int FN, int WN, int D>
-hipError_t tiles(const Mx4GemmArgs& a, hipStream_t s) {
+hipError_t tiles(const Mx4GemmArgs& a, hipStream_t s, int splits = 1) {
   const int mt = ceil_div(a.M, 32 * FM), nt = ceil_div(a.N, 16 * FN * WN);
-  const dim3 grid(mt * nt), block(128 * WN);
-  if (a.K % 512) hipLaunchKernelGGL((mx4_tile_kernel<FM, FN, WN, D, true>), grid, block, 0, s, a, mt, nt);
-  else hipLaunchKernelGGL((mx4_tile_kernel<FM, FN, WN, D, false>), grid, block, 0, s, a, mt, nt);
+  const dim3 grid(mt * nt * splits), block(128 * WN);
+  if (a.K % 512) hipLaunchKernelGGL((mx4_tile_kernel<FM, FN, WN, D, true>), grid, block, 0, s, a, mt, nt, splits);
+  else hipLaunchKernelGGL((mx4_tile_kernel<FM, FN, WN, D, false>), grid, block, 0, s, a, mt, nt, splits);
+  if (splits > 1) {
+    const int64_t quads = static_cast<int64_t>(a.M) * (split_cols(a.N) / 4);
+    hipLaunchKernelGGL(mx4_join_kernel, dim3(static_cast<uint32_t>((quads + 255) / 256)), dim3(256), 0, s, a, splits);
+  }
   return hipGetLastError();
 }
 
-// Tiles of 256 x 256, 128 x 128 or 64 x 128, by what a stage of all of them takes, in ns: the rounds that fill the card, and the
-// last one, which may leave CUs to fewer workgroups. Measured at 8192 x 8192 x 8192 (265, 353 and 464 us) and, a workgroup to a CU or
-// less, at 128 x 4096 x 4096 (23.8, 12.9 and 10.8 us); 2011 x 12288 x 4096 takes 71, 76 and 93 us.
-int tile_choice(int M, int N) {
+// Tiles of 256 x 256, 128 x 128 or 64 x 128, and parts of K, by what they would take, in ns: a start, the stages in rounds that
+// fill the card, of which the last may leave CUs to fewer workgroups, and a second launch that joins the parts. Measured at
+// 8192 x 8192 x 8192 (265, 353 and 464 us) and, a workgroup to a CU or less, at 128 x 4096 x 4096 (23.8, 12.9 and 10.8 us);
+// 2011 x 12288 x 4096 takes 71, 76 and 93 us.
+struct TileChoice {
+  int kind, splits;
+};
+TileChoice tile_choice(int M, int N, int K) {
   const struct {
     int m, n, slots, full, one, none;  // workgroups at a time; ns of a stage with all of them, with one to a CU, with few
   } kinds[] = {{256, 256, 256, 1030, 1030, 650}, {128, 128, 512, 690, 400, 310}, {64, 128, 512, 450, 300, 240}};
-  int64_t best = INT64_MAX;
-  int choice = 0;
+  const int pieces = ceil_div(K, 512);
+  double best = 1e30;
+  TileChoice choice{0, 1};
   for (int i = 0; i < 3; ++i) {
     const auto& k = kinds[i];
-    const int64_t tiles = static_cast<int64_t>(ceil_div(M, k.m)) * ceil_div(N, k.n), left = tiles % k.slots;
-    const int64_t last = left > 256 ? k.full : k.none + (k.one - k.none) * left / 256;
-    const int64_t ns = tiles / k.slots * k.full + (left ? last : 0);
-    if (ns < best) best = ns, choice = i;
+    const int64_t tiles = static_cast<int64_t>(ceil_div(M, k.m)) * ceil_div(N, k.n);
+    for (int want = 1; want <= 32 && want <= pieces; want *= 2) {
+      const int each = ceil_div(pieces, want), splits = ceil_div(pieces, each);
+      const double bytes = 8.0 * splits * M * split_cols(N);
+      if (splits > 1 && (tiles * splits > 1024 || bytes > 128e6)) continue;
+      const int64_t all = tiles * splits, left = all % k.slots;
+      const double last = left > 256 ? k.full : k.none + (k.one - k.none) * left / 256.0;
+      const double ns = 4.0 * each * (all / k.slots * k.full + (left ? last : 0)) + (splits > 1 ? 2500 + bytes / 4000 : 0);
+      if (ns < best) best = ns, choice = {i, splits};
+    }
   }
   return choice;
 }
@@ -654,16 +693,17 @@ hipError_t launch_mx4_quant(const Mx4QuantArgs& a, hipStream_t s) {
 // Few enough numbers that every workgroup may quantise them for itself, which saves a launch.
 bool mx4_quantises(int M, int N, int K) { return few_fits(M, N, K) && static_cast<int64_t>(M) * K <= 1 << 17; }
 
-int64_t mx4_parts_bytes(int, int, int) { return 0; }
+int64_t mx4_parts_bytes(int M, int N, int K) {
+  if (few_fits(M, N, K)) return 0;
+  const int splits = tile_choice(M, N, K).splits;
+  return splits > 1 ? 4ll * splits * M * split_cols(N) : 0;
+}
 
 hipError_t launch_mx4_gemm(const Mx4GemmArgs& a, hipStream_t s) {
   if (a.dtype >= 0) return a.dtype == 0 ? few<XFp32>(a, s) : a.dtype == 1 ? few<XBf16>(a, s) : few<XFp16>(a, s);
   if (few_fits(a.M, a.N, a.K)) return few<Codes>(a, s);
-  switch (tile_choice(a.M, a.N)) {
-    case 0: return tiles<8, 4, 4, 2>(a, s);
-    case 1: return tiles<4, 4, 2, 2>(a, s);
-    default: return tiles<2, 4, 2, 2>(a, s);
-  }
+  const TileChoice c = tile_choice(a.M, a.N, a.K);
+  return c.kind == 0 ? tiles<8, 4, 4, 2>(a, s, c.splits) : c.kind == 1 ? tiles<4, 4, 2, 2>(a, s, c.splits) : tiles<2, 4, 2, 2>(a, s, c.splits);
 }
 
 }  // namespace tars
