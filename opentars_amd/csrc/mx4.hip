@@ -624,16 +624,16 @@ __global__ __launch_bounds__(128 * WN, 2) void mx4_tile_kernel(Mx4GemmArgs a, in
   }
 }
 
-// The splits' sums in order: four neighbours to a thread.
+// The splits' sums in order: four neighbours to a thread, which pass 32 bits in no shape that is split (tile_choice).
 __global__ __launch_bounds__(256) void mx4_join_kernel(Mx4GemmArgs a, int splits) {
   const int cols = split_cols(a.N), quads = cols / 4;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, all = static_cast<int64_t>(a.M) * quads;
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x, all = static_cast<uint32_t>(a.M) * quads;
   if (i >= all) return;
-  const int m = static_cast<int>(i / quads), n = static_cast<int>(i - static_cast<int64_t>(m) * quads) * 4;
+  const int m = i / quads, n = (i - m * quads) * 4;
   const v4f* from = reinterpret_cast<const v4f*>(a.work) + i;
   v4f y = from[0];
 #pragma unroll 4
-  for (int k = 1; k < splits; ++k) y += from[k * all];
+  for (int k = 1; k < splits; ++k) y += from[static_cast<int64_t>(k) * all];
   if (n < a.N) store_outputs(a, m, n, y);
 }
 
@@ -673,7 +673,7 @@ TileChoice tile_choice(int M, int N, int K) {
       if (splits > 1 && (tiles * splits > 1024 || bytes > 128e6)) continue;
       const int64_t all = tiles * splits, left = all % k.slots;
       const double last = left > 256 ? k.full : k.none + (k.one - k.none) * left / 256.0;
-      const double ns = 4.0 * each * (all / k.slots * k.full + (left ? last : 0)) + (splits > 1 ? 2500 + bytes / 4000 : 0);
+      const double ns = 4.0 * each * (all / k.slots * k.full + (left ? last : 0)) + (splits > 1 ? 2500 + bytes / 3000 : 0);
       if (ns < best) best = ns, choice = {i, splits};
     }
   }

@@ -121,6 +121,26 @@ def test_outputs_bias_and_strides(M, N, K, out):
         assert (rest == 7.0).all()
 
 
+@pytest.mark.parametrize("M,N,K", [(112, 11, 4352), (100, 1024, 8192), (97, 200, 10272), (842, 194, 4128), (130, 64, 16384)])
+def test_few_tiles_with_k_in_parts(M, N, K):
+    """A long K for few tiles is summed in parts: their sums in fp32 are whole quarters too, whichever part holds a k."""
+    x, w, want = exact_case(M + N + K, M, N, K)
+    a, b = dev(*x), dev(*w)
+    bias = (torch.arange(N) % 16 - 8).float()
+    assert _lib.lib().tars_mx4_workspace(M, N, K, 0) > 0
+    assert torch.equal(ops.gemm_mx4(a, b, out=OUT_FP32).cpu().double(), want)
+    for out, lead in ((OUT_FP32, 1), (OUT_BF16, 0), (OUT_FP16, 3)):
+        dt = TYPES["bf16" if out == OUT_BF16 else "fp16" if out == OUT_FP16 else "fp32"]
+        room = torch.full((M, lead + N + 5), 7.0, dtype=dt, device="cuda")
+        ops.gemm_mx4(a, b, bias=bias.cuda(), y=room[:, lead:lead + N])
+        assert torch.equal(room[:, lead:lead + N].cpu(), (want + bias.double()).to(dt))
+        room[:, lead:lead + N] = 7.0
+        assert (room == 7.0).all()
+    x[1][5, K // 32 - 1] = 255                                        # NaN in the last part alone
+    y = ops.gemm_mx4(dev(*x), b, out=OUT_FP32).cpu()
+    assert torch.isnan(y[5]).all() and torch.equal(y[:5].double(), want[:5]) and torch.equal(y[6:].double(), want[6:])
+
+
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("M,N,K", [(1, 64, 1024), (5, 33, 96), (16, 100, 4096), (17, 40, 288), (64, 64, 64), (90, 200, 512), (1, 3000, 512)])
 def test_a_tensor_is_quantised_in_the_call(t, M, N, K):
