@@ -454,7 +454,7 @@ int tars_quant_mx4(const void* x, int64_t ldx, int32_t dtype, const tars_mx4* ds
  *   address), out FP32, BF16 or FP16. Products of codes are exact, their sums fp32; past the output's
  *   largest value is infinity. Scales whose sum of exponents passes fp32's ends do so in the product too:
  *   sums below 2^-126 may come out 0. Without a sum that is NaN, the result is the same bits for any M
- *   that runs the same way (few rows, many rows). At most 2^22 rows of x and 2^24 of w.
+ *   that runs the same way (few rows, many rows). At most 2^22 rows of x, 2^24 of w and 2^38 outputs.
  */
 int tars_gemm_mx4(const tars_mx4* x, const tars_mx4* w, const float* bias, void* y, int64_t ldy,
                   int32_t out, void* work, int64_t work_bytes, void* stream);

@@ -731,7 +731,7 @@ int attention_args(const float* const* q, int64_t ldq, const float* const* k, in
 // ---- a serving step around the cache
 
 constexpr int kMaxMxK = 1 << 20, kMaxMxX = 1 << 22, kMaxMxW = 1 << 24, kMaxVocab = 1 << 24, kMaxGiven = 1 << 16, kMaxTop = 64;
-constexpr int64_t kMaxMxStride = 1 << 22;
+constexpr int64_t kMaxMxStride = 1 << 22, kMaxMxY = 1LL << 38;
 
 bool float_type(int32_t t) { return t == TARS_OUT_FP32 || t == TARS_OUT_BF16 || t == TARS_OUT_FP16; }
 int64_t mx_scale_row(int32_t k) { return (k + 511LL) / 512 * 16; }
@@ -795,6 +795,7 @@ int check_mx4_product(const tars_mx4* w, const float* bias, void* y, int64_t ldy
   Mx4Rows c;
   if (int rc = check_mx4(w, kMaxMxW, c)) return rc;
   if (w->k != a.K) return fail(TARS_E_FIELD, "x and w disagree on k");
+  if (static_cast<int64_t>(a.M) * w->rows > kMaxMxY) return fail(TARS_E_RANGE, "at most 2^38 outputs");
   a.w = c.m;
   a.N = w->rows;
   a.bias = bias;
@@ -827,7 +828,8 @@ int64_t mx4_need(int32_t M, int32_t N, int32_t K, bool quantises) {
   return (quantises && !tars::mx4_quantises(M, N, K) ? M * (K / 2 + mx_scale_row(K)) : 0) + tars::mx4_parts_bytes(M, N, K);
 }
 bool mx4_sizes_ok(int32_t M, int32_t N, int32_t K) {
-  return M >= 1 && N >= 1 && K >= 32 && K % 32 == 0 && M <= kMaxMxX && N <= kMaxMxW && K <= kMaxMxK;
+  return M >= 1 && N >= 1 && K >= 32 && K % 32 == 0 && M <= kMaxMxX && N <= kMaxMxW && K <= kMaxMxK &&
+         static_cast<int64_t>(M) * N <= kMaxMxY;
 }
 bool logprobs_sizes_ok(int32_t rows_, int32_t vocab, int32_t dtype, int32_t top) {
   return rows_ >= 1 && vocab >= 1 && float_type(dtype) && top >= 0 && top <= kMaxTop && top <= vocab && rows_ <= kMaxPagedRows && vocab <= kMaxVocab;
