@@ -17,6 +17,7 @@
 
 #include "kernels.h"
 #include "paged_index.h"
+#include "wave_reduce.h"
 
 namespace tars {
 namespace {
@@ -98,23 +99,23 @@ struct List {
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int i = 0; i < kRoom / kLanes; ++i) {
+      place[i] = top;
+      if (kLanes * i >= n) continue;
       a[i] = lane + kLanes * i < n ? keys[lane + kLanes * i] : 0;
-      place[i] = 0;
-    }
+      place[i] = a[i] ? 0 : top;
 #pragma unroll 1
-    for (int k = 0; k < n; k += kAhead) {
-      Key c[kAhead];
+      for (int k = 0; k < n; k += kAhead) {
+        Key c[kAhead];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) c[i] = keys[k + i];
-#pragma unroll
-      for (int i = 0; i < kRoom / kLanes; ++i)
+        for (int j = 0; j < kAhead; ++j) c[j] = keys[k + j];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) place[i] += c[j] > a[i];
+      }
     }
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int i = 0; i < kRoom / kLanes; ++i)
-      if (a[i] && place[i] < top) keys[place[i]] = a[i];
+      if (place[i] < top) keys[place[i]] = a[i];
     __builtin_amdgcn_wave_barrier();
     n = min(n, top);
     const Key end = keys[top - 1];
@@ -125,11 +126,13 @@ struct List {
 
 struct XF32 {
   static constexpr int kEach = 4;  // logits in 16 bytes
+  static constexpr bool kWhole = false;  // whether the upper 16 bits are all of a logit
   static __device__ __forceinline__ float at(const uint32_t* w, int e) { return __uint_as_float(w[e]); }
   static __device__ __forceinline__ float one(const char* p) { return *reinterpret_cast<const float*>(p); }
 };
 struct XBf16 {
   static constexpr int kEach = 8;
+  static constexpr bool kWhole = true;
   static __device__ __forceinline__ float at(const uint32_t* w, int e) {
     return __uint_as_float(e & 1 ? w[e / 2] & 0xFFFF0000u : w[e / 2] << 16);
   }
@@ -139,6 +142,7 @@ struct XBf16 {
 };
 struct XF16 {
   static constexpr int kEach = 8;
+  static constexpr bool kWhole = false;
   static __device__ __forceinline__ float at(const uint32_t* w, int e) {
     return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)))));
   }
@@ -146,17 +150,26 @@ struct XF16 {
 };
 
 __device__ __forceinline__ Sums over_wave(Sums a) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    a.join({__shfl_xor(a.m, d), __shfl_xor(a.s, d), __shfl_xor(a.t, d)});
-  }
+  const auto with = [&](auto other) { a.join({other(a.m), other(a.s), other(a.t)}); };
+  with([](float x) { return __int_as_float(dpp<kDppQuadXor1>(__float_as_int(x))); });
+  with([](float x) { return __int_as_float(dpp<kDppQuadXor2>(__float_as_int(x))); });
+  with([](float x) { return __int_as_float(dpp<kDppRowHalfMirror>(__float_as_int(x))); });
+  with([](float x) { return __int_as_float(dpp<kDppRowMirror>(__float_as_int(x))); });
+  with([](float x) { return __shfl_xor(x, 16); });
+  with([](float x) { return __shfl_xor(x, 32); });
   return a;
+}
+
+// Whether the upper 16 of a logit's `ordered` bits are all of it: a bfloat16, or -infinity, which is much of a masked row.
+template <class X>
+__device__ __forceinline__ bool whole(uint32_t upper) {
+  return X::kWhole || upper == ordered(-INFINITY) >> 16;
 }
 
 // The workgroup's bound, for every wave: the top-th largest of the lanes' maxima, to 16 bits of their `ordered` values (0: a lane
 // without one); where more lanes than that are equal by those bits, by their whole keys (place() is where a lane has its maximum
 // first).
-template <class F>
+template <class X, class F>
 __device__ __forceinline__ Key bound_of(Shared& sh, uint32_t most, int top, F place) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const bool mine = wave == static_cast<int>((blockIdx.x + blockIdx.y) & (kWaves - 1));  // one wave's work, another's in each workgroup
@@ -187,13 +200,20 @@ __device__ __forceinline__ Key bound_of(Shared& sh, uint32_t most, int top, F pl
     Key k[kWaves];
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) k[w] = sh.keys[w][lane];
+    const auto search = [&](Key from, Key to) __attribute__((always_inline)) {
 #pragma unroll 1
-    for (Key bit = Key{1} << 47; bit; bit >>= 1) {
-      int count = 0;
+      for (Key bit = from; bit >= to; bit >>= 1) {
+        int count = 0;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) count += __popcll(__ballot(k[w] >= (b | bit)));
-      if (count >= top) b |= bit;
-    }
+        for (int w = 0; w < kWaves; ++w) count += __popcll(__ballot(k[w] >= (b | bit)));
+        if (count >= top) b |= bit;
+      }
+    };
+    // the logit's lower bits where it has any, then the place's 24: the bits above those are ones in every key
+    if (whole<X>(static_cast<uint32_t>(b >> 48))) b |= b >> 48 & 0x8000u ? 0 : Key{0xFFFF} << 32;
+    else search(Key{1} << 47, Key{1} << 32);
+    b |= 0xFF000000u;
+    search(Key{1} << 23, 1);
     __syncthreads();  // before the lists take the keys' room
   }
   return b ? b - 1 : 0;
@@ -244,8 +264,23 @@ __device__ __forceinline__ Sums over_workgroup(Shared& sh, Sums a, List& list) {
   return all;
 }
 
+// The logit of the row's i-th given token; `in`: whether it has one.
+struct Given {
+  float x;
+  bool in;
+};
 template <class X>
-__device__ __forceinline__ void answer(const LogprobArgs& a, const Shared& sh, Sums all, int row) {
+__device__ __forceinline__ Given given_at(const LogprobArgs& a, int row, int i) {
+  if (i >= a.given) return {0, false};
+  const char* tokens = static_cast<const char*>(a.tokens) + row * a.ld_tokens;
+  const int64_t t = a.wide_tokens ? reinterpret_cast<const int64_t*>(tokens)[i] : reinterpret_cast<const int32_t*>(tokens)[i];
+  const bool in = t >= 0 && t < a.vocab;
+  return {in ? X::one(a.x + row * a.ld + t * (16 / X::kEach)) : 0.0f, in};
+}
+
+// The row's results; `first` is the thread's first given token, fetched before its value is needed.
+template <class X>
+__device__ __forceinline__ void answer(const LogprobArgs& a, const Shared& sh, Sums all, int row, Given first) {
   const bool none = all.s == 0;
   const double log_s = none ? 0.0 : ::log(static_cast<double>(all.s));  // once a row: in 64 bits
   const auto lp = [&](float x) { return none ? -INFINITY : static_cast<float>(static_cast<double>(x) - all.m - log_s); };
@@ -258,12 +293,9 @@ __device__ __forceinline__ void answer(const LogprobArgs& a, const Shared& sh, S
     a.top_values[static_cast<int64_t>(row) * a.top + threadIdx.x] = lp(value_of(static_cast<uint32_t>(k >> 32)));
     a.top_ids[static_cast<int64_t>(row) * a.top + threadIdx.x] = static_cast<int32_t>(~static_cast<uint32_t>(k));
   }
-  const char* tokens = static_cast<const char*>(a.tokens) + row * a.ld_tokens;
   for (int i = threadIdx.x; i < a.given; i += blockDim.x) {
-    const int64_t t = a.wide_tokens ? reinterpret_cast<const int64_t*>(tokens)[i] : reinterpret_cast<const int32_t*>(tokens)[i];
-    const bool in = t >= 0 && t < a.vocab;
-    a.logprobs[static_cast<int64_t>(row) * a.given + i] =
-        in ? lp(X::one(a.x + row * a.ld + t * (16 / X::kEach))) : -INFINITY;
+    a.logprobs[static_cast<int64_t>(row) * a.given + i] = first.in ? lp(first.x) : -INFINITY;
+    first = given_at<X>(a, row, i + blockDim.x);
   }
 }
 
@@ -345,7 +377,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void logprobs_kernel(LogprobArgs a)
   if constexpr (TOP) {
     const auto at_of = [&](int p, int i, int e) { return head + (p + 64 * i + lane) * kEach + e; };
     const bool any = p0 + lane < p1;
-    list.last = bound_of(sh, any ? ordered(most) : 0, a.top, [&]() {  // where the lane has its maximum first
+    list.last = bound_of<X>(sh, any ? ordered(most) : 0, a.top, [&]() {  // where the lane has its maximum first
       int at = a.vocab - 1;
 #pragma unroll 1
       for (int p = p0; __ballot(any && at == a.vocab - 1) && p < p1; p += 64 * kLoads) {
@@ -360,8 +392,16 @@ __global__ __launch_bounds__(64 * kWaves, 4) void logprobs_kernel(LogprobArgs a)
       return at;
     });
     list.take(key_of(edge_v, edge_at), edge);
+    // The groups that reach the bound. Where its 16 bits are all of a logit, a group that equals them and lies behind the bound's
+    // own place does not.
+    const uint32_t line = static_cast<uint32_t>((list.last + 1) >> 48), least_at = ~static_cast<uint32_t>(list.last + 1);
+    const bool all_bits = whole<X>(line);
     uint32_t groups = 0;
-    for (int k = 0; k < group; ++k) groups |= static_cast<uint32_t>(sh.group[k][threadIdx.x] >= static_cast<uint32_t>((list.last + 1) >> 48)) << k;
+    for (int k = 0; k < group; ++k) {
+      const uint32_t g = sh.group[k][threadIdx.x];
+      const bool before = !all_bits || static_cast<uint32_t>(at_of(p0 + k * stride * 64 * kLoads, 0, 0)) <= least_at;
+      groups |= static_cast<uint32_t>(g > line || (g == line && before)) << k;
+    }
 #pragma unroll 1
     for (uint32_t all = any ? groups : 0; __ballot(all != 0); all &= all - 1) {
       const int k = all ? __builtin_ctz(all) : 0;
@@ -401,9 +441,10 @@ __global__ __launch_bounds__(64 * kWaves, 4) void logprobs_kernel(LogprobArgs a)
       }
     }
   }
+  const Given first = a.parts == 1 ? given_at<X>(a, row, threadIdx.x) : Given{0, false};
   const Sums all = over_workgroup(sh, sums, list);
   if (a.parts == 1) {
-    answer<X>(a, sh, all, row);
+    answer<X>(a, sh, all, row, first);
     return;
   }
   char* to = part_at(a, row, part);
@@ -415,6 +456,7 @@ template <class X>
 __global__ __launch_bounds__(64 * kWaves) void logprobs_join_kernel(LogprobArgs a) {
   __shared__ Shared sh;
   const int row = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Given first = given_at<X>(a, row, threadIdx.x);
   Sums sums = Sums::none();
   for (int p = threadIdx.x; p < a.parts; p += 64 * kWaves) {
     const float4 v = *reinterpret_cast<const float4*>(part_at(a, row, p));
@@ -428,13 +470,13 @@ __global__ __launch_bounds__(64 * kWaves) void logprobs_join_kernel(LogprobArgs 
       const int at = base + threadIdx.x, k = at / a.parts;  // the parts' largest first
       const bool in = at < n;
       const Key key = in ? reinterpret_cast<const Key*>(part_at(a, row, at - k * a.parts) + 16)[k] : 0;
-      if (base == 0) list.last = bound_of(sh, static_cast<uint32_t>(key >> 32), a.top, [&]() { return static_cast<int>(~static_cast<uint32_t>(key)); });
+      if (base == 0) list.last = bound_of<X>(sh, static_cast<uint32_t>(key >> 32), a.top, [&]() { return static_cast<int>(~static_cast<uint32_t>(key)); });
       list.cut();
       list.take(key, in);
     }
   }
   const Sums all = over_workgroup(sh, sums, list);
-  answer<X>(a, sh, all, row);
+  answer<X>(a, sh, all, row, first);
 }
 
 template <class X>
