@@ -405,7 +405,7 @@ int tars_paged_decode(const tars_kv_pool* pool, const void* q, int64_t ldq, int3
  *   qgamma, kgamma fp32 [hd] or NULL; tab fp32 [positions, rot], dense; rot a multiple of 16, up to hd.
  *   lens, starts, seqs: the rows' sequences, as tars_kv_append's; row i of a sequence's n is at position
  *   lens[b] - n + i. A row without a sequence, at a negative position or at one that tab does not have
- *   leaves its outputs as they were.
+ *   leaves its outputs as they were. rows * (heads + 2 kv_heads) * hd is at most 2^35.
  */
 int tars_qk_norm_rope(const void* q, int64_t ldq, const void* k, int64_t ldk, int32_t dtype, int32_t heads,
                       int32_t kv_heads, int32_t hd, int32_t rows, const float* qgamma, const float* kgamma,

@@ -145,7 +145,7 @@ float f32_of(uint32_t b) {
 // ---- the paged key / value cache
 
 constexpr int kMaxPagedRows = 1 << 22, kMaxPositions = 1 << 30, kMaxPagedHeads = 1024, kMaxPagedSeqs = 65535;
-constexpr int64_t kMaxSlotBytes = 1 << 26, kMaxSeqHeads = 1 << 22, kMaxRowHeads = 1 << 28;
+constexpr int64_t kMaxSlotBytes = 1 << 26, kMaxSeqHeads = 1 << 22, kMaxRowHeads = 1 << 28, kMaxRowElements = 1LL << 35;
 
 bool head_ok(int32_t hd) { return hd == 64 || hd == 128 || hd == 256; }
 bool page_ok(int32_t page) { return page >= 16 && (page & (page - 1)) == 0 && page <= kMaxPositions; }
@@ -761,7 +761,8 @@ int check_rope(const void* q, int64_t& ldq, int32_t heads, int32_t kv_heads, int
   if (positions < 1) return fail(TARS_E_ALIGN, "positions >= 1");
   if (!aligned(tab, 16) || !aligned(qgamma, 16) || !aligned(kgamma, 16)) return fail(TARS_E_ALIGN, "pointers must be 16-byte aligned");
   if (positions > kMaxPositions) return fail(TARS_E_RANGE, "at most 2^30 positions");
-  if (static_cast<int64_t>(rows_) * heads > kMaxRowHeads) return fail(TARS_E_RANGE, "rows * heads must be at most 2^28");
+  if (static_cast<int64_t>(rows_) * (heads + 2 * kv_heads) * hd > kMaxRowElements)
+    return fail(TARS_E_RANGE, "rows * (heads + 2 kv_heads) * hd must be at most 2^35");
   if (!extent_ok(tab, 4LL * rot, positions, 4LL * rot)) return fail(TARS_E_RANGE, "extent overflows");
   if (int rc = check_rows(q, ldq, rows_, 2LL * heads * hd)) return rc;
   return check_rows(yq, ldyq, rows_, 2LL * heads * hd);

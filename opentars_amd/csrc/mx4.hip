@@ -297,7 +297,10 @@ int few_split(int M, int N, int K) {
   while (kw < kFewWaves && tiles * kw < (M <= 16 ? 2048 : 1024) && 2 * kw <= steps) kw *= 2;
   return kw;
 }
-bool few_fits(int M, int N, int K) { return M <= 64 && few_lds_bytes(M, K, few_split(M, N, K)) <= kLds; }
+// Up to 48 rows run this way: 48 x 2048 x 1024 takes 4.6 us either way, 32 x 4096 x 2048 5.1 us (tiles 5.8), 64 x 2048 x 1024
+// would take 5.4 (tiles 4.7).
+constexpr int kFewRows = 48;
+bool few_fits(int M, int N, int K) { return M <= kFewRows && few_lds_bytes(M, K, few_split(M, N, K)) <= kLds; }
 
 template <class X>
 hipError_t few(const Mx4GemmArgs& a, hipStream_t s) {
@@ -307,8 +310,7 @@ hipError_t few(const Mx4GemmArgs& a, hipStream_t s) {
   const dim3 grid(std::min(groups, 256 * (kLds / lds))), block(64 * kFewWaves);
   if (a.M <= 16) hipLaunchKernelGGL((mx4_few_kernel<X, 1>), grid, block, lds, s, a, kw, per);
   else if (a.M <= 32) hipLaunchKernelGGL((mx4_few_kernel<X, 2>), grid, block, lds, s, a, kw, per);
-  else if (a.M <= 48) hipLaunchKernelGGL((mx4_few_kernel<X, 3>), grid, block, lds, s, a, kw, per);
-  else hipLaunchKernelGGL((mx4_few_kernel<X, 4>), grid, block, lds, s, a, kw, per);
+  else hipLaunchKernelGGL((mx4_few_kernel<X, 3>), grid, block, lds, s, a, kw, per);
   return hipGetLastError();
 }
 
@@ -596,32 +598,58 @@ __global__ __launch_bounds__(128 * WN, 2) void mx4_tile_kernel(Mx4GemmArgs a, in
     else of(Int<3>{});
     return;
   }
-  // the output's edge, or rows that are not aligned: 16 rows at a time through the wave's own part of the ring
-  constexpr int kCols = 16 * FN, kPitch = kCols + 4, kAtOnce = FM > 4 ? 1 : 8;
+  if (a.wide_store) {  // four neighbours of a row are aligned
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const int thread = thread_again(), m = mw + 16 * i + (thread & 15), n = nw + (thread & 48);
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+        if (m < a.M && n + 4 * j < a.N) store_outputs(a, m, n + 4 * j, c[i][j]);
+      hold(i + 1);
+      issue_fence();
+    }
+    return;
+  }
+  // the output's edge, or rows that are not aligned: 16 rows at a time through the wave's own part of the ring, then a column to a
+  // lane (170 x 11 x 736, a case of one element after the other: TIME)
+  static_assert(FN == 4, "a column of a wave's to each lane");
+  constexpr int kPitch = 68, kAtOnce = FM > 4 ? 8 : 16;
   static_assert(kWaves * 16 * kPitch * 4 <= D * kPair, "a wave's 16 rows fit");
   float* mine = reinterpret_cast<float*>(lds) + wave * 16 * kPitch;
+  const auto store_columns = [&](auto out_) __attribute__((always_inline)) {
+    constexpr int out = decltype(out_)::value, e = out == 0 ? 4 : 2;
 #pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int thread = thread_again(), col = thread & 15, part = thread >> 4 & 3;
+    for (int i = 0; i < FM; ++i) {
+      const int thread = thread_again(), col = thread & 15, part = thread >> 4 & 3, lane = thread & 63;
+      const int n = nw + lane, first = __builtin_amdgcn_readfirstlane(mw) + 16 * i;
 #pragma unroll
-    for (int j = 0; j < FN; ++j)
-      *reinterpret_cast<v4f*>(mine + col * kPitch + 64 * (j / 4) + 16 * part + 4 * (j % 4)) = c[i][j];
-    hold(i + 1);
-    wait_lgkm0();
-    issue_fence();
-#pragma unroll kAtOnce
-    for (int k = thread & 63; k < 16 * kCols; k += 64) {
-      const int m = mw + 16 * i + k / kCols, n = nw + k % kCols;
-      if (m < a.M && n < a.N) {
-        const float y = mine[k / kCols * kPitch + k % kCols] + (a.bias ? a.bias[n] : 0.0f);
-        char* to = a.y + m * a.ldy;
-        if (a.out == 0) reinterpret_cast<float*>(to)[n] = y;
-        else reinterpret_cast<uint16_t*>(to)[n] = static_cast<uint16_t>(pair(a.out, y, 0.0f));
+      for (int j = 0; j < FN; ++j) *reinterpret_cast<v4f*>(mine + col * kPitch + 16 * part + 4 * j) = c[i][j];
+      hold(i + 1);
+      wait_lgkm0();
+      issue_fence();
+      const float bias = a.bias ? a.bias[min(n, a.N - 1)] : 0.0f;
+#pragma unroll 1
+      for (int r0 = 0; r0 < 16 && first + r0 < a.M; r0 += kAtOnce) {
+        float y[kAtOnce];
+#pragma unroll
+        for (int r = 0; r < kAtOnce; ++r) y[r] = mine[(r0 + r) * kPitch + lane] + bias;
+#pragma unroll
+        for (int r = 0; r < kAtOnce; ++r) {
+          const int m = first + r0 + r;
+          char* to = a.y + m * a.ldy;
+          if (m < a.M && n < a.N) {
+            if constexpr (out == 0) reinterpret_cast<float*>(to)[n] = y[r];
+            else reinterpret_cast<uint16_t*>(to)[n] = static_cast<uint16_t>(pair(out, y[r], 0.0f));
+          }
+        }
       }
+      wait_lgkm0();
+      issue_fence();
     }
-    wait_lgkm0();
-    issue_fence();
-  }
+  };
+  if (a.out == 0) store_columns(Int<0>{});
+  else if (a.out == 1) store_columns(Int<1>{});
+  else store_columns(Int<3>{});
 }
 
 // The splits' sums in order: four neighbours to a thread, which pass 32 bits in no shape that is split (tile_choice).
@@ -660,7 +688,7 @@ struct TileChoice {
 TileChoice tile_choice(int M, int N, int K) {
   const struct {
     int m, n, slots, full, one, none;  // workgroups at a time; ns of a stage with all of them, with one to a CU, with few
-  } kinds[] = {{256, 256, 256, 1030, 1030, 650}, {128, 128, 512, 690, 400, 310}, {64, 128, 512, 450, 300, 240}};
+  } kinds[] = {{256, 256, 256, 1030, 1030, 650}, {128, 128, 512, 690, 400, 310}, {64, 128, 512, 450, 260, 200}};
   const int pieces = ceil_div(K, 512);
   double best = 1e30;
   TileChoice choice{0, 1};
@@ -672,7 +700,7 @@ TileChoice tile_choice(int M, int N, int K) {
       const double bytes = 8.0 * splits * M * split_cols(N);
       if (splits > 1 && (tiles * splits > 1024 || bytes > 128e6)) continue;
       const int64_t all = tiles * splits, left = all % k.slots;
-      const double last = left > 256 ? k.full : k.none + (k.one - k.none) * left / 256.0;
+      const double last = left > 256 ? k.full : all > left ? k.one : k.none + (k.one - k.none) * left / 256.0;
       const double ns = 4.0 * each * (all / k.slots * k.full + (left ? last : 0)) + (splits > 1 ? 2500 + bytes / 3000 : 0);
       if (ns < best) best = ns, choice = {i, splits};
     }
