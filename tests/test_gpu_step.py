@@ -138,3 +138,50 @@ def test_a_queue_of_products_of_one_quantised_input():
     for n in (64, 300, 1000):
         w = on_gpu(random_codes(g, n, 512, low=120, spread=4))
         assert torch.equal(bits(ops.gemm_mx4(q, w).cpu()), bits(ops.gemm_mx4(x, w).cpu()))
+
+
+# ------------------------------------------------------------------------------------------------ the ends of the ranges
+@pytest.mark.parametrize("M,N,K", [(1, 16, 2 ** 20), (50, 3, 2 ** 20), (1, 300001, 32), (70001, 3, 64), (49, 70000, 32), (200, 24, 2 ** 18)])
+def test_products_at_the_ends(M, N, K):
+    g = torch.Generator().manual_seed(M + N)
+    x, w = random_codes(g, M, K, low=124, spread=4), random_codes(g, N, K, low=124, spread=4)
+    a, b = values_of(*x), values_of(*w)
+    want, size = a @ b.T, a.abs() @ b.abs().T
+    got = ops.gemm_mx4(on_gpu(x), on_gpu(w), out=OUT_FP32)
+    tol = (8 + 2 * math.sqrt(K)) * 2.0 ** -24 * size
+    assert ((got.cpu().double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("rows,vocab,top,dt", [(1, 2 ** 24, 64, torch.float32), (70001, 3, 3, torch.bfloat16), (1, 2 ** 24, 0, torch.bfloat16),
+                                               (257, 20000, 7, torch.float16), (70, 262144, 64, torch.bfloat16)])
+def test_log_probabilities_at_the_ends(rows, vocab, top, dt):
+    g = torch.Generator().manual_seed(vocab)
+    x = (3 * torch.randn(rows, vocab, generator=g)).to(dt)
+    t = torch.randint(-1, vocab, (rows, 2), generator=g)
+    r = ops.token_logprobs(x.cuda(), t.cuda(), top=top)
+    for i in {0, 1, rows // 2, rows - 2, rows - 1} & set(range(rows)):
+        d = x[i].double()
+        lp = torch.log_softmax(d, 0)
+        tol = (16 + 2 * math.sqrt(vocab)) * 2.0 ** -24 + 8 * 2.0 ** -24 * max(20.0, float(d.max() - d.min()))
+        order = torch.sort(d, descending=True, stable=True).indices[:top]
+        for got, want in ((r.entropy[i], -(lp.exp() * lp).sum()),
+                          (r.logprobs[i], torch.stack([lp[k] if k >= 0 else torch.tensor(-math.inf, dtype=torch.float64) for k in t[i]]))):
+            far = (got.cpu().double() - want).abs()
+            assert ((far <= tol) | (got.cpu().double() == want)).all()
+        if top:
+            assert torch.equal(r.top_ids[i].cpu().long(), order)
+            assert ((r.top_logprobs[i].cpu().double() - lp[order]).abs() <= tol).all()
+
+
+def test_rotation_of_many_rows_and_heads():
+    """Rows past 2^16, and 1024 heads of one row, of sequences that the lengths place anywhere."""
+    g = torch.Generator().manual_seed(9)
+    for rows, heads, kv, hd in ((70001, 1, 1, 64), (3, 1024, 1024, 64), (2, 3, 1, 256)):
+        q, k = (torch.randn(rows, h * hd, generator=g).half() for h in (heads, kv))
+        tab = table(rows + 5, 16)
+        starts, lens = torch.tensor([0, rows], dtype=torch.int32), torch.tensor([rows + 5], dtype=torch.int32)
+        yq, yk = ops.qk_norm_rope(q.cuda(), k.cuda(), hd, tab.cuda(), lens.cuda(), starts.cuda())
+        for got, x in ((yq, q), (yk, k)):
+            want, tol = rotated(x, None, tab, torch.arange(5, rows + 5), hd, 1e-6)
+            tol = tol + HALF[torch.float16] * (want.abs() + tol) + TINY[torch.float16]
+            assert ((got.cpu().double().view(want.shape) - want).abs() <= tol).all()
