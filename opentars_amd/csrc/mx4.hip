@@ -688,7 +688,9 @@ hipError_t tiles(const Mx4GemmArgs& a, hipStream_t s, int splits = 1) {
 // fill the card, of which the last may leave CUs to fewer workgroups, and a second launch that joins the parts. Measured at
 // 8192 x 8192 x 8192 (265, 353 and 464 us) and, a workgroup to a CU or less, at 64 x 4096 x 4096 (23.6, 10.8 and 8.8 us);
 // 2011 x 12288 x 4096 takes 65, 73 and 93 us. In eight parts 100 x 1024 x 8192 takes 10.4 us for 17.9 (64 x 128 tiles), in two
-// 64 x 4096 x 4096 10.4 for 8.8, which is why the join counts.
+// 64 x 4096 x 4096 10.4 for 8.8, which is why the join counts. (Whole rounds of columns first and the rest in smaller tiles, by a
+// second launch, took 75 us where this takes 75 for 2011 x 12288 x 4096, 86 and 83 for 5000 x 5000 x 5120, 90 and 102 for 3000 x
+// 11008 x 4096: at the power limit a round half empty runs faster.)
 struct TileChoice {
   int kind, splits;
 };
@@ -725,7 +727,6 @@ hipError_t launch_mx4_quant(const Mx4QuantArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
-// Few enough numbers that every workgroup may quantise them for itself, which saves a launch.
 // Whether few rows are quantised by every workgroup itself rather than by a launch before: 1 x 4096 x 4096 then takes 3.8 us for
 // 5.2, 16 x 4096 x 4096 6.1 for 7.0; from 2^17 elements on it is the same (2 x 2048 x 65536, 32 x 1024 x 8192).
 bool mx4_quantises(int M, int N, int K) { return few_fits(M, N, K) && static_cast<int64_t>(M) * K <= 1 << 17; }

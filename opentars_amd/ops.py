@@ -776,7 +776,7 @@ def _mx4_rows(x: torch.Tensor, what: str = "x"):
 def quant_mx4(x: torch.Tensor) -> Mx4:
     """x [rows, cols], fp32, bf16 or fp16, cols a multiple of 32, in microscaled 4 bits: each 32 columns' scale has the exponent
     of their largest magnitude, less 2; x over it is rounded to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6, even codes on a tie
-    and 6 past it. A block that holds an infinity or NaN is NaN."""
+    and 6 past it. A block that holds an infinity or NaN is NaN. Rows contiguous and on 16 bytes."""
     code, rows, cols, ld = _mx4_rows(x)
     if cols % 32 or cols == 0:
         raise ValueError("x must be [rows, cols], cols a multiple of 32")
@@ -801,7 +801,7 @@ def gemm_mx4(x: torch.Tensor | Mx4, w: Mx4, bias: torch.Tensor | None = None, ou
              y: torch.Tensor | None = None) -> torch.Tensor:
     """y = x w^T + bias for a weight matrix w [N, K] in microscaled 4 bits. x [M, K]: a tensor (fp32, bf16 or fp16), which the
     call quantises as quant_mx4 does, or an Mx4. bias fp32 [N]. Sums are fp32 and rounded once, to out (OUT_FP32, OUT_BF16,
-    OUT_FP16; a given y's type, else x's own, else OUT_BF16). y [M, N], rows contiguous."""
+    OUT_FP16; a given y's type, else x's own, else OUT_BF16). y [M, N], rows contiguous; a tensor x's rows also on 16 bytes."""
     mx = isinstance(x, Mx4)
     if mx:
         code, M, K, ld = None, x.rows, x.cols, 0

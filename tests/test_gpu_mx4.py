@@ -141,6 +141,20 @@ def test_few_tiles_with_k_in_parts(M, N, K):
     assert torch.isnan(y[5]).all() and torch.equal(y[:5].double(), want[:5]) and torch.equal(y[6:].double(), want[6:])
 
 
+@pytest.mark.parametrize("M,N,K,lead", [(2011, 12288, 4096, 0), (2011, 12301, 4096, 3), (1200, 20000, 2048, 0)])
+def test_more_tiles_than_a_round(M, N, K, lead):
+    """Every 64th column, those around tiles' ends, the last."""
+    x, w = (random_codes(torch.Generator().manual_seed(M + n), n, K) for n in (M, N))
+    bias = (torch.arange(N) % 16 - 8).float()
+    room = torch.full((M, lead + N + 5), 7.0, dtype=torch.float32, device="cuda")
+    ops.gemm_mx4(dev(*x), dev(*w), bias=bias.cuda(), y=room[:, lead:lead + N])
+    at = torch.tensor([n for n in range(N) if n % 64 == 5 or n % 128 in (0, 127) or n > N - 20])
+    want = values_of(*x).float() @ values_of(w[0][at], w[1][at]).float().T + bias[at]     # exact: whole quarters below 2^24 of them
+    assert torch.equal(room[:, lead:lead + N].cpu()[:, at], want)
+    room[:, lead:lead + N] = 7.0
+    assert (room == 7.0).all()
+
+
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("M,N,K", [(1, 64, 1024), (5, 33, 96), (16, 100, 4096), (17, 40, 288), (64, 64, 64), (90, 200, 512), (1, 3000, 512)])
 def test_a_tensor_is_quantised_in_the_call(t, M, N, K):
