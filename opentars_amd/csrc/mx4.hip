@@ -227,6 +227,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx4_few_kernel(Mx4GemmArgs a, 
     asm volatile("" ::: "memory");
   };
   if (tile < tiles && first < end) issue(tile, first, 0);
+  // a block to a thread: 16 x 4096 x 4096 from bf16 takes 5.7 us (three of a thread's at once 6.8, four lanes to a block 8.8)
   for (int i = threadIdx.x; i < blocks * a.M; i += 64 * kFewWaves) {
     const int m = i / blocks, b = i - m * blocks;
     const Operand o = load_x<X>(a, m, b);
