@@ -453,8 +453,9 @@ int tars_quant_mx4(const void* x, int64_t ldx, int32_t dtype, const tars_mx4* ds
  *   bias fp32 [N] or NULL; y [M, N] at ldy bytes (0 = dense; a multiple of the element size, as y's
  *   address), out FP32, BF16 or FP16. Products of codes are exact, their sums fp32; past the output's
  *   largest value is infinity. Scales whose sum of exponents passes fp32's ends do so in the product too:
- *   sums below 2^-126 may come out 0. Without a sum that is NaN, the result is the same bits for any M
- *   that runs the same way (few rows, many rows). At most 2^22 rows of x, 2^24 of w and 2^38 outputs.
+ *   sums below 2^-126 may come out 0. The order of a sum, and with it its last bits, goes by M, N and K
+ *   alone: at the same sizes a row's result has the same bits wherever it is and whatever the other rows
+ *   are, at another M it may not. At most 2^22 rows of x, 2^24 of w and 2^38 outputs.
  */
 int tars_gemm_mx4(const tars_mx4* x, const tars_mx4* w, const float* bias, void* y, int64_t ldy,
                   int32_t out, void* work, int64_t work_bytes, void* stream);

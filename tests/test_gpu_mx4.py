@@ -308,3 +308,21 @@ def test_the_workspace_ends_where_it_says():
         assert rc == 0, _lib.last_error()
         assert torch.equal(bits(y), bits(ops.gemm_mx4(x, w)))
         assert (room[:256] == 0x5A).all() and (room[256 + need:] == 0x5A).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(16, 600, 5120), (37, 515, 1536), (64, 256, 4096), (100, 1024, 8192), (300, 300, 1056)])
+def test_a_rows_bits_are_its_own(M, N, K):
+    """At the same sizes a row's result has the same bits wherever it is and whatever the other rows are. The scales are far enough
+    apart (2^30) that fp32 rounds the sums."""
+    g = torch.Generator().manual_seed(M + K)
+    x = torch.randn(M, K, generator=g).bfloat16()
+    codes = random_codes(g, N, K, low=100, spread=30)
+    w = dev(*codes)
+    y = ops.gemm_mx4(x.cuda(), w, out=OUT_FP32).cpu()
+    exact = values_of(*quantised(x)) @ values_of(*codes).T
+    assert (y.double() != exact).double().mean() > 0.5
+    order = torch.randperm(M, generator=g)
+    assert torch.equal(bits(ops.gemm_mx4(x[order].cuda(), w, out=OUT_FP32).cpu()), bits(y[order]))
+    other = torch.randn(M, K, generator=g).bfloat16()
+    other[M // 3] = x[M // 3]
+    assert torch.equal(bits(ops.gemm_mx4(other.cuda(), w, out=OUT_FP32).cpu()[M // 3]), bits(y[M // 3]))
