@@ -326,3 +326,46 @@ def test_a_rows_bits_are_its_own(M, N, K):
     other = torch.randn(M, K, generator=g).bfloat16()
     other[M // 3] = x[M // 3]
     assert torch.equal(bits(ops.gemm_mx4(other.cuda(), w, out=OUT_FP32).cpu()[M // 3]), bits(y[M // 3]))
+
+
+# ------------------------------------------------------------------------------------------------ few rows, the ways through w
+# Several loads of a wave's share of K to a tile of w, K ending inside the last one; waves without a share; a workgroup's second
+# tiles, with and without waves that share one; one, two and three groups of 16 rows.
+FEW = [(1, 80, 5120), (1, 64, 10336), (3, 6001, 5120), (16, 6000, 2560), (16, 9728, 2560), (16, 12288, 4096), (5, 2100, 5152), (17, 5120, 2560),
+       (24, 1000, 3616), (20, 70000, 1056), (2, 66000, 544), (33, 70000, 288), (37, 12288, 1536), (48, 300, 1568), (48, 200, 2560)]
+
+
+def few_case(M, N, K):
+    """Codes of sums that are whole quarters below 2^24 of them, in fp32 too; NaN in the last block of a row of each."""
+    g = torch.Generator().manual_seed(M + N + K)
+    x, w = random_codes(g, M, K), random_codes(g, N, K)
+    a, b = values_of(*x).float(), values_of(*w).float()
+    want = a @ b.T
+    w[1][N // 2, -1] = 255
+    want[:, N // 2] = math.nan
+    return x, w, a, want
+
+
+@pytest.mark.parametrize("M,N,K", FEW)
+def test_few_rows_of_a_long_k_and_of_many_columns(M, N, K):
+    x, w, _, want = few_case(M, N, K)
+    wd = dev(*w)
+    bias = (torch.arange(N) % 16 - 8).float()
+    got = ops.gemm_mx4(dev(*x), wd, bias=bias.cuda(), out=OUT_FP32).cpu()
+    assert torch.equal(torch.nan_to_num(got, nan=1e9), torch.nan_to_num(want + bias, nan=1e9))
+    x[1][M // 2, -1] = 255
+    want[M // 2] = math.nan
+    got = ops.gemm_mx4(dev(*x), wd, out=OUT_FP32).cpu()
+    assert torch.equal(torch.nan_to_num(got, nan=1e9), torch.nan_to_num(want, nan=1e9))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("M,N,K", [(1, 80, 5120), (16, 9728, 2560), (16, 1000, 5120), (17, 5120, 2560), (37, 12288, 1536), (48, 200, 2560)])
+def test_few_rows_quantised_by_the_product_itself(t, M, N, K):
+    """Values of four bits come back as themselves: a block whose largest is 3 or less has a smaller scale and the same values."""
+    _, w, a, want = few_case(M, N, K)
+    assert _lib.lib().tars_mx4_workspace(M, N, K, 1) == 0             # no launch before it
+    x = a.to(TYPES[t])
+    assert torch.equal(x.float(), a)
+    got = ops.gemm_mx4(x.cuda(), dev(*w), out=OUT_FP32).cpu()
+    assert torch.equal(torch.nan_to_num(got, nan=1e9), torch.nan_to_num(want, nan=1e9))
