@@ -58,10 +58,6 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 }
 __device__ __forceinline__ float value_of(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o); }
 __device__ __forceinline__ Key key_of(float x, uint32_t at) { return static_cast<Key>(ordered(x)) << 32 | static_cast<uint32_t>(~at); }
-__device__ __forceinline__ Key lane_key(Key k, int lane) {
-  return static_cast<Key>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(k >> 32), lane))) << 32 |
-         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(k), lane));
-}
 
 constexpr int kAtOnce = 4;                     // keys of a lane that are offered together
 constexpr int kRoom = (1 + kAtOnce) * kLanes;  // of a wave's list: 64 and what may be offered
@@ -457,7 +453,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void logprobs_kernel(LogprobArgs a)
 template <class X>
 __global__ __launch_bounds__(64 * kWaves) void logprobs_join_kernel(LogprobArgs a) {
   __shared__ Shared sh;
-  const int row = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int row = blockIdx.x, wave = threadIdx.x >> 6;
   const Given first = given_at<X>(a, row, threadIdx.x);
   Sums sums = Sums::none();
   for (int p = threadIdx.x; p < a.parts; p += 64 * kWaves) {

@@ -624,7 +624,7 @@ __global__ __launch_bounds__(128 * WN, 2) void mx4_tile_kernel(Mx4GemmArgs a, in
   static_assert(kWaves * 16 * kPitch * 4 <= D * kPair, "a wave's 16 rows fit");
   float* mine = reinterpret_cast<float*>(lds) + wave * 16 * kPitch;
   const auto store_columns = [&](auto out_) __attribute__((always_inline)) {
-    constexpr int out = decltype(out_)::value, e = out == 0 ? 4 : 2;
+    constexpr int out = decltype(out_)::value;
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const int thread = thread_again(), col = thread & 15, part = thread >> 4 & 3, lane = thread & 63;
