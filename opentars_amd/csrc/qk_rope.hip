@@ -157,7 +157,8 @@ template <class T, bool STORE, bool E4M3>
 hipError_t go(const QkRopeArgs& a, hipStream_t s) {
   const int l = a.hd / 16, all = a.heads + (STORE ? 2 : 1) * a.kv_heads;
   const int per_row = ceil_div(all, 64 / l);
-  const dim3 grid(ceil_div(static_cast<int64_t>(a.seqs.rows) * per_row, kThreads / 64)), block(kThreads);
+  // waves: at most 2^35 / 1024 elements' and one for each of 2^22 rows, and so below 2^32 threads
+  const dim3 grid(ceil_div(a.seqs.rows * per_row, kThreads / 64)), block(kThreads);
   if (l == 4) hipLaunchKernelGGL((qk_rope_kernel<T, 4, STORE, E4M3>), grid, block, 0, s, a, per_row);
   else if (l == 8) hipLaunchKernelGGL((qk_rope_kernel<T, 8, STORE, E4M3>), grid, block, 0, s, a, per_row);
   else hipLaunchKernelGGL((qk_rope_kernel<T, 16, STORE, E4M3>), grid, block, 0, s, a, per_row);
