@@ -342,8 +342,8 @@ typedef struct tars_kv_pool {
 
 /*
  * Stores the K and V rows ([rows, kv_heads * hd], BF16 or FP16, row strides ldk / ldv bytes, 0 =
- * dense) of new tokens at their positions; an E4M3 pool gets x / scale rounded to nearest even and
- * saturated (NaN kept). starts NULL: one row for each sequence (rows == seqs). Rows behind the last
+ * dense) of new tokens at their positions; an E4M3 pool gets x / scale as fp32, rounded to nearest even
+ * and saturated (NaN kept). starts NULL: one row for each sequence (rows == seqs). Rows behind the last
  * sequence, at negative positions or on pages outside the pool are not stored. No two rows may have
  * one slot (a table that names a shared page where a sequence writes), and the pools overlap no input and
  * not one another (they may interleave: the same strides, or extents that are apart).
@@ -416,8 +416,9 @@ int tars_qk_norm_rope(const void* q, int64_t ldq, const void* k, int64_t ldk, in
 /*
  * tars_qk_norm_rope with the keys going to their pages instead of yk, and the values beside them as they
  * are: tars_kv_append of keys that were never written in between (an E4M3 pool gets the fp32 key over its
- * scale, rounded once). The pool's kv_heads and hd are k's and v's; the rules on rows and pages are
- * tars_kv_append's, and of rows at positions that tab does not have neither key nor value is stored.
+ * scale as tars_kv_append rounds it, without a rounding to the rows' type before). The pool's kv_heads and
+ * hd are k's and v's; the rules on rows and pages are tars_kv_append's, and of rows at positions that tab
+ * does not have neither key nor value is stored.
  */
 int tars_kv_append_rope(const tars_kv_pool* pool, const void* q, int64_t ldq, const void* k, int64_t ldk,
                         const void* v, int64_t ldv, int32_t dtype, int32_t heads, int32_t rows,

@@ -13,8 +13,9 @@
 // place among the largest is the number of larger ones, counted over all lists at the end.
 //
 // A workgroup takes a row, or a part of one where there are few; a second launch joins the parts. 2048 rows of 151936 bf16 logits
-// take 123 us, 5.1 TB/s. Smaller calls are chains of latencies: of the 20 us of 61 rows with 20 alternatives the sums alone take
-// 10.5, the bound, the second look and the ranking the rest.
+// take 123 us, 5.1 TB/s. Smaller calls are chains of latencies (waves wait for half of their time, three quarters in the join): of
+// the 20 us of 61 rows with 20 alternatives the sums alone take 10.5, the bound, the second look and the ranking the rest, which
+// hardly goes by the size: 200 rows take 17.8 us without alternatives and 25.7 with five, one row 6.2 and 12.0.
 #include <algorithm>
 
 #include "kernels.h"

@@ -184,8 +184,11 @@ __device__ __forceinline__ int swap_of(int r) { return -(r >> 2) & 3; }
 // A wave takes tiles of 16 rows of w over its share of K; the kw waves that share a tile add theirs in LDS, in order. w comes by
 // direct loads into the wave's own two slots of four steps of 128 k: lanes that are neighbours then read neighbouring bytes of a
 // row (an operand's lanes are rows apart: read straight into it, 83 MB took 25 us, the loads' addresses what bounded it; so
-// 14.4, 5.7 TB/s). One slot is
-// loaded while the other is multiplied, the first one while x is quantised.
+// 14.4, 5.7 TB/s, and 16.5 where 20 such matrices take turns, which no cache holds). One slot is loaded while the other is
+// multiplied, the first one while x is quantised.
+//
+// Smaller products are chains of latencies, launch, x, the first slot, the next: 37 x 12288 x 1536 takes 7.6 us, one of them x's
+// quantising (6.5 with x in 4 bits), for 1.7 of bytes, and waves wait 61 % of their time.
 constexpr int kFewWaves = 8, kFewSteps = 4, kFewSlot = kFewSteps * 1024 + 256;
 
 template <class X, int MT>
@@ -227,7 +230,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void mx4_few_kernel(Mx4GemmArgs a, 
     asm volatile("" ::: "memory");
   };
   if (tile < tiles && first < end) issue(tile, first, 0);
-  // a block to a thread: 16 x 4096 x 4096 from bf16 takes 5.7 us (three of a thread's at once 6.8, four lanes to a block 8.8)
+  // a block to a thread: 16 x 4096 x 4096 from bf16 takes 5.7 us with weights that a cache holds (three of a thread's at once 6.8,
+  // four lanes to a block 8.8)
   for (int i = threadIdx.x; i < blocks * a.M; i += 64 * kFewWaves) {
     const int m = i / blocks, b = i - m * blocks;
     const Operand o = load_x<X>(a, m, b);
@@ -295,22 +299,28 @@ int64_t few_lds_bytes(int M, int K, int kw) {
   return 2 * kFewSlot * kFewWaves + (17ll * (K / 32) * M + 15) / 16 * 16 + (kw > 1 ? kFewWaves * 1024 * ceil_div(M, 16) : 0);
 }
 // Waves to a tile of w, for 2048 waves in all, or 1024 with more than 16 rows of x: 1 x 4096 x 4096 takes
-// 5.8, 4.4, 3.6 and 3.7 us with 512, 1024, 2048 and 4096 in all, 32 x 12288 x 4096 13.0, 10.3, 11.3 and 11.7.
+// 5.8, 4.4, 3.6 and 3.7 us with 512, 1024, 2048 and 4096 in all, 32 x 12288 x 4096 13.0, 10.3, 11.3 and 11.7. Both have 32 steps
+// of 128 k: with other numbers the shares are uneven (few()).
 int few_split(int M, int N, int K) {
   const int tiles = ceil_div(N, 16), steps = ceil_div(K, 128);
   int kw = 1;
   while (kw < kFewWaves && tiles * kw < (M <= 16 ? 2048 : 1024) && 2 * kw <= steps) kw *= 2;
   return kw;
 }
-// Up to 48 rows run this way: 48 x 2048 x 1024 takes 4.6 us either way, 32 x 4096 x 2048 5.1 us (tiles 5.8), 64 x 2048 x 1024
-// would take 5.4 (tiles 4.7).
+// Up to 48 rows run this way, as far as x fits: x in 4 bits, weights that no cache holds, 32 x 12288 x 4096 takes 11.5 us (tiles
+// 16.9), 32 x 4096 x 2048 5.6 (7.4), 48 x 4096 x 2560 7.4 (8.6), 48 x 2048 x 1024 4.6 (4.7), 48 x 12288 x 1536 7.1 (6.9); 64 x
+// 2048 x 1024 would take 5.4 (4.7). Many columns of a short K are faster as tiles before that: 20, 32 and 48 x 32000 x 2048 10.8,
+// 11.5 and 12.6 (11.6, 11.7 and 11.8). What does not fit runs as tiles: 16 x 4096 x 14336 14.9 us, 32 x 5120 x 5120 11.2,
+// 48 x 4096 x 4096 10.8, for 5.0, 2.3 and 1.5 of bytes.
 constexpr int kFewRows = 48;
 bool few_fits(int M, int N, int K) { return M <= kFewRows && few_lds_bytes(M, K, few_split(M, N, K)) <= kLds; }
 
 template <class X>
 hipError_t few(const Mx4GemmArgs& a, hipStream_t s) {
   const int kw = few_split(a.M, a.N, a.K), groups = ceil_div(ceil_div(a.N, 16), kFewWaves / kw), share = ceil_div(ceil_div(a.K, 128), kw);
-  const int per = share <= 2 ? share : ceil_div(share, kFewSteps) * kFewSteps;  // no slot's steps in two 16-byte pieces of scales
+  // No slot's steps in two 16-byte pieces of scales, for which the last waves of a tile may have less or nothing: of 40 steps in
+  // eight shares five take 8 each (16 x 5120 x 5120: 8.6 us).
+  const int per = share <= 2 ? share : ceil_div(share, kFewSteps) * kFewSteps;
   const int lds = static_cast<int>(few_lds_bytes(a.M, a.K, kw));
   const dim3 grid(std::min(groups, 256 * (kLds / lds))), block(64 * kFewWaves);
   if (a.M <= 16) hipLaunchKernelGGL((mx4_few_kernel<X, 1>), grid, block, lds, s, a, kw, per);
@@ -334,7 +344,9 @@ hipError_t few(const Mx4GemmArgs& a, hipStream_t s) {
 // Fragment j of w holds rows 64 (j / 4) + 16 (r / 4) + 4 (j % 4) + r % 4: the outputs of a lane's four neighbouring fragments
 // are then 16 neighbours of a row.
 //
-// 8192 x 8192 x 8192 takes 265 us, 4.1 PFLOP/s: the power limit, at which the same instructions alone reach 6.0 to 6.6.
+// 8192 x 8192 x 8192 takes 265 us, 4.1 PFLOP/s. The clock falls to 1.77 of 2.4 GHz under it, at which the matrix units are busy for
+// 53 % of the cycles: waves wait for loads and barriers a quarter of their time. Under the same instructions alone it falls to 1.6
+// GHz, and they are busy for 93 %: 6.0 to 6.6 PFLOP/s.
 //
 // The swap of a row's blocks: row r of a fragment, by lane r (and as swap_of, for rows of 128 bytes).
 __device__ __forceinline__ int x_swap(int row) { return row >> 1 & 7; }
@@ -686,12 +698,14 @@ hipError_t tiles(const Mx4GemmArgs& a, hipStream_t s, int splits = 1) {
 }
 
 // Tiles of 256 x 256, 128 x 128 or 64 x 128, and parts of K, by what they would take, in ns: a start, the stages in rounds that
-// fill the card, of which the last may leave CUs to fewer workgroups, and a second launch that joins the parts. Measured at
-// 8192 x 8192 x 8192 (265, 353 and 464 us) and, a workgroup to a CU or less, at 64 x 4096 x 4096 (23.6, 10.8 and 8.8 us);
-// 2011 x 12288 x 4096 takes 65, 73 and 93 us. In eight parts 100 x 1024 x 8192 takes 10.4 us for 17.9 (64 x 128 tiles), in two
-// 64 x 4096 x 4096 10.4 for 8.8, which is why the join counts. (Whole rounds of columns first and the rest in smaller tiles, by a
-// second launch, took 75 us where this takes 75 for 2011 x 12288 x 4096, 86 and 83 for 5000 x 5000 x 5120, 90 and 102 for 3000 x
-// 11008 x 4096: at the power limit a round half empty runs faster.)
+// fill the card, of which the last may leave CUs to fewer workgroups, and a second launch that joins the parts. A stage's times
+// are of 8192 x 8192 x 8192 (265, 353 and 464 us) and, a workgroup to a CU or less, of 64 x 4096 x 4096 (23.6, 10.8 and 8.8 us),
+// whose weights a cache held. 2011 x 12288 x 4096 takes 67, 72 and 92 us with such weights, 71, 77 and 110 with weights that none
+// holds. In eight parts 100 x 1024 x 8192 takes 10 us for 17.9 (64 x 128 tiles), in two 64 x 4096 x 4096 10.4 for 8.8, which is why
+// the join counts. Where few workgroups wait for memory the times are too short, and parts would be better than the rule has it:
+// 64 x 4096 x 4096 takes 12.0 us whole and 11.5 in two, 128 x 8192 x 8192 30.3 and 23.4 (21.4 and 19.2 out of a cache). (Whole
+// rounds of columns first and the rest in smaller tiles, by a second launch, took 75, 86 and 90 us where the rule took 75, 83 and
+// 102 on the same card, for 2011 x 12288 x 4096, 5000 x 5000 x 5120 and 3000 x 11008 x 4096.)
 struct TileChoice {
   int kind, splits;
 };

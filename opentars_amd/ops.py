@@ -924,8 +924,8 @@ def kv_append_rope(cache: PagedCache, q: torch.Tensor, k: torch.Tensor, v: torch
                    tab: torch.Tensor, starts: torch.Tensor | None = None, qgamma: torch.Tensor | None = None,
                    kgamma: torch.Tensor | None = None, eps: float = 1e-6, yq: torch.Tensor | None = None) -> torch.Tensor:
     """qk_norm_rope and kv_append in one pass: the keys, normed and rotated, and the values as they are go to the pages of their
-    sequences (an e4m3 pool gets the fp32 key over its scale, rounded once), and the queries come back, ready for
-    paged_attention or paged_decode. Arguments as theirs; a position that tab does not have is not stored either."""
+    sequences (an e4m3 pool gets the fp32 key over its scale, without a rounding to the rows' type before), and the queries come
+    back, ready for paged_attention or paged_decode. Arguments as theirs; a position that tab does not have is not stored either."""
     index, hd = cache.index, cache.hd
     code, rows, heads, ldq = _rope_rows(index, q, "q", hd)
     kcode, krows, kheads, ldk = _rope_rows(index, k, "k", hd)
